@@ -460,6 +460,56 @@ Q35_API int q35_kv_append(const void *k_new, const void *v_new, void *k_cache, v
                           int64_t B, int Hkv, int64_t S, int D, int64_t cap, int64_t offset,
                           q35_stream_t stream);
 
+/* ---- 4-bit KV cache -------------------------------------------------------
+ * A layer's keys and values held as 4-bit codes: codes uint8
+ * [B, Hkv, cap, D/2], scales bf16 [B, Hkv, cap, D/group, 2], one (scale s,
+ * minimum m) pair per group of 32, 64 or 128 consecutive channels (group <= D,
+ * D in {32, 64, 128}).  For a group with minimum m and maximum M:
+ *   s = bf16((M - m) / 15), c = min(15, rint((x - m) / s)), value = m + c s
+ * (codes 0 where s = 0; a group holding a NaN or an infinity reads back NaN).
+ * As 32-bit words, word t * (D/32) + j of a row holds channels 32 j + 8 t + e
+ * (e = 0..7), channel e in the 4-bit field e/2 + 4 * (e % 2), field 0 lowest.
+ * cap is a multiple of 16; all pointers are 16-byte aligned.  At D = 128 a key
+ * and its value take 160, 144 or 136 bytes (group 32, 64, 128), 512 in bf16.
+ * Rows no call has written may hold anything.  No reference counterpart: the
+ * reference keeps K/V in the activations' type (REF modules/attention.py:89-93).
+ *
+ * Append: rows s < S of k_new / v_new (bf16, [B, Hkv, S, D] addressed by the
+ * element strides {batch, head, position}, multiples of 8; channels contiguous)
+ * go to rows offset + s, or offsets[b] + s when offsets (device int32 [B]) is
+ * not NULL.  A row outside [0, cap) is left out and recorded as a device error
+ * (code 2, site 105).                                                       */
+Q35_API int q35_kv_append_q4(const void *k_new, const void *v_new, const int64_t *k_strides,
+                             const int64_t *v_strides, void *k_codes, void *k_scales,
+                             void *v_codes, void *v_scales, int64_t B, int Hkv, int64_t S, int D,
+                             int group, int64_t cap, int64_t offset, const int32_t *offsets,
+                             q35_stream_t stream);
+
+/* Read back: rows start .. start + n (starts[b] .. when starts is not NULL) as
+ * bf16 k_out / v_out [B, Hkv, out_cap, D], out_cap >= n; rows n .. out_cap are
+ * set to zero.  A row outside [0, cap) reads as zero and is recorded as a device
+ * error (code 2, site 106).                                                 */
+Q35_API int q35_kv_read_q4(const void *k_codes, const void *k_scales, const void *v_codes,
+                           const void *v_scales, void *k_out, void *v_out, int64_t B, int Hkv,
+                           int64_t n, int64_t out_cap, int D, int group, int64_t cap,
+                           int64_t start, const int32_t *starts, q35_stream_t stream);
+
+/* Attention over the first kv_len rows (kv_lens[b] <= kv_len rows of sequence b
+ * when kv_lens, device int32 [B], is not NULL): q bf16 [B, Hq, Sq, D], out bf16
+ * token-major [B, Sq, Hq*D], any Hq/Hkv and Sq.  Meant for few query rows per
+ * kv head (a decode step, drafted tokens); for a chunk of a prompt read the rows
+ * back and call q35_attn_prefill_cache_fwd.  causal != 0: query s sees keys
+ * <= s + len - Sq.  A query that sees no key gives zeros.  A kv_lens entry
+ * outside [0, kv_len] is clamped and recorded as a device error (code 2, site
+ * 311).  workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.      */
+Q35_API int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
+                                      int D);
+Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_scales,
+                            const void *v_codes, const void *v_scales, void *out, int64_t B,
+                            int Hq, int Hkv, int64_t Sq, int64_t kv_len, const int32_t *kv_lens,
+                            int64_t cap, int D, int group, float scale, int causal,
+                            float *workspace, q35_stream_t stream);
+
 /* ---- Vision-tower operators (bf16, fp32 math) -------------------------- */
 /* LayerNorm over the last dim: (x - mean) * rsqrt(var + eps) * w (+ b); b may
  * be NULL.  cols % 8 == 0.  Replaces layernorm_forward

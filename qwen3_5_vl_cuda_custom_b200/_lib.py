@@ -115,6 +115,16 @@ _SIGS = {
     "q35_attn_decode_workspace": (c_int64, [c_int64, c_int, c_int64, c_int64, c_int]),
     "q35_attn_decode_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int,
                                     c_int64, c_int64, c_int, c_float, c_void_p, c_void_p]),
+    "q35_kv_append_q4": (c_int, [c_void_p, c_void_p, POINTER(c_int64), POINTER(c_int64), c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_int, c_int,
+                                 c_int64, c_int64, c_void_p, c_void_p]),
+    "q35_kv_read_q4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                               c_int, c_int64, c_int64, c_int, c_int, c_int64, c_int64, c_void_p,
+                               c_void_p]),
+    "q35_attn_q4_workspace": (c_int64, [c_int64, c_int, c_int, c_int64, c_int64, c_int]),
+    "q35_attn_q4_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                c_int, c_int, c_int64, c_int64, c_void_p, c_int64, c_int, c_int,
+                                c_float, c_int, c_void_p, c_void_p]),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -167,3 +177,8 @@ def device_error_check() -> tuple[int, int, int, int]:
 def sections_arg(sections) -> ctypes.Array:
     arr = (ctypes.c_int32 * 3)(*[int(s) for s in sections])
     return arr
+
+
+def strides_arg(t) -> ctypes.Array:
+    """Element strides of all dims but the last of a 4-D tensor, as int64[3]."""
+    return (c_int64 * 3)(*t.stride()[:3])

@@ -1,0 +1,61 @@
+// The stored form of a 4-bit KV cache, shared by the kernels that write it,
+// read it back and attend over it.
+//
+// A row of D channels (D = 32, 64 or 128) is D/8 32-bit words of eight 4-bit
+// codes and D/group (scale, minimum) pairs of bf16, the scale in the low half
+// of a 32-bit word.  Word t * (D/32) + j (t = 0..3) holds channels
+// 32 j + 8 t + e, e = 0..7, channel e in field e/2 + 4 * (e & 1).
+//
+// Why this order: a matrix instruction wants its operands as pairs of
+// neighbouring values along the summed axis.  With channel 2i in field i and
+// channel 2i + 1 in field i + 4, `(w >> 4i) & 0x000f000f` is the pair
+// (2i, 2i + 1), and OR-ing 0x43004300 makes it the bf16 pair (128 + c, 128 + c')
+// exactly: one shift and one logic operation per two codes.  The words of a
+// thread quarter t are contiguous, so the four threads that share a key read
+// 16 bytes each (D = 128).
+#pragma once
+
+#include "common.cuh"
+
+namespace q35 {
+namespace q4 {
+
+// Device arrays of one layer's cache: codes [B, Hkv, cap, D/2] bytes, scales
+// [B, Hkv, cap, D/group] (scale, minimum) words.
+struct Cache {
+  uint32_t *k_codes, *k_scales, *v_codes, *v_scales;
+};
+
+// Host-side checks that every entry point over a cache shares.
+inline int check_cache(const char *what, const void *kc, const void *ks, const void *vc,
+                       const void *vs, int64_t B, int Hkv, int D, int group, int64_t cap) {
+  if (D != 32 && D != 64 && D != 128)
+    return fail(Q35_ERR_UNSUPPORTED, "%s: head_dim %d (32, 64 or 128)", what, D);
+  if ((group != 32 && group != 64 && group != 128) || group > D)
+    return fail(Q35_ERR_UNSUPPORTED, "%s: group %d (32, 64 or 128, at most head_dim %d)", what,
+                group, D);
+  if (B < 0 || Hkv <= 0 || cap < 0 || cap % 16 != 0)
+    return fail(Q35_ERR_SHAPE, "%s: B %lld, Hkv %d, capacity %lld (a multiple of 16)", what,
+                (long long)B, Hkv, (long long)cap);
+  if (cap >= (int64_t(1) << 31) - 256)
+    return fail(Q35_ERR_SHAPE, "%s: capacity %lld does not fit 31 bits", what, (long long)cap);
+  if (B * Hkv * cap == 0) return Q35_OK;
+  if (!kc || !ks || !vc || !vs) return fail(Q35_ERR_INVALID, "%s: null cache pointer", what);
+  if (!aligned16(kc) || !aligned16(ks) || !aligned16(vc) || !aligned16(vs))
+    return fail(Q35_ERR_ALIGN, "%s: cache pointers not 16-byte aligned", what);
+  return Q35_OK;
+}
+
+// value = minimum + code * scale, rounded once to fp32 (code * scale is exact:
+// 4 x 8 significant bits).
+__device__ __forceinline__ float value(uint32_t code, uint32_t pair) {
+  return fmaf(static_cast<float>(code), __uint_as_float(pair << 16),
+              __uint_as_float(pair & 0xffff0000u));
+}
+// Code of channel e of a word.
+__device__ __forceinline__ uint32_t code_of(uint32_t word, int e) {
+  return (word >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u;
+}
+
+}  // namespace q4
+}  // namespace q35

@@ -18,7 +18,10 @@ fixed length: a replay rewrites the same positions and does NOT advance
 ``cache.length``.  The cache length is restored after the warm-up and the
 capture, so the cache reads as it did before construction.  This suits a
 fixed-position step (a benchmark); a decode loop needs one capture per
-position, or the eager module.
+position, or the eager module.  A ``Q4LayerKVCache`` with per-sequence lengths
+(``set_lengths``) keeps them on the device: each replay appends behind them and
+advances them, so one capture serves a whole decode loop (advance
+``static_pos`` between replays).
 """
 from __future__ import annotations
 
@@ -40,23 +43,23 @@ class GraphedDecoderLayer:
             raise RuntimeError("GraphedDecoderLayer captures one layer: pass that layer's "
                                "LayerKVCache, not the model's KVCache")
         self.past_kv = past_kv
-        length0 = past_kv.length if isinstance(past_kv, LayerKVCache) else None
+        length0 = past_kv.save_length() if isinstance(past_kv, LayerKVCache) else None
         bound = rotary.bind(self.static_pos)
         side = torch.cuda.Stream(device=example_x.device)
         side.wait_stream(torch.cuda.current_stream(example_x.device))
         with torch.no_grad(), torch.cuda.stream(side):
             for _ in range(warmup):  # caches (fused weights, TMA attributes) filled outside capture
                 if length0 is not None:
-                    past_kv.length = length0
+                    past_kv.restore_length(length0)
                 layer(self.static_x, bound, past_kv=past_kv)
         torch.cuda.current_stream(example_x.device).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
         if length0 is not None:
-            past_kv.length = length0
+            past_kv.restore_length(length0)
         with torch.no_grad(), torch.cuda.graph(self.graph):
             self.static_out = layer(self.static_x, bound, past_kv=past_kv)
         if length0 is not None:
-            past_kv.length = length0
+            past_kv.restore_length(length0)
 
     def replay(self):
         """Replays the captured forward on the current static input."""

@@ -555,6 +555,158 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
                   B, Hkv, S, D, k_cache.shape[2], offset, _stream(k))
 
 
+# ---------------------------------------------------------------- 4-bit KV cache
+def _cache_q4(name: str, k_codes, k_scales, v_codes, v_scales) -> tuple[int, int, int, int, int]:
+    """Checks the four tensors of a 4-bit cache; returns (B, Hkv, capacity, D, group)."""
+    for t, part, dt, dims in ((k_codes, "k_codes", torch.uint8, 4), (k_scales, "k_scales", _BF16, 5),
+                              (v_codes, "v_codes", torch.uint8, 4), (v_scales, "v_scales", _BF16, 5)):
+        _require(t, f"{name}.{part}", dt)
+        if t.dim() != dims or not t.is_contiguous():
+            raise RuntimeError(f"{name}: {part} must be contiguous with {dims} dims (it is used in place)")
+        if t.device != k_codes.device:
+            raise RuntimeError(f"{name}: the cache's tensors are on different devices")
+    B, Hkv, cap, half = k_codes.shape
+    D, groups = 2 * half, k_scales.shape[3]
+    if D not in (32, 64, 128) or groups == 0 or D % groups:
+        raise RuntimeError(f"{name}: codes {tuple(k_codes.shape)} and scales {tuple(k_scales.shape)} "
+                           "do not belong to a head_dim of 32, 64 or 128")
+    if (v_codes.shape != k_codes.shape or v_scales.shape != k_scales.shape
+            or tuple(k_scales.shape) != (B, Hkv, cap, groups, 2)):
+        raise RuntimeError(f"{name}: shapes {tuple(k_codes.shape)}, {tuple(k_scales.shape)}, "
+                           f"{tuple(v_codes.shape)}, {tuple(v_scales.shape)} do not match")
+    return B, Hkv, cap, D, D // groups
+
+
+def _per_sequence(t: torch.Tensor, name: str, B: int, device) -> torch.Tensor:
+    t = _require(t, name, torch.int32)
+    if t.shape != (B,) or t.device != device:
+        raise RuntimeError(f"{name}: expected {B} int32 values on {device}")
+    return t
+
+
+def _same_device(t: torch.Tensor, name: str, device) -> torch.Tensor:
+    if t.device != device:
+        raise RuntimeError(f"{name}: on {t.device}, the cache is on {device}")
+    return t
+
+
+def _strided_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """t [B, Hkv, S, D] as the append kernel can address it: contiguous channels,
+    16-byte aligned rows (a transposed view of a token-major tensor needs no copy)."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 4:
+        raise TypeError(f"{name}: expected a 4-D tensor")
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:3])
+    if ok and t.is_cuda and t.dtype == _BF16:
+        return t
+    t = _require(t, name)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
+                 v_codes: torch.Tensor, v_scales: torch.Tensor, offset) -> None:
+    """Stores k/v (B,Hkv,S,D) bf16 in rows [offset, offset+S) of a 4-bit cache in
+    place.  The cache is k_codes/v_codes uint8 (B,Hkv,capacity,D/2) and
+    k_scales/v_scales bf16 (B,Hkv,capacity,D/group,2), one (scale s, minimum m)
+    pair per group of 32, 64 or 128 channels: a value is m + code * s with
+    s = bf16((max - m) / 15) and the nearest code (code order in q35b200.h).  A
+    group that holds a NaN or an infinity reads back as NaN.
+
+    ``offset`` is an int, or an int32 (B,) tensor on the cache's device with a
+    row per sequence (no host synchronisation); a row outside the cache is left
+    out and recorded as a device error.  k and v may be strided views."""
+    B, Hkv, cap, D, group = _cache_q4("kv_append_q4", k_codes, k_scales, v_codes, v_scales)
+    dev = k_codes.device
+    k = _same_device(_strided_rows(k, "kv_append_q4.k"), "kv_append_q4.k", dev)
+    v = _same_device(_strided_rows(v, "kv_append_q4.v"), "kv_append_q4.v", dev)
+    S = k.shape[2]
+    if tuple(k.shape) != (B, Hkv, S, D) or v.shape != k.shape:
+        raise RuntimeError(f"kv_append_q4: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of "
+                           f"{(B, Hkv, cap, D)}")
+    rows = _per_sequence(offset, "kv_append_q4.offset", B, dev) if isinstance(offset, torch.Tensor) else None
+    with torch.cuda.device(dev):
+        _lib.call("q35_kv_append_q4", k.data_ptr(), v.data_ptr(), _lib.strides_arg(k),
+                  _lib.strides_arg(v), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                  v_scales.data_ptr(), B, Hkv, S, D, group, cap, 0 if rows is not None else int(offset),
+                  _ptr(rows), _stream(k_codes))
+
+
+def _read_q4(cache, shape, start: int, starts, n: int, out_cap: int):
+    B, Hkv, cap, D, group = shape
+    dev = cache[0].device
+    k = torch.empty(B, Hkv, out_cap, D, device=dev, dtype=_BF16)
+    v = torch.empty_like(k)
+    with torch.cuda.device(dev):
+        _lib.call("q35_kv_read_q4", *[t.data_ptr() for t in cache], k.data_ptr(), v.data_ptr(), B, Hkv,
+                  n, out_cap, D, group, cap, start, _ptr(starts), _stream(cache[0]))
+    return k, v
+
+
+def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+               v_scales: torch.Tensor, start, length: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows [start, start+length) of a 4-bit cache (kv_append_q4) as bf16 k, v
+    (B,Hkv,length,D), each value rounded once.  ``start`` is an int or an int32
+    (B,) device tensor; a row outside the cache reads as zero and is recorded as
+    a device error."""
+    cache = (k_codes, k_scales, v_codes, v_scales)
+    shape = _cache_q4("kv_read_q4", *cache)
+    starts = (_per_sequence(start, "kv_read_q4.start", shape[0], k_codes.device)
+              if isinstance(start, torch.Tensor) else None)
+    return _read_q4(cache, shape, 0 if starts is not None else int(start), starts, int(length), int(length))
+
+
+# Query rows per kv head from which attention_cache_q4 reads the rows back and
+# runs the bf16 prefill kernel instead of attending over the codes.
+_Q4_PREFILL_ROWS = 256
+
+
+def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
+                       v_codes: torch.Tensor, v_scales: torch.Tensor, kv_len, scale: float,
+                       causal: bool, max_kv_len: int | None = None) -> torch.Tensor:
+    """attention_cache over the first ``kv_len`` rows of a 4-bit cache
+    (kv_append_q4): q (B,Hq,Sq,D) bf16, returns the token-major (B,Sq,Hq*D).
+
+    ``kv_len`` is an int, or an int32 (B,) tensor on the cache's device with a
+    length per sequence, at most ``max_kv_len`` (the capacity if not given); it
+    is read on the device, so such a call can be captured once and replayed as
+    the lengths grow.  Causal masking is aligned to each sequence's last row; a
+    query that sees no row gives zeros.  Decode-shaped calls run on the codes;
+    with an int ``kv_len`` a chunk of a prompt reads the rows back into a
+    temporary bf16 copy and runs the prefill kernel."""
+    cache = (k_codes, k_scales, v_codes, v_scales)
+    shape = _cache_q4("attention_cache_q4", *cache)
+    B, Hkv, cap, D, group = shape
+    q = _same_device(_require(q, "attention_cache_q4.q"), "attention_cache_q4.q", k_codes.device)
+    if q.data_ptr() % 16:
+        q = q.clone()
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[1] % Hkv:
+        raise RuntimeError(f"attention_cache_q4: q {tuple(q.shape)} for a cache of {(B, Hkv, cap, D)}")
+    Hq, Sq = q.shape[1], q.shape[2]
+    lens = None
+    if isinstance(kv_len, torch.Tensor):
+        lens = _per_sequence(kv_len, "attention_cache_q4.kv_len", B, q.device)
+        n = cap if max_kv_len is None else int(max_kv_len)
+    else:
+        n = int(kv_len)
+    if n < 0 or n > cap:
+        raise RuntimeError(f"attention_cache_q4: {n} rows exceed the capacity {cap}")
+    out = torch.empty(B, Sq, Hq * D, device=q.device, dtype=q.dtype)
+    with torch.cuda.device(q.device):
+        if lens is None and (Hq // Hkv) * Sq >= _Q4_PREFILL_ROWS and n > 0:
+            # whole key tiles, zero-filled: the prefill kernel reads (and masks) to the end of one
+            pad = -(-n // 128) * 128
+            k, v = _read_q4(cache, shape, 0, None, n, pad)
+            _lib.call("q35_attn_prefill_cache_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                      out.data_ptr(), None, B, Hq, Hkv, Sq, n, pad, D, float(scale),
+                      1 if causal else 0, _stream(q))
+        else:
+            w = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, n, D)
+            ws = torch.empty(max(1, w), device=q.device, dtype=torch.float32)
+            _lib.call("q35_attn_q4_fwd", q.data_ptr(), *[t.data_ptr() for t in cache], out.data_ptr(),
+                      B, Hq, Hkv, Sq, n, _ptr(lens), cap, D, group, float(scale), 1 if causal else 0,
+                      ws.data_ptr(), _stream(q))
+    return out
+
+
 def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
                     is_causal: bool = True, num_kv_groups: int = 1) -> torch.Tensor:
     """Reference op signature (REF kernels/flash_attention.py:82-100): returns
@@ -637,6 +789,7 @@ __all__ = [
     "rmsnorm", "matmul", "softmax", "cuda_topk", "cuda_index_add", "swiglu", "residual_add",
     "router_topk", "router_split_weights", "pack_b_tiles", "embedding", "moe_permute", "moe_permute_slabs", "moe_permute_counted", "router_fused_supported", "Permutation", "gather_rows", "grouped_gateup_swiglu",
     "grouped_down", "moe_combine", "qknorm_mrope", "mrope", "attention_tokens",
-    "flash_attention", "attention_cache", "kv_append", "device_error_check", "default_scale",
+    "flash_attention", "attention_cache", "kv_append", "kv_append_q4", "kv_read_q4",
+    "attention_cache_q4", "device_error_check", "default_scale",
     "layernorm", "gelu_tanh", "apply_rope", "conv3d_patch",
 ]

@@ -14,7 +14,7 @@ import torch
 from torch import nn
 
 from .configs import MoETextConfig, Qwen3VLConfig
-from .kv_cache import KVCache
+from .kv_cache import KVCache, LayerKVCache, Q4KVCache
 from .modules import CudaEmbedding, CudaLinear, CudaRMSNorm, CudaTextDecoderLayer, TextMRoPE
 
 
@@ -26,6 +26,22 @@ def _layer_uses_moe(cfg: MoETextConfig, layer_idx: int) -> bool:
     if layer_idx in cfg.mlp_only_layers:
         return False
     return ((layer_idx + 1) % cfg.decoder_sparse_step) == 0
+
+
+def _next_positions(past_key_values, B: int, S: int, device) -> torch.Tensor:
+    """(3, B, S) text positions behind the rows that ``past_key_values`` holds
+    (each sequence's own, for a cache with per-sequence lengths)."""
+    pos = torch.arange(S, device=device).unsqueeze(0)
+    if past_key_values:
+        past = past_key_values[0]
+        if not isinstance(past, LayerKVCache):
+            pos = pos + past[0].shape[2]
+        elif past.lengths is None:
+            pos = pos + past.length
+        else:
+            pos = pos + past.lengths.long().unsqueeze(1)
+    pos = pos.expand(B, S)
+    return torch.stack([pos, pos, pos], dim=0)
 
 
 class CudaQwen3VLMoeModel(nn.Module):
@@ -91,10 +107,7 @@ class CudaQwen3VLMoeModel(nn.Module):
             inputs_embeds[image_token_mask] = feats.to(inputs_embeds.dtype)
         B, S = inputs_embeds.shape[:2]
         if position_ids is None:
-            past_len = past_key_values[0][0].shape[2] if past_key_values else 0
-            pos = torch.arange(past_len, past_len + S, device=inputs_embeds.device)
-            pos = pos.unsqueeze(0).expand(B, S)
-            position_ids = torch.stack([pos, pos, pos], dim=0)
+            position_ids = _next_positions(past_key_values, B, S, inputs_embeds.device)
         hidden, router_logits, new_kvs = self._text_forward(inputs_embeds, position_ids,
                                                             past_key_values=past_key_values)
         logits = self.lm_head(hidden)
@@ -102,11 +115,19 @@ class CudaQwen3VLMoeModel(nn.Module):
             return logits, router_logits, new_kvs
         return logits, router_logits
 
-    def make_kv_cache(self, batch: int, capacity: int, device=None) -> KVCache:
-        """A zeroed ``KVCache`` for every layer of this model (bf16)."""
+    def make_kv_cache(self, batch: int, capacity: int, device=None, bits: int = 16,
+                      group_size: int = 32) -> KVCache:
+        """A zeroed ``KVCache`` for every layer of this model: bf16, or with
+        ``bits=4`` a ``Q4KVCache`` (4-bit codes, a scale and minimum per
+        ``group_size`` channels)."""
         t = self.cfg.text
         device = device or self.embed_tokens.weight.device
-        return KVCache(len(self.layers), batch, t.num_kv_heads, capacity, t.head_dim, device)
+        shape = (len(self.layers), batch, t.num_kv_heads, capacity, t.head_dim, device)
+        if bits == 4:
+            return Q4KVCache(*shape, group_size=group_size)
+        if bits != 16:
+            raise ValueError(f"a KV cache holds 16 or 4 bits a value, not {bits}")
+        return KVCache(*shape)
 
     def _last_logits(self, input_ids: torch.Tensor, cache) -> torch.Tensor:
         """Logits of the last position only (B, vocab): the forward of
@@ -114,9 +135,7 @@ class CudaQwen3VLMoeModel(nn.Module):
         the last hidden row instead of all of them."""
         B, S = input_ids.shape
         emb = self.embed_tokens(input_ids)
-        past_len = cache.length if cache is not None else 0
-        pos = torch.arange(past_len, past_len + S, device=emb.device).unsqueeze(0).expand(B, S)
-        hidden, _, _ = self._text_forward(emb, torch.stack([pos, pos, pos], dim=0),
+        hidden, _, _ = self._text_forward(emb, _next_positions(cache, B, S, emb.device),
                                           past_key_values=cache)
         return self.lm_head(hidden[:, -1:].contiguous())[:, 0]
 

@@ -261,13 +261,11 @@ class CudaFullAttention(nn.Module):
         if isinstance(past_kv, LayerKVCache):
             # preallocated cache: append in place, attend over the buffers
             cache = past_kv
-            Sk = cache.length + S
-            if Sk > cache.capacity:
-                raise RuntimeError(f"KV cache full: {cache.length} + {S} > {cache.capacity}")
-            K.kv_append(k, v, cache.k, cache.v, cache.length)
-            causal = (S == Sk) if self.reference_chunk_mask else S > 1
-            out = K.attention_cache(q, cache.k, cache.v, Sk, self.scale, causal)
-            cache.length = Sk
+            if self.reference_chunk_mask:
+                causal = cache.lengths is None and cache.length == 0
+            else:
+                causal = S > 1
+            out = cache.append_attend(q, k, v, self.scale, causal)
             return self.o_proj(out, residual=residual, out_dtype=out_dtype), cache
         if past_kv is not None:
             past_k, past_v = past_kv

@@ -1,0 +1,570 @@
+"""The 4-bit KV cache on the GPU against its definition in 64 bits: storing
+rows, reading them back, attention over them, and the layer, model and captured
+step that use them."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kv_q4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+SHAPES = [(32, 32), (64, 32), (64, 64), (128, 32), (128, 64), (128, 128)]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _ready():
+    from qwen3_5_vl_cuda_custom_b200 import build
+    build.build()
+    yield
+    from qwen3_5_vl_cuda_custom_b200 import kernels as K
+    K.device_error_check()
+
+
+def K():
+    from qwen3_5_vl_cuda_custom_b200 import kernels
+    return kernels
+
+
+def rows(shape, seed, scale=1.0):
+    """bf16 rows with a channel profile and a few wide channels, as keys have."""
+    g = torch.Generator().manual_seed(seed)
+    p = torch.exp(0.4 * torch.randn(1, shape[1], 1, shape[-1], generator=g))
+    p[..., ::29] *= 4
+    return (torch.randn(shape, generator=g) * p * scale).bfloat16()
+
+
+def empty_cache(B, Hkv, cap, D, group, fill=0):
+    mk = lambda *s, dt: torch.full(s, fill, dtype=torch.uint8, device=DEV).view(dt)
+    return (mk(B, Hkv, cap, D // 2, dt=torch.uint8), mk(B, Hkv, cap, D // group, 4, dt=torch.bfloat16),
+            mk(B, Hkv, cap, D // 2, dt=torch.uint8), mk(B, Hkv, cap, D // group, 4, dt=torch.bfloat16))
+
+
+def filled_cache(B, Hkv, cap, D, group, seed, scale=1.0):
+    """A cache with every row stored, and its float64 k, v values."""
+    out, vals = [], []
+    for i in range(2):
+        c, s, m = R.quantise(rows((B, Hkv, cap, D), seed + i, scale), group)
+        codes = R.pack(c)
+        sm = torch.from_numpy(np.stack([s, m], -1)).bfloat16()
+        out += [codes.to(DEV), sm.to(DEV)]
+        vals.append(R.values(codes, sm))
+    return tuple(out), vals[0], vals[1]
+
+
+def check_stored(codes, scales, x, group):
+    """Stored rows are exactly the 64-bit definition of x."""
+    c, s, m = R.quantise(x, group)
+    assert torch.equal(codes.cpu(), R.pack(c))
+    want = torch.from_numpy(np.stack([s, m], -1))
+    assert torch.equal(torch.nan_to_num(scales.double().cpu(), nan=-77.0),
+                       torch.nan_to_num(want, nan=-77.0))
+
+
+# ------------------------------------------------------------------ storing
+@pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("B,Hkv,S,cap,offset", [(1, 1, 1, 16, 0), (2, 3, 37, 64, 11), (5, 2, 1, 48, 47)])
+def test_append_is_the_definition(D, group, B, Hkv, S, cap, offset):
+    k, v = rows((B, Hkv, S, D), 1), rows((B, Hkv, S, D), 2, 3e-3)
+    cache = empty_cache(B, Hkv, cap, D, group, fill=0x5A)
+    before = [t.clone() for t in cache]
+    K().kv_append_q4(k.to(DEV), v.to(DEV), *cache, offset)
+    w = slice(offset, offset + S)
+    check_stored(cache[0][:, :, w], cache[1][:, :, w], k, group)
+    check_stored(cache[2][:, :, w], cache[3][:, :, w], v, group)
+    for t, old in zip(cache, before):  # other rows are left as they were
+        t, old = t.view(torch.uint8), old.view(torch.uint8)
+        assert torch.equal(t[:, :, :offset], old[:, :, :offset])
+        assert torch.equal(t[:, :, offset + S:], old[:, :, offset + S:])
+
+
+@pytest.mark.parametrize("name", ["ties", "borders", "wide", "tiny", "subnormal", "huge", "constant",
+                                  "signed_zero", "steps", "nonfinite"])
+def test_append_where_rounding_is_delicate(name):
+    """Groups whose codes or scales lie on (or a hair beside) a border, groups at
+    both ends of bf16's range, and groups that hold a NaN or an infinity."""
+    g = torch.Generator().manual_seed(3)
+    B, Hkv, S, D, group = 2, 2, 64, 128, 32
+    x = torch.randn(B, Hkv, S, D, generator=g)
+    if name == "ties":  # s a power of two, every half step present
+        x = torch.randint(0, 31, x.shape, generator=g) * 0.5
+        x[..., 0::32], x[..., 1::32] = 0, 15
+    elif name == "borders":  # the same beside a minimum that is almost 0
+        x = torch.randint(0, 31, x.shape, generator=g) * 0.5
+        x[..., 0::32], x[..., 1::32] = -1e-5, 15
+    elif name == "wide":  # (x - m) needs more than 24 bits
+        x = x.sign() * torch.exp(12 * torch.randn(x.shape, generator=g))
+    elif name == "tiny":
+        x = x * 1e-33
+    elif name == "subnormal":
+        x = x * 3e-39
+    elif name == "huge":
+        x = x.clamp(-3, 3) * 1e38
+    elif name == "constant":
+        x = x[..., :1].expand(B, Hkv, S, D)
+    elif name == "signed_zero":
+        x = torch.where(x > 0, 0.0, -0.0)
+    elif name == "steps":  # differences of few bits: quotients near many borders
+        x = torch.randint(-127, 128, x.shape, generator=g).float()
+    elif name == "nonfinite":
+        x[0, 0, :, 5], x[0, 1, ::2, 40], x[1, 0, 3, 127] = math.nan, math.inf, -math.inf
+    x = x.bfloat16().contiguous()
+    cache = empty_cache(B, Hkv, S, D, group)
+    K().kv_append_q4(x.to(DEV), x.flip(2).to(DEV), *cache, 0)
+    check_stored(cache[0], cache[1], x, group)
+    check_stored(cache[2], cache[3], x.flip(2), group)
+
+
+def test_append_takes_strided_rows_and_per_sequence_offsets():
+    B, Hkv, S, D, cap = 3, 4, 5, 64, 64
+    k = rows((B, S, Hkv, D), 5).to(DEV).transpose(1, 2)  # token-major, no copy
+    v = rows((B, Hkv, S + 2, 2 * D), 6).to(DEV)[:, :, 1:S + 1, D:]
+    odd = torch.empty(B * Hkv * S * D + 1, dtype=torch.bfloat16, device=DEV)[1:].view(B, Hkv, S, D)
+    odd.copy_(v)  # 2-byte aligned only
+    cache, other = empty_cache(B, Hkv, cap, D, 32), empty_cache(B, Hkv, cap, D, 32)
+    off = torch.tensor([0, 59, 17], dtype=torch.int32, device=DEV)
+    K().kv_append_q4(k, v, *cache, off)
+    K().kv_append_q4(k.contiguous(), odd, *other, off)
+    for b, o in enumerate(off.tolist()):
+        check_stored(cache[0][b, :, o:o + S], cache[1][b, :, o:o + S], k[b].cpu(), 32)
+        check_stored(cache[2][b, :, o:o + S], cache[3][b, :, o:o + S], v[b].cpu(), 32)
+    for a, b in zip(cache, other):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_rows_outside_the_cache_are_left_out_and_reported():
+    B, Hkv, S, D, cap = 3, 2, 4, 64, 16
+    k = rows((B, Hkv, S, D), 7).to(DEV)
+    cache = empty_cache(B, Hkv, cap, D, 64)
+    K().kv_append_q4(k, k, *cache, torch.tensor([-2, 14, 3], dtype=torch.int32, device=DEV))
+    with pytest.raises(RuntimeError, match="code 2 at site 105"):
+        K().device_error_check()
+    for b, lo, hi, skip in ((0, 0, 2, 2), (1, 14, 16, 0), (2, 3, 7, 0)):
+        check_stored(cache[0][b, :, lo:hi], cache[1][b, :, lo:hi], k[b, :, skip:skip + hi - lo].cpu(), 64)
+        rest = torch.ones(cap, dtype=torch.bool)
+        rest[lo:hi] = False
+        assert not cache[0][b][:, rest].any() and not cache[3][b][:, rest].any()
+    kr, _ = K().kv_read_q4(*cache, torch.tensor([-1, 14, 3], dtype=torch.int32, device=DEV), 4)
+    with pytest.raises(RuntimeError, match="code 2 at site 106"):
+        K().device_error_check()
+    assert not kr[0, :, 0].any() and not kr[1, :, 2:].any() and kr[2].any()
+    q = rows((B, 4, 1, D), 8).to(DEV)
+    got = K().attention_cache_q4(q, *cache, torch.tensor([17, -1, 16], dtype=torch.int32, device=DEV),
+                                 0.125, False)
+    with pytest.raises(RuntimeError, match="code 2 at site 311"):
+        K().device_error_check()
+    want = K().attention_cache_q4(q, *cache, torch.tensor([16, 0, 16], dtype=torch.int32, device=DEV),
+                                  0.125, False)
+    assert torch.equal(got, want) and not got[1].any()
+
+
+# ------------------------------------------------------------------ reading back
+@pytest.mark.parametrize("D,group", SHAPES)
+def test_read_rounds_each_value_once(D, group):
+    B, Hkv, cap = 2, 3, 80
+    cache, kv, vv = filled_cache(B, Hkv, cap, D, group, 11)
+    for start, n in ((0, cap), (13, 1), (79, 1), (5, 66), (40, 0)):
+        k, v = K().kv_read_q4(*cache, start, n)
+        for got, want in ((k, kv), (v, vv)):
+            assert got.shape == (B, Hkv, n, D)
+            # code * scale is exact in fp32, so one fp32 and one bf16 rounding
+            assert torch.equal(got.cpu(), want[:, :, start:start + n].float().bfloat16())
+    starts = torch.tensor([60, 3], dtype=torch.int32, device=DEV)
+    k, v = K().kv_read_q4(*cache, starts, 20)
+    for b, s in enumerate((60, 3)):
+        assert torch.equal(k[b].cpu(), kv[b, :, s:s + 20].float().bfloat16())
+        assert torch.equal(v[b].cpu(), vv[b, :, s:s + 20].float().bfloat16())
+
+
+# ------------------------------------------------------------------ attention
+def check_attention(out, q, kv, vv, lens, scale, causal, group, chunk=False):
+    """|error| of one output value, with A = sum p |v| and ref in 64 bits:
+      * weights and values each rounded to bf16 (half a step, 2^-8):  2 * 2^-8 * A
+      * scores off by at most d each: weights off by a factor e^(2d), so (e^(2d) - 1) * A.
+        On the codes d is fp32 accumulation over T = scale sum_d |q_d| (128 s + |m|)
+        (the codes enter as 128 + c): 2^-19 T.  A chunk also rounds the keys to
+        bf16, 2^-8 scale sum_d |q_d k_d|, and its kernel's exp2 is off by up to
+        7.5e-5 < 2^-13.
+      * the output's own rounding: 2^-8 |ref|."""
+    ref, A = R.attention(q, kv, vv, lens, scale, causal)
+    qa = q.double().cpu().abs().amax(dim=(0, 1, 2))
+    # per key at most: values lie in [m, m + 15 s], so s <= 2/15 max|k| and |m| <= max|k|
+    ka = kv.abs().amax(dim=(0, 1, 2)) if kv.numel() else torch.zeros_like(qa)
+    groups = ka.view(-1, group).amax(-1).repeat_interleave(group)
+    d = 2.0 ** -19 * scale * float((qa * groups).sum()) * (128 * 2 / 15 + 1)
+    if chunk:
+        d += 2.0 ** -8 * scale * float((qa * ka).sum()) + 2.0 ** -13
+    tol = A * (2 ** -7 + math.expm1(2 * d)) + 2 ** -8 * ref.abs() + 1e-30
+    err = (out.double().cpu() - ref).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), f"worst {(err / tol).max():.3f} of the bound"
+    return float((err / tol).max())
+
+
+@pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("Hq,Hkv,Sq,kv,causal", [
+    (8, 1, 1, 1, False), (4, 4, 1, 31, False), (14, 2, 1, 33, False), (8, 2, 1, 129, True),
+    (32, 2, 1, 700, False),                        # 16 rows per kv head
+    (8, 2, 4, 77, True), (8, 2, 4, 3, True),       # queries that see nothing
+    (6, 2, 5, 64, False), (4, 1, 24, 200, True),   # 96 rows per kv head
+])
+def test_attention_on_the_codes(D, group, Hq, Hkv, Sq, kv, causal):
+    B, cap = 2, -(-kv // 16) * 16 + 16
+    cache, kk, vv = filled_cache(B, Hkv, cap, D, group, 21)
+    q = rows((B, Hq, Sq, D), 23)
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, causal)
+    assert out.shape == (B, Sq, Hq * D)
+    check_attention(out, q, kk, vv, [kv] * B, D ** -0.5, causal, group)
+
+
+@pytest.mark.parametrize("D,group", [(128, 32), (64, 64)])
+def test_attention_long_and_split(D, group):
+    B, Hq, Hkv, kv = 1, 8, 2, 9001
+    cache, kk, vv = filled_cache(B, Hkv, 9008, D, group, 31)
+    q = rows((B, Hq, 2, D), 33)
+    check_attention(K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, True), q, kk, vv, [kv],
+                    D ** -0.5, True, group)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,group,Sq", [(8, 2, 128, 32, 1), (8, 1, 64, 32, 3), (20, 4, 32, 32, 2)])
+def test_attention_with_a_length_per_sequence(Hq, Hkv, D, group, Sq):
+    lens = [0, 1, 2, 31, 32, 33, 500, 512]
+    B, cap = len(lens), 512
+    cache, kk, vv = filled_cache(B, Hkv, cap, D, group, 41)
+    q = rows((B, Hq, Sq, D), 43)
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = K().attention_cache_q4(q.to(DEV), *cache, t, D ** -0.5, True)
+    check_attention(out, q, kk, vv, lens, D ** -0.5, True, group)
+    assert not out[0].any()
+    # the bound on the lengths only changes how the work is split
+    lens2 = [min(n, 100) for n in lens]
+    out = K().attention_cache_q4(q.to(DEV), *cache, t.clamp(max=100), D ** -0.5, True, max_kv_len=100)
+    check_attention(out, q, kk, vv, lens2, D ** -0.5, True, group)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,group,Sq,kv,causal", [
+    (32, 4, 128, 32, 100, 333, True), (32, 4, 128, 128, 64, 64, True), (8, 2, 64, 64, 130, 400, True),
+    (6, 2, 32, 32, 128, 100, True),                # the first 28 queries see nothing
+    (32, 4, 128, 64, 40, 129, False),
+])
+def test_attention_of_a_chunk(Hq, Hkv, D, group, Sq, kv, causal):
+    B = 2
+    cache, kk, vv = filled_cache(B, Hkv, -(-kv // 16) * 16, D, group, 51, 0.5)
+    q = rows((B, Hq, Sq, D), 53, 0.5)
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, causal)
+    check_attention(out, q, kk, vv, [kv] * B, D ** -0.5, causal, group, chunk=True)
+
+
+@pytest.mark.parametrize("Sq", [1, 3, 64])
+def test_rows_behind_the_length_do_not_matter(Sq):
+    """Unwritten rows may hold anything: NaN and infinite scales, any codes."""
+    B, Hq, Hkv, D, kv, cap = 2, 32, 4, 128, 170, 272
+    cache, _, _ = filled_cache(B, Hkv, cap, D, 32, 61)
+    q = rows((B, Hq, Sq, D), 63).to(DEV)
+    lens = torch.full((B,), kv, dtype=torch.int32, device=DEV)
+    want = K().attention_cache_q4(q, *cache, kv, 0.1, True), K().attention_cache_q4(q, *cache, lens, 0.1, True)
+    for t in (cache[0], cache[2]):
+        t[:, :, kv:] = 255
+    for t, bad in ((cache[1], math.nan), (cache[3], math.inf)):
+        t[:, :, kv:] = bad
+    got = K().attention_cache_q4(q, *cache, kv, 0.1, True), K().attention_cache_q4(q, *cache, lens, 0.1, True)
+    assert torch.isfinite(want[0]).all()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_nonfinite_key_or_value_reaches_only_the_rows_that_see_it():
+    B, Hq, Hkv, D, kv, Sq = 1, 8, 2, 64, 40, 4
+    cache, _, _ = filled_cache(B, Hkv, 48, D, 32, 65)
+    q = rows((B, Hq, Sq, D), 66).to(DEV)
+    want = K().attention_cache_q4(q, *cache, kv, 0.125, True).view(Sq, Hkv, -1)
+    cache[1][0, 0, kv - 2] = math.nan  # a key of head 0 that queries 2 and 3 see
+    got = K().attention_cache_q4(q, *cache, kv, 0.125, True).view(Sq, Hkv, -1)
+    assert torch.equal(got[:2], want[:2]) and torch.equal(got[:, 1], want[:, 1])
+    assert got[2:, 0].isnan().all()
+
+
+def test_large_scores_and_equal_scores():
+    """Scores of thousands (one key takes all) and a row of equal scores."""
+    B, Hq, Hkv, D, kv = 1, 4, 1, 128, 300
+    cache, kk, vv = filled_cache(B, Hkv, 304, D, 32, 71, 8.0)
+    q = rows((B, Hq, 1, D), 73, 8.0)
+    q[0, 3] = 0
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, 1.0, False)
+    ref, A = R.attention(q, kk, vv, [kv], 1.0, False)
+    top = [int((kk[0, 0, :kv] @ q[0, h, 0].double()).argmax()) for h in range(3)]
+    for h in range(3):
+        v = vv[0, 0, top[h]]
+        assert ((out[0, 0, h * D:(h + 1) * D].cpu().double() - v).abs() <= 2 ** -7 * v.abs()).all()
+    mean = vv[0, 0, :kv].mean(0)
+    tol = 2 ** -7 * A[0, 0, 3 * D:] + 2 ** -8 * mean.abs()
+    assert ((out[0, 0, 3 * D:].cpu().double() - mean).abs() <= tol).all()
+
+
+def test_rows_past_32_bit_offsets():
+    """The last head of a cache whose codes pass 4 GiB."""
+    B, Hkv, D, group, cap, n = 1, 3, 128, 128, 1 << 25, 50
+    assert B * Hkv * cap * D // 2 > 1 << 32
+    cache = (torch.empty(B, Hkv, cap, D // 2, dtype=torch.uint8, device=DEV),
+             torch.empty(B, Hkv, cap, 1, 2, dtype=torch.bfloat16, device=DEV),
+             torch.empty(B, Hkv, cap, D // 2, dtype=torch.uint8, device=DEV),
+             torch.empty(B, Hkv, cap, 1, 2, dtype=torch.bfloat16, device=DEV))
+    k, v = rows((B, Hkv, n, D), 81), rows((B, Hkv, n, D), 82)
+    K().kv_append_q4(k.to(DEV), v.to(DEV), *cache, cap - n)
+    check_stored(cache[0][:, :, cap - n:], cache[1][:, :, cap - n:], k, group)
+    check_stored(cache[2][:, :, cap - n:], cache[3][:, :, cap - n:], v, group)
+    kr, vr = K().kv_read_q4(*cache, cap - n, n)
+    K().kv_append_q4(k.to(DEV), v.to(DEV), *cache, 0)
+    k0, v0 = K().kv_read_q4(*cache, 0, n)
+    assert torch.equal(kr, k0) and torch.equal(vr, v0)
+    q = rows((B, 6, 1, D), 83)
+    out = K().attention_cache_q4(q.to(DEV), *cache, n, 0.1, False)
+    small = [t[:, :, :n].contiguous() for t in cache]
+    kk, vv = R.values(small[0], small[1]), R.values(small[2], small[3])
+    check_attention(out, q, kk, vv, [n], 0.1, False, group)
+
+
+# ------------------------------------------------------------------ streams, graphs, determinism
+def test_calls_on_another_stream_and_together():
+    """Two calls in flight on two streams, and the same call again, agree."""
+    B, Hq, Hkv, D, kv = 4, 32, 4, 128, 3000
+    cache, _, _ = filled_cache(B, Hkv, 3008, D, 64, 91)
+    q = rows((B, Hq, 1, D), 93).to(DEV)
+    want = K().attention_cache_q4(q, *cache, kv, 0.09, False)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(K().attention_cache_q4(q, *cache, kv, 0.09, False))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_a_captured_step_follows_the_lengths():
+    """One capture of append + advance + attention, replayed as the cache grows,
+    gives what eager calls give; so does a second graph captured beside it."""
+    B, Hq, Hkv, D, cap = 3, 8, 2, 64, 64
+    bufs = [empty_cache(B, Hkv, cap, D, 32) for _ in range(3)]
+    start = torch.tensor([0, 5, 30], dtype=torch.int32, device=DEV)
+    past = rows((B, Hkv, cap, D), 101).to(DEV)
+    q, k, v = (torch.empty(B, h, 1, D, dtype=torch.bfloat16, device=DEV) for h in (Hq, Hkv, Hkv))
+    lens = [start.clone() for _ in range(3)]
+    for c in bufs:
+        K().kv_append_q4(past[:, :, :30], past[:, :, :30], *c, 0)
+
+    def step(i):
+        K().kv_append_q4(k, v, *bufs[i], lens[i])
+        lens[i].add_(1)
+        return K().attention_cache_q4(q, *bufs[i], lens[i], 0.125, False)
+
+    graphs, outs = [], []
+    for i in range(2):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            step(i)
+        torch.cuda.current_stream().wait_stream(side)
+        lens[i].copy_(start)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i))
+        graphs.append(g)
+        lens[i].copy_(start)
+    for n in range(20):
+        q.copy_(rows((B, Hq, 1, D), 200 + n))
+        k.copy_(rows((B, Hkv, 1, D), 300 + n))
+        v.copy_(rows((B, Hkv, 1, D), 400 + n))
+        for g in graphs:
+            g.replay()
+        want = step(2)
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want), n
+    assert lens[0].tolist() == [20, 25, 50]
+    K().device_error_check()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_a_cache_on_another_device():
+    cache, kk, vv = filled_cache(1, 2, 64, 64, 32, 111)
+    cache = tuple(t.to("cuda:1") for t in cache)
+    q = rows((1, 4, 1, 64), 113)
+    out = K().attention_cache_q4(q.to("cuda:1"), *cache, 50, 0.125, False)
+    check_attention(out, q, kk, vv, [50], 0.125, False, 32)
+
+
+def test_refusals():
+    cache = empty_cache(2, 2, 32, 64, 32)
+    x = torch.zeros(2, 2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device=DEV)
+    Kk = K()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    bad = [lambda: Kk.kv_append_q4(x, x, *cache, 29), lambda: Kk.kv_append_q4(x, x, *cache, -1),
+           lambda: Kk.kv_append_q4(x, x[:, :, :3], *cache, 0),
+           lambda: Kk.kv_append_q4(x[..., :32], x[..., :32], *cache, 0),
+           lambda: Kk.kv_append_q4(x.float(), x, *cache, 0),
+           lambda: Kk.kv_append_q4(x, x, *cache, i32(1)), lambda: Kk.kv_append_q4(x, x, *cache, i32(1, 2).long()),
+           lambda: Kk.kv_append_q4(x, x, *cache, i32(1, 2).cpu()),
+           lambda: Kk.kv_append_q4(x, x, cache[0], cache[1][..., :1, :], cache[2], cache[3], 0),
+           lambda: Kk.kv_append_q4(x, x, cache[0].float(), *cache[1:], 0),
+           lambda: Kk.kv_append_q4(x, x, cache[0].transpose(0, 1), *cache[1:], 0),
+           lambda: Kk.kv_read_q4(*cache, 30, 3), lambda: Kk.kv_read_q4(*cache, 0, -1),
+           lambda: Kk.kv_read_q4(*[t[:, :, :24].contiguous() for t in cache], 0, 1),
+           lambda: Kk.attention_cache_q4(q, *cache, 33, 0.1, False),
+           lambda: Kk.attention_cache_q4(q, *cache, -1, 0.1, False),
+           lambda: Kk.attention_cache_q4(q[:, :3], *cache, 3, 0.1, False),
+           lambda: Kk.attention_cache_q4(q[:1], *cache, 3, 0.1, False),
+           lambda: Kk.attention_cache_q4(q, *cache, i32(1, 2), 0.1, False, max_kv_len=33),
+           lambda: Kk.attention_cache_q4(q.float(), *cache, 3, 0.1, False)]
+    for call in bad:
+        with pytest.raises(RuntimeError):
+            call()
+    # nothing to do is no error
+    Kk.kv_append_q4(x[:, :, :0], x[:, :, :0], *cache, 32)
+    assert Kk.attention_cache_q4(q[:, :, :0], *cache, 3, 0.1, False).shape == (2, 0, 256)
+    assert not Kk.attention_cache_q4(q, *cache, 0, 0.1, False).any()
+    assert not Kk.attention_cache_q4(q.expand(2, 4, 300, 64), *cache, 0, 0.1, True).any()
+
+
+# ------------------------------------------------------------------ layer, model
+def _layer(cfg, g):
+    from qwen3_5_vl_cuda_custom_b200 import synthetic as syn
+    from qwen3_5_vl_cuda_custom_b200.modules import CudaTextDecoderLayer, TextMRoPE
+    layer = CudaTextDecoderLayer(cfg.hidden_size, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim,
+                                 cfg.intermediate_size, cfg.rms_norm_eps, use_moe=True,
+                                 num_experts=cfg.num_experts, top_k=cfg.num_experts_per_tok,
+                                 moe_intermediate_size=cfg.moe_intermediate_size)
+    layer.load_state_dict(syn.layer_params(cfg, g))
+    return (layer.to(DEV, torch.bfloat16),
+            TextMRoPE(cfg.head_dim, cfg.rope_theta, cfg.mrope_section).to(DEV))
+
+
+@pytest.mark.parametrize("group", [32, 128])
+def test_attention_module_over_a_prompt_chunk_and_decode_steps(group):
+    """Prompt (exact k/v), a second chunk (rows read back), decode steps (codes):
+    every call stores its rows and matches attention over what the cache holds."""
+    from qwen3_5_vl_cuda_custom_b200.configs import a3b_moe_text
+    from qwen3_5_vl_cuda_custom_b200.kv_cache import Q4LayerKVCache
+    cfg = a3b_moe_text(1)
+    g = torch.Generator().manual_seed(5)
+    layer, rot = _layer(cfg, g)
+    attn, D, B = layer.self_attn, cfg.head_dim, 2
+    cache = Q4LayerKVCache(B, cfg.num_kv_heads, 250, D, DEV, group_size=group)
+    at = 0
+    with torch.no_grad():
+        for S in (100, 60, 1, 3, 1):
+            x = torch.randn(B, S, cfg.hidden_size, generator=g).bfloat16().to(DEV)
+            pos = torch.arange(at, at + S, device=DEV).expand(B, S)
+            bound = rot.bind(torch.stack([pos] * 3))
+            q, k, v = attn._project(x, bound)
+            y, kept = attn(x, bound, past_kv=cache)
+            at += S
+            assert kept is cache and cache.length == at
+            w = slice(at - S, at)
+            check_stored(cache.k_codes[:, :, w], cache.k_scales[:, :, w], k.cpu(), group)
+            check_stored(cache.v_codes[:, :, w], cache.v_scales[:, :, w], v.cpu(), group)
+            kr, vr = cache
+            assert kr.shape == (B, cfg.num_kv_heads, at, D)
+            if S == 100:
+                o = K().attention_tokens(q, k, v, attn.scale, True)
+            else:
+                o = K().attention_cache_q4(q, *cache.buffers, at, attn.scale, S > 1)
+                check_attention(o, q, R.values(cache.k_codes[:, :, :at], cache.k_scales[:, :, :at]),
+                                R.values(cache.v_codes[:, :, :at], cache.v_scales[:, :, :at]), [at] * B,
+                                attn.scale, S > 1, group, chunk=S == 60)
+            assert torch.equal(y, attn.o_proj(o))
+        with pytest.raises(RuntimeError, match="KV cache full"):
+            x = torch.zeros(B, 90, cfg.hidden_size, dtype=torch.bfloat16, device=DEV)
+            pos = torch.arange(90, device=DEV).expand(B, 90)
+            attn(x, rot.bind(torch.stack([pos] * 3)), past_kv=cache)
+        assert cache.length == at
+
+
+def test_graphed_layer_decodes_a_ragged_batch():
+    """GraphedDecoderLayer over a cache with per-sequence lengths: one capture
+    serves a decode loop and matches the eager layer step by step."""
+    from qwen3_5_vl_cuda_custom_b200.configs import tiny_moe_text
+    from qwen3_5_vl_cuda_custom_b200.graphs import GraphedDecoderLayer
+    from qwen3_5_vl_cuda_custom_b200.kv_cache import Q4LayerKVCache
+    cfg = tiny_moe_text()
+    g = torch.Generator().manual_seed(9)
+    layer, rot = _layer(cfg, g)
+    B, S0 = 3, 20
+    lens = torch.tensor([20, 7, 13])
+    caches = [Q4LayerKVCache(B, cfg.num_kv_heads, 64, cfg.head_dim, DEV) for _ in range(2)]
+    x = torch.randn(B, S0, cfg.hidden_size, generator=g).bfloat16().to(DEV)
+    pos = torch.arange(S0, device=DEV).expand(B, S0)
+    with torch.no_grad():
+        for c in caches:  # right-padded prompts, then their true lengths
+            layer(x, rot.bind(torch.stack([pos] * 3)), past_kv=c)
+            c.set_lengths(lens)
+        x1 = torch.randn(B, 1, cfg.hidden_size, generator=g).bfloat16().to(DEV)
+        p = lens.to(DEV)[:, None].expand(3, B, 1).contiguous()
+        gl = GraphedDecoderLayer(layer, rot, x1, p, past_kv=caches[0])
+        assert caches[0].lengths.tolist() == lens.tolist()
+        for i in range(6):
+            x1 = torch.randn(B, 1, cfg.hidden_size, generator=g).bfloat16().to(DEV)
+            got = gl(x1)[0]
+            want = layer(x1, rot.bind(p + i), past_kv=caches[1])[0]
+            assert torch.equal(got, want), i
+            gl.static_pos.add_(1)
+    assert caches[0].lengths.tolist() == (lens + 6).tolist() == caches[1].lengths.tolist()
+    for a, b in zip(caches[0].buffers, caches[1].buffers):
+        for s, n in enumerate((lens + 6).tolist()):
+            assert torch.equal(a[s, :, :n].view(torch.uint8), b[s, :, :n].view(torch.uint8))
+    K().device_error_check()
+
+
+def _tiny_model():
+    from qwen3_5_vl_cuda_custom_b200.configs import MoETextConfig, moe_config
+    from qwen3_5_vl_cuda_custom_b200.models import CudaQwen3VLMoeModel
+    t = MoETextConfig(hidden_size=256, intermediate_size=512, num_layers=2, num_heads=4,
+                      num_kv_heads=2, head_dim=64, vocab_size=512, rope_theta=1e4,
+                      mrope_section=[16, 8, 8], num_experts=32, num_experts_per_tok=2,
+                      moe_intermediate_size=64)
+    torch.manual_seed(0)
+    return CudaQwen3VLMoeModel(moe_config(t), vision=False).to(DEV, torch.bfloat16)
+
+
+def test_generate_with_a_4_bit_cache():
+    model = _tiny_model()
+    ids = torch.randint(0, 512, (2, 12), device=DEV)
+    with torch.no_grad():
+        cache = model.make_kv_cache(2, 20, bits=4)
+        out = model.generate(ids, max_new_tokens=6, kv_cache=cache)
+        assert out.shape == (2, 18) and cache.length == 17
+        # the same loop through forward(); the prompt attends over its exact k/v
+        step, seq = model.make_kv_cache(2, 20, bits=4), [ids]
+        bf16 = model.make_kv_cache(2, 20)
+        logits, _ = model(ids, past_key_values=step)
+        ref, _ = model(ids, past_key_values=bf16)
+        assert torch.equal(logits, ref)
+        for _ in range(5):
+            seq.append(logits[:, -1].argmax(-1)[:, None])
+            logits, _ = model(seq[-1], past_key_values=step)
+        seq.append(logits[:, -1].argmax(-1)[:, None])
+    assert torch.equal(out, torch.cat(seq, dim=1))
+    with pytest.raises(ValueError):
+        model.make_kv_cache(2, 20, bits=8)
+
+
+def test_model_decodes_ragged_prompts_like_single_ones():
+    """Prompts of different lengths in one right-padded batch, then per-sequence
+    lengths: each sequence's logits match its own run within the kernels' batch
+    variation (other GEMM shapes round differently)."""
+    model = _tiny_model()
+    ids = torch.randint(0, 512, (2, 12), device=DEV)
+    nxt = torch.randint(0, 512, (2, 3), device=DEV)
+    lens = [12, 7]
+    with torch.no_grad():
+        cache = model.make_kv_cache(2, 32, bits=4)
+        model(ids, past_key_values=cache)
+        cache.set_lengths(torch.tensor(lens))
+        got = [model(nxt[:, i:i + 1], past_key_values=cache)[0][:, 0] for i in range(3)]
+        for b, n in enumerate(lens):
+            one = model.make_kv_cache(1, 32, bits=4)
+            model(ids[b:b + 1, :n], past_key_values=one)
+            for i in range(3):
+                want = model(nxt[b:b + 1, i:i + 1], past_key_values=one)[0][0, 0]
+                assert (got[i][b] - want).abs().max() <= 0.05 * want.abs().max(), (b, i)
+            assert one.length == n + 3 == int(cache[0].lengths[b])
