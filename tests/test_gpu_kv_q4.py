@@ -286,6 +286,24 @@ def test_a_nonfinite_key_or_value_reaches_only_the_rows_that_see_it():
     assert got[2:, 0].isnan().all()
 
 
+@pytest.mark.parametrize("D,group", SHAPES)
+def test_a_nonfinite_value_reaches_only_the_rows_that_see_it(D, group):
+    """A weight of 0 times NaN is NaN: a value group stored as NaN must not touch
+    the queries in front of it, the other channels or the other heads."""
+    B, Hq, Hkv, kv, Sq = 2, 4, 2, 150, 40  # the mask crosses more than one key tile
+    cache, _, _ = filled_cache(B, Hkv, 160, D, group, 67)
+    q = rows((B, Hq, Sq, D), 68).to(DEV)
+    want = K().attention_cache_q4(q, *cache, kv, 0.125, True).view(B, Sq, Hkv, 2, D // group, group)
+    first = D // group - 1
+    for key in (112, 149):  # seen from query 2 on, and by the last query only
+        cache[3][1, 0, key, first] = math.nan
+    got = K().attention_cache_q4(q, *cache, kv, 0.125, True).view(B, Sq, Hkv, 2, D // group, group)
+    hit = got[1, 2:, 0, :, first]
+    assert hit.isnan().all()
+    hit.copy_(want[1, 2:, 0, :, first])
+    assert torch.equal(got, want)
+
+
 def test_large_scores_and_equal_scores():
     """Scores of thousands (one key takes all) and a row of equal scores."""
     B, Hq, Hkv, D, kv = 1, 4, 1, 128, 300
