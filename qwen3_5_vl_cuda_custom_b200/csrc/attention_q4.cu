@@ -9,18 +9,27 @@
 // is two codes to unpack, so the instructions per code decide.  Per SM and clock
 // HBM delivers about 24 bytes = 48 codes against 128 lanes of issue.
 //
+// Codes as bf16.  The bits c << 4 (c = 0..15) read as bf16 are c * 2^-129 and the
+// bits c are c * 2^-133: bf16's subnormals and its first binade are evenly
+// spaced.  The matrix units and fma.bf16x2 take subnormals at full precision, so
+// `w & 0x000f000f` and `w & 0x00f000f0` are pairs of codes as they stand, without
+// a conversion or an offset to take out again; one shift by 8 gives the other
+// four codes of a word.  The powers of two go into the other operand.
+//
 // Scores.  With K = m + s c per group j, q . K = sum_j s_j (Q_j . c_j) + m_j sum(Q_j).
-// The codes go into the matrix instruction as the exact bf16 numbers 128 + c (one
-// logic operation per two codes); its accumulator starts at -128 sum(Q_j), which
-// takes the 128 out again.  So K is never rounded, and scale and minimum cost two
-// fp32 operations per key, query and group.
+// Q is scaled by 2^52 (codes at bit 0) or 2^48 (at bit 4), so a product is
+// 2^-81 Q . c; the minima go through one more matrix instruction whose other
+// operand is 2^-81 sum(Q_j) split into three bf16 parts (24 bits).  So K is never
+// rounded, and the scale costs one fp32 operation per key, query and group.
+// |Q| must stay below 2^75.
 //
 // Keys are the 16 rows of the instruction and queries its 8 columns (S^T = K Q^T,
 // O^T = V^T P^T): a decode step has G = Hq/Hkv queries per kv head, often 8, and
 // no half of the tile is idle.  P moves from accumulator to operand layout by an
 // 8x8 transpose between the lanes (movmatrix).  P is rounded to bf16 (as in the
 // bf16 attention kernels), V is dequantised to bf16 in registers, one rounding of
-// m + s c: what a read back gives.
+// m + s c: what a read back gives, as (2^-129 c) (2^69 s) + 2^-60 m, or 2^-64 of the
+// value for codes at bit 0 (exact scales: |V| between 2^-60 and 2^58).
 //
 // Each warp walks its own 32-key tiles with a private ring of bulk copies (four
 // per tile: K codes, K scales, V codes, V scales, all contiguous in memory), so
@@ -29,6 +38,8 @@
 // are then on both sides of the 128-byte bank window at every head size.
 #include "kv_q4.cuh"
 #include "sm100.cuh"
+
+#include <float.h>
 
 #include <type_traits>
 
@@ -95,19 +106,27 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The bf16 pair (128 + field i, 128 + field i + 4) of a code word.
-__device__ __forceinline__ uint32_t codes128(uint32_t w, int i) {
-  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+// The codes of fields 0..3 and 4..7 of a word as bf16 pairs (field i, field i + 4):
+// c * 2^-133 for i = 0, 2 and c * 2^-129 for i = 1, 3.
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t (&c)[4]) {
+  const uint32_t h = w >> 8;
+  c[0] = w & 0x000f000fu;
+  c[1] = w & 0x00f000f0u;
+  c[2] = h & 0x000f000fu;
+  c[3] = h & 0x00f000f0u;
 }
-// (c, c') * s + m as a bf16 pair; c and s per half.
-__device__ __forceinline__ uint32_t dequant2(uint32_t c128, uint32_t s, uint32_t m) {
-  const uint32_t k128 = 0x43004300u;
-  __nv_bfloat162 c = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&c128),
-                             *reinterpret_cast<const __nv_bfloat162 *>(&k128));
-  __nv_bfloat162 v = __hfma2(c, *reinterpret_cast<__nv_bfloat162 *>(&s),
-                             *reinterpret_cast<__nv_bfloat162 *>(&m));
-  return *reinterpret_cast<uint32_t *>(&v);
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
 }
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Powers of two as bf16 bits.
+constexpr uint32_t pow2_bf16(int e) { return static_cast<uint32_t>(127 + e) << 7; }
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
   if constexpr (N == 4)
@@ -192,8 +211,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
   // Query rows: row r -> head hk G + r / Sq, position r % Sq.  Column g of an
   // operand tile holds 8 channels of every 32; accumulator columns are 2t, 2t + 1.
   uint32_t qf[NT][J][4];
-  float nsum[NT][NS][2];  // -128 sum(Q_j) for the two accumulator columns
-  int lim[NT][2];         // keys the column's query sees
+  uint32_t qm[NT][2];  // 2^-81 sum(Q_t) of group t in three bf16 parts
+  int lim[NT][2];      // keys the column's query sees
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = (rg * NT + nt) * 8 + g;
@@ -209,25 +228,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
     for (int j = 0; j < J; ++j) {
       const uint4 x = src ? *reinterpret_cast<const uint4 *>(src + 32 * j + 8 * t)
                           : make_uint4(0u, 0u, 0u, 0u);
-      qf[nt][j][0] = x.x;
-      qf[nt][j][1] = x.y;
-      qf[nt][j][2] = x.z;
-      qf[nt][j][3] = x.w;
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float lo, hi;
-        unpack_bf2(qf[nt][j][i], lo, hi);
+        unpack_bf2(xs[i], lo, hi);
         sum[j / BPG] += lo + hi;
+        const float up = i % 2 == 0 ? 0x1p52f : 0x1p48f;
+        qf[nt][j][i] = pack_bf2(lo * up, hi * up);
       }
     }
+    float mine = 0.f;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       float v = sum[j];
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       v += __shfl_xor_sync(0xffffffffu, v, 2);
-      nsum[nt][j][0] = -128.f * __shfl_sync(0xffffffffu, v, 8 * t);
-      nsum[nt][j][1] = -128.f * __shfl_sync(0xffffffffu, v, 8 * t + 4);
+      if (j == t) mine = v * 0x1p-81f;
     }
+    const float h0 = bf2f(f2bf(mine)), h1 = bf2f(f2bf(mine - h0));
+    qm[nt][0] = pack_bf2(h0, h1);
+    qm[nt][1] = pack_bf2(mine - h0 - h1, 0.f);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int rc = (rg * NT + nt) * 8 + 2 * t + c;
@@ -240,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
   float row_m[NT][2], row_l[NT][2];  // in units of log2; l of this lane's keys only
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    row_m[nt][0] = row_m[nt][1] = -INFINITY;
+    row_m[nt][0] = row_m[nt][1] = -FLT_MAX;
     row_l[nt][0] = row_l[nt][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
@@ -250,6 +271,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
   const int pit = t + (t >= 2 ? 4 : 0);                           // pi(2t); pi(2t + 1) = pit ^ 3
   const int jv = D == 128 ? 2 * (g & 1) : (D == 64 ? (g & 1) : 0);  // 32-channel block of V word 0
 
+  constexpr uint32_t kUpS = pow2_bf16(69) * 0x10001u, kDownM0 = pow2_bf16(-64) * 0x10001u,
+                     kDownM1 = pow2_bf16(-60) * 0x10001u;
+  const float scale_up = p.scale_log2 * 0x1p81f;
   bool ok = true;
   int stage = 0, phase = 0;
   int tl = tile0 + warp;
@@ -268,27 +292,30 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
     float s[2][NT][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      uint32_t wl[J], wh[J], pl[NS], ph[NS];
+      uint32_t wl[J], wh[J], pl[NS], ph[NS], ml[1], mh[1];
       const int kl = 16 * mt + pig;
       lds_words<J>(wl, sk + kl * (D / 2) + t * (4 * J));
       lds_words<J>(wh, sk + (kl + 8) * (D / 2) + t * (4 * J));
       lds_words<NS>(pl, sks + kl * (NS * 4));
       lds_words<NS>(ph, sks + (kl + 8) * (NS * 4));
+      lds_words<1>(ml, sks + (kl * NS + t % NS) * 4);
+      lds_words<1>(mh, sks + ((kl + 8) * NS + t % NS) * 4);
+      // minima: (m, m, m) of group t times the parts of its sum(Q)
+      const uint32_t m0 = __byte_perm(ml[0], 0u, 0x3232), m1 = __byte_perm(mh[0], 0u, 0x3232);
       float part[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        mma(s[mt][nt], m0, m1, m0, m1, qm[nt][0], qm[nt][1], 0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         uint32_t a[4], c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] = codes128(wl[j], i);
-          c[i] = codes128(wh[j], i);
-        }
+        codes4(wl[j], a);
+        codes4(wh[j], c);
         const int sg = j / BPG;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float n0 = nsum[nt][sg][0], n1 = nsum[nt][sg][1];
           if (j % BPG == 0)
-            mma(part[nt], a[0], c[0], a[1], c[1], qf[nt][j][0], qf[nt][j][1], n0, n1, n0, n1);
+            mma(part[nt], a[0], c[0], a[1], c[1], qf[nt][j][0], qf[nt][j][1], 0.f, 0.f, 0.f, 0.f);
           else
             mma(part[nt], a[0], c[0], a[1], c[1], qf[nt][j][0], qf[nt][j][1], part[nt][0],
                 part[nt][1], part[nt][2], part[nt][3]);
@@ -296,24 +323,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
               part[nt][1], part[nt][2], part[nt][3]);
         }
         if (j % BPG == BPG - 1) {
-          // scale * part + minimum * sum(Q), the sum as nsum / -128
           const float s0 = __uint_as_float(pl[sg] << 16), s1 = __uint_as_float(ph[sg] << 16);
-          const float m0 = __uint_as_float(pl[sg] & 0xffff0000u) * -0.0078125f;
-          const float m1 = __uint_as_float(ph[sg] & 0xffff0000u) * -0.0078125f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float n0 = nsum[nt][sg][0], n1 = nsum[nt][sg][1];
-            if (sg == 0) {
-              s[mt][nt][0] = m0 * n0;
-              s[mt][nt][1] = m0 * n1;
-              s[mt][nt][2] = m1 * n0;
-              s[mt][nt][3] = m1 * n1;
-            } else {
-              s[mt][nt][0] = fmaf(m0, n0, s[mt][nt][0]);
-              s[mt][nt][1] = fmaf(m0, n1, s[mt][nt][1]);
-              s[mt][nt][2] = fmaf(m1, n0, s[mt][nt][2]);
-              s[mt][nt][3] = fmaf(m1, n1, s[mt][nt][3]);
-            }
             s[mt][nt][0] = fmaf(s0, part[nt][0], s[mt][nt][0]);
             s[mt][nt][1] = fmaf(s0, part[nt][1], s[mt][nt][1]);
             s[mt][nt][2] = fmaf(s1, part[nt][2], s[mt][nt][2]);
@@ -324,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][nt][e] *= p.scale_log2;
+        for (int e = 0; e < 4; ++e) s[mt][nt][e] *= scale_up;
     }
 
     if (masked) {
@@ -391,9 +403,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
         }
         mx0 = fmaxf(mx0, row_m[nt][0]);
         mx1 = fmaxf(mx1, row_m[nt][1]);
-        // a column that has seen no key keeps -inf: its factor is 1, not exp2(nan)
-        const float a0 = mx0 == -INFINITY ? 1.f : exp2_fast(row_m[nt][0] - mx0);
-        const float a1 = mx1 == -INFINITY ? 1.f : exp2_fast(row_m[nt][1] - mx1);
+        const float a0 = exp2_fast(row_m[nt][0] - mx0), a1 = exp2_fast(row_m[nt][1] - mx1);
         row_m[nt][0] = mx0;
         row_m[nt][1] = mx1;
         row_l[nt][0] *= a0;
@@ -406,8 +416,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
           o[i][nt][3] *= a1;
         }
       }
-      const float mu0 = row_m[nt][0] == -INFINITY ? 0.f : row_m[nt][0];
-      const float mu1 = row_m[nt][1] == -INFINITY ? 0.f : row_m[nt][1];
+      const float mu0 = row_m[nt][0], mu1 = row_m[nt][1];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         const float p0 = exp2_fast(s[mt][nt][0] - mu0), p1 = exp2_fast(s[mt][nt][1] - mu1);
@@ -444,21 +453,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
 #pragma unroll
       for (int w = 0; w < WV; ++w) {
         const int sw = w * PS / WV;
-        // (key a, key b) pairs of scales and minima, and of codes
-        const uint32_t s2 = __byte_perm(pa[sw], pbb[sw], 0x5410);
-        const uint32_t m2 = __byte_perm(pa[sw], pbb[sw], 0x7632);
-        const uint32_t s28 = __byte_perm(pa8[sw], pb8[sw], 0x5410);
-        const uint32_t m28 = __byte_perm(pa8[sw], pb8[sw], 0x7632);
-        const uint32_t x = __byte_perm(wa[w], wb[w], 0x5410), y = __byte_perm(wa[w], wb[w], 0x7632);
-        const uint32_t x8 = __byte_perm(wa8[w], wb8[w], 0x5410);
-        const uint32_t y8 = __byte_perm(wa8[w], wb8[w], 0x7632);
+        // (key a, key b) pairs of scales and minima, with their powers of two, and of codes
+        const uint32_t s2 = mul2(__byte_perm(pa[sw], pbb[sw], 0x5410), kUpS);
+        const uint32_t m2[2] = {mul2(__byte_perm(pa[sw], pbb[sw], 0x7632), kDownM0),
+                                mul2(__byte_perm(pa[sw], pbb[sw], 0x7632), kDownM1)};
+        const uint32_t s28 = mul2(__byte_perm(pa8[sw], pb8[sw], 0x5410), kUpS);
+        const uint32_t m28[2] = {mul2(__byte_perm(pa8[sw], pb8[sw], 0x7632), kDownM0),
+                                 mul2(__byte_perm(pa8[sw], pb8[sw], 0x7632), kDownM1)};
+        uint32_t x[4], x8[4], y[4], y8[4];
+        codes4(__byte_perm(wa[w], wb[w], 0x5410), x);
+        codes4(__byte_perm(wa8[w], wb8[w], 0x5410), x8);
+        if constexpr (D > 32) {
+          codes4(__byte_perm(wa[w], wb[w], 0x7632), y);
+          codes4(__byte_perm(wa8[w], wb8[w], 0x7632), y8);
+        }
 #pragma unroll
         for (int i = 0; i < MT / WV; ++i) {
           // channels of rows g and g + 8: fields i, i + 4 (D = 32: i, i + 2 of a half word)
-          const uint32_t a0 = dequant2(codes128(x, i), s2, m2);
-          const uint32_t a1 = dequant2(D == 32 ? codes128(x, i + 2) : codes128(y, i), s2, m2);
-          const uint32_t a2 = dequant2(codes128(x8, i), s28, m28);
-          const uint32_t a3 = dequant2(D == 32 ? codes128(x8, i + 2) : codes128(y8, i), s28, m28);
+          const uint32_t a0 = fma2(x[i], s2, m2[i % 2]);
+          const uint32_t a1 = fma2(D == 32 ? x[i + 2] : y[i], s2, m2[i % 2]);
+          const uint32_t a2 = fma2(x8[i], s28, m28[i % 2]);
+          const uint32_t a3 = fma2(D == 32 ? x8[i + 2] : y8[i], s28, m28[i % 2]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float(&acc)[4] = o[w * (MT / WV) + i][nt];
@@ -489,6 +504,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
   }
 
   // ---- join the warps: [warp][row][D channels, m, l]
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][nt][e] *= i % 2 == 0 ? 0x1p64f : 0x1p60f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -529,16 +550,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Para
     const int lr = it / (D / 4), ch = (it - lr * (D / 4)) * 4;
     const int r = rg * 8 * NT + lr;
     if (r >= p.R) continue;
-    float M = -INFINITY;
+    float M = -FLT_MAX;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm[(w * 8 * NT + lr) * L::kRowF + D]);
-    const float Mu = M == -INFINITY ? 0.f : M;
     float l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float *row = sm + (w * 8 * NT + lr) * L::kRowF;
-      const float f = exp2_fast(row[D] - Mu);
+      const float f = exp2_fast(row[D] - M);
       l += row[D + 1] * f;
       const float4 x = *reinterpret_cast<const float4 *>(row + ch);
       acc.x += x.x * f;
@@ -569,17 +589,16 @@ __global__ void __launch_bounds__(128) attn_q4_join_kernel(Params p, int64_t row
   if (gr >= rows) return;
   const float2 *ml = reinterpret_cast<const float2 *>(p.ws + rows * p.n_splits * D) + gr * p.n_splits;
   const float *acc = p.ws + gr * p.n_splits * D + lane * E;
-  float M = -INFINITY;
+  float M = -FLT_MAX;
   for (int s = lane; s < p.n_splits; s += 32) M = fmaxf(M, ml[s].x);
   M = warp_max(M);
-  const float Mu = M == -INFINITY ? 0.f : M;
   float l = 0.f, v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 4
   for (int s = 0; s < p.n_splits; ++s) {
     const float2 x = ml[s];
-    const float f = exp2_fast(x.x - Mu);
+    const float f = exp2_fast(x.x - M);
     l += x.y * f;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] += acc[int64_t(s) * D + e] * f;

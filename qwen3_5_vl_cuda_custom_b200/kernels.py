@@ -30,6 +30,15 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """_lib.call with ``device`` current (no context switch when it is already)."""
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args)
+
+
 def _require(t: torch.Tensor, name: str, dtype: torch.dtype | tuple = _BF16) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
@@ -558,23 +567,25 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 # ---------------------------------------------------------------- 4-bit KV cache
 def _cache_q4(name: str, k_codes, k_scales, v_codes, v_scales) -> tuple[int, int, int, int, int]:
     """Checks the four tensors of a 4-bit cache; returns (B, Hkv, capacity, D, group)."""
+    cs, ss = k_codes.shape, k_scales.shape
+    if (len(cs) == 4 and len(ss) == 5 and cs == v_codes.shape and ss == v_scales.shape
+            and k_codes.dtype == v_codes.dtype == torch.uint8
+            and k_scales.dtype == v_scales.dtype == _BF16
+            and k_codes.is_cuda and k_codes.device == k_scales.device == v_codes.device == v_scales.device
+            and k_codes.is_contiguous() and v_codes.is_contiguous()
+            and k_scales.is_contiguous() and v_scales.is_contiguous()):
+        B, Hkv, cap, half = cs
+        D, groups = 2 * half, ss[3]
+        if D in (32, 64, 128) and groups > 0 and D % groups == 0 and ss == (B, Hkv, cap, groups, 2):
+            return B, Hkv, cap, D, D // groups
     for t, part, dt, dims in ((k_codes, "k_codes", torch.uint8, 4), (k_scales, "k_scales", _BF16, 5),
                               (v_codes, "v_codes", torch.uint8, 4), (v_scales, "v_scales", _BF16, 5)):
         _require(t, f"{name}.{part}", dt)
         if t.dim() != dims or not t.is_contiguous():
             raise RuntimeError(f"{name}: {part} must be contiguous with {dims} dims (it is used in place)")
-        if t.device != k_codes.device:
-            raise RuntimeError(f"{name}: the cache's tensors are on different devices")
-    B, Hkv, cap, half = k_codes.shape
-    D, groups = 2 * half, k_scales.shape[3]
-    if D not in (32, 64, 128) or groups == 0 or D % groups:
-        raise RuntimeError(f"{name}: codes {tuple(k_codes.shape)} and scales {tuple(k_scales.shape)} "
-                           "do not belong to a head_dim of 32, 64 or 128")
-    if (v_codes.shape != k_codes.shape or v_scales.shape != k_scales.shape
-            or tuple(k_scales.shape) != (B, Hkv, cap, groups, 2)):
-        raise RuntimeError(f"{name}: shapes {tuple(k_codes.shape)}, {tuple(k_scales.shape)}, "
-                           f"{tuple(v_codes.shape)}, {tuple(v_scales.shape)} do not match")
-    return B, Hkv, cap, D, D // groups
+    raise RuntimeError(f"{name}: codes {tuple(cs)}, {tuple(v_codes.shape)} and scales {tuple(ss)}, "
+                       f"{tuple(v_scales.shape)} do not belong to one cache (head_dim 32, 64 or 128, "
+                       "all on one device)")
 
 
 def _per_sequence(t: torch.Tensor, name: str, B: int, device) -> torch.Tensor:
@@ -623,11 +634,10 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
         raise RuntimeError(f"kv_append_q4: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of "
                            f"{(B, Hkv, cap, D)}")
     rows = _per_sequence(offset, "kv_append_q4.offset", B, dev) if isinstance(offset, torch.Tensor) else None
-    with torch.cuda.device(dev):
-        _lib.call("q35_kv_append_q4", k.data_ptr(), v.data_ptr(), _lib.strides_arg(k),
-                  _lib.strides_arg(v), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-                  v_scales.data_ptr(), B, Hkv, S, D, group, cap, 0 if rows is not None else int(offset),
-                  _ptr(rows), _stream(k_codes))
+    _call_on(dev, "q35_kv_append_q4", k.data_ptr(), v.data_ptr(), _lib.strides_arg(k),
+             _lib.strides_arg(v), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+             v_scales.data_ptr(), B, Hkv, S, D, group, cap, 0 if rows is not None else int(offset),
+             _ptr(rows), _stream(k_codes))
 
 
 def _read_q4(cache, shape, start: int, starts, n: int, out_cap: int):
@@ -635,9 +645,8 @@ def _read_q4(cache, shape, start: int, starts, n: int, out_cap: int):
     dev = cache[0].device
     k = torch.empty(B, Hkv, out_cap, D, device=dev, dtype=_BF16)
     v = torch.empty_like(k)
-    with torch.cuda.device(dev):
-        _lib.call("q35_kv_read_q4", *[t.data_ptr() for t in cache], k.data_ptr(), v.data_ptr(), B, Hkv,
-                  n, out_cap, D, group, cap, start, _ptr(starts), _stream(cache[0]))
+    _call_on(dev, "q35_kv_read_q4", *[t.data_ptr() for t in cache], k.data_ptr(), v.data_ptr(), B, Hkv,
+             n, out_cap, D, group, cap, start, _ptr(starts), _stream(cache[0]))
     return k, v
 
 
@@ -690,20 +699,19 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     if n < 0 or n > cap:
         raise RuntimeError(f"attention_cache_q4: {n} rows exceed the capacity {cap}")
     out = torch.empty(B, Sq, Hq * D, device=q.device, dtype=q.dtype)
-    with torch.cuda.device(q.device):
-        if lens is None and (Hq // Hkv) * Sq >= _Q4_PREFILL_ROWS and n > 0:
-            # whole key tiles, zero-filled: the prefill kernel reads (and masks) to the end of one
-            pad = -(-n // 128) * 128
-            k, v = _read_q4(cache, shape, 0, None, n, pad)
-            _lib.call("q35_attn_prefill_cache_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                      out.data_ptr(), None, B, Hq, Hkv, Sq, n, pad, D, float(scale),
-                      1 if causal else 0, _stream(q))
-        else:
-            w = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, n, D)
-            ws = torch.empty(max(1, w), device=q.device, dtype=torch.float32)
-            _lib.call("q35_attn_q4_fwd", q.data_ptr(), *[t.data_ptr() for t in cache], out.data_ptr(),
-                      B, Hq, Hkv, Sq, n, _ptr(lens), cap, D, group, float(scale), 1 if causal else 0,
-                      ws.data_ptr(), _stream(q))
+    if lens is None and (Hq // Hkv) * Sq >= _Q4_PREFILL_ROWS and n > 0:
+        # whole key tiles, zero-filled: the prefill kernel reads (and masks) to the end of one
+        pad = -(-n // 128) * 128
+        k, v = _read_q4(cache, shape, 0, None, n, pad)
+        _call_on(q.device, "q35_attn_prefill_cache_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                 out.data_ptr(), None, B, Hq, Hkv, Sq, n, pad, D, float(scale), 1 if causal else 0,
+                 _stream(q))
+    else:
+        w = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, n, D)
+        ws = torch.empty(w, device=q.device, dtype=torch.float32) if w > 0 else None
+        _call_on(q.device, "q35_attn_q4_fwd", q.data_ptr(), *[t.data_ptr() for t in cache],
+                 out.data_ptr(), B, Hq, Hkv, Sq, n, _ptr(lens), cap, D, group, float(scale),
+                 1 if causal else 0, _ptr(ws), _stream(q))
     return out
 
 
