@@ -7,7 +7,8 @@
 // What bounds it: a key and its value are 160 bytes at D = 128 (groups of 32),
 // read once, so a long cache should run at memory speed; but each of those bytes
 // is two codes to unpack, so the instructions per code decide.  Per SM and clock
-// HBM delivers about 24 bytes = 48 codes against 128 lanes of issue.
+// HBM delivers about 24 bytes = 48 codes against 128 lanes of issue, 64 of them
+// for logic operations.
 //
 // Codes as bf16.  The bits c << 4 (c = 0..15) read as bf16 are c * 2^-129 and the
 // bits c are c * 2^-133: bf16's subnormals and its first binade are evenly
@@ -31,17 +32,27 @@
 // m + s c: what a read back gives, as (2^-129 c) (2^69 s) + 2^-60 m, or 2^-64 of the
 // value for codes at bit 0 (exact scales: |V| between 2^-60 and 2^58).
 //
-// Each warp walks its own 32-key tiles with a private ring of bulk copies (four
-// per tile: K codes, K scales, V codes, V scales, all contiguous in memory), so
-// no warp waits for another before the end.  Within a block of 8 keys, row r of
-// the instruction is key pi(r) = 0,3,1,2,6,5,7,4: the four keys a V load touches
-// are then on both sides of the 128-byte bank window at every head size.
-#include "kv_q4.cuh"
-#include "sm100.cuh"
-
+// V's operand wants pairs of neighbouring keys.  A transposing ldmatrix over the
+// codes as 16-bit units (four codes) gives exactly that: a lane receives, for two
+// keys, the unit of its column, so its eight V channels per 16-byte chunk pair
+// come without a byte permutation and belong to one scale group.
+//
+// Work.  The 32-key tiles of all (sequence, kv head, group of 8 NT query rows)
+// form one list that is cut into equal runs, one per resident CTA; a run may end
+// one group, take several whole and begin another.  Nothing depends on the
+// lengths being alike, and the rings below never drain between groups.  A group
+// that one run holds whole is written at once, the others leave (max, sum, O)
+// partials that a second kernel joins; a run leaves at most two.
+//
+// Each warp takes every fourth tile of the run through a private ring of
+// asynchronous 16-byte copies, so warps meet only at the end of a group.  The
+// 16-byte chunks of a row are XOR-swizzled by the row so that both the 16-byte
+// reads of K and the 8-row reads of V touch every bank once.
 #include <float.h>
 
 #include <type_traits>
+
+#include "kv_q4.cuh"
 
 namespace q35 {
 namespace {
@@ -50,8 +61,11 @@ using q4::Cache;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 32;    // keys per tile
-constexpr int kStages = 3;   // tiles in flight per warp
+constexpr int kTile = 32;  // keys per tile
+// CTAs per SM, and tiles in flight per warp: what registers and shared memory
+// (40 KB of rings and 13.5 KB to join the warps at D = 128, NT = 1) allow.
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : 2; }
+constexpr int stages(int d, int nt) { return d == 128 && nt == 1 ? 2 : 4; }
 
 struct Params {
   const uint16_t *q;
@@ -60,32 +74,99 @@ struct Params {
   float *ws;
   const int32_t *kv_lens;
   int *err;
-  int Hq, Hkv, G, Sq, R, n_rg, n_splits, causal;
-  int64_t kv_len, cap;
+  int B, Hq, Hkv, G, Sq, R, n_rg, causal;
+  int runs;  // CTAs of the main kernel
+  int per;   // tiles of a run (without kv_lens)
+  int kv_len;
+  int64_t cap;
   float scale_log2;
 };
 
-template <int D, int GS>
+template <int D, int GS, int NT>
 struct Layout {
   static constexpr int J = D / 32;       // code words per lane and key
   static constexpr int NS = D / GS;      // scale words per key
+  static constexpr int kStages = stages(D, NT);
   static constexpr int kCodes = kTile * D / 2, kScales = kTile * NS * 4;
   static constexpr int kStage = 2 * (kCodes + kScales);
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kRowF = D + 4;    // floats per row of the warps' merge
-  static constexpr int smem(int nt) {
-    const int merge = kWarps * 8 * nt * kRowF * 4;
-    return kWarps * kRing > merge ? kWarps * kRing : merge;
-  }
+  static constexpr int kRegs = NT * (D / 4 + 4);  // a lane's O, m, l
+  static constexpr int kSmem = kWarps * kRing + (kWarps - 1) * kRegs * 128;
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
-                                          uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
-      : "memory");
+// Partials: [2 runs][8 NT rows][D] floats, then [2 runs][8 NT rows] (m, l).
+// Slot 2 r holds the group that run r continues, 2 r + 1 the one it begins.
+constexpr int64_t partial_rows(int64_t runs, int nt) { return 2 * runs * 8 * nt; }
+
+__device__ __forceinline__ int clamp_len(const Params &p, int b) {
+  if (!p.kv_lens) return p.kv_len;
+  return max(0, min(p.kv_lens[b], p.kv_len));
+}
+// Tiles of a group; a sequence without rows counts as one tile, so that some CTA
+// writes its zeros.
+__host__ __device__ __forceinline__ int tiles_of(int len) {
+  return len > 0 ? (len + kTile - 1) / kTile : 1;
+}
+__host__ __device__ __forceinline__ int run_length(int total, int runs) {
+  const int per = (total + runs - 1) / runs;
+  return (per + kWarps - 1) / kWarps * kWarps;  // whole rounds of the four warps
+}
+
+// A group of the list: its sequence, its (kv head, row group) index, its first
+// tile, the sequence's length in keys and tiles.
+struct Group {
+  int b, hg, begin, len, tiles;
+};
+// Prefix sums over the sequences' tiles by the whole CTA.  Returns the tiles of
+// all groups; finds the sequence that holds tile at(total) (or, if seq >= 0,
+// looks at that sequence) and sets its first tile.
+template <typename At>
+__device__ __forceinline__ int scan_tiles(const Params &p, int seq, At &&at, Group &gr) {
+  __shared__ int warp_sum[kWarps], found[2];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int each = (p.B + kThreads - 1) / kThreads, b0 = tid * each, b1 = min(b0 + each, p.B);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of(clamp_len(p, b));
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  if (lane == 31) warp_sum[tid >> 5] = incl;
+  __syncthreads();
+  int total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < (tid >> 5)) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  const int unit = p.Hkv * p.n_rg;
+  total *= unit;
+  const int want = at(total);
+  for (int b = b0; b < b1; ++b) {
+    const int t = tiles_of(clamp_len(p, b));
+    if (seq >= 0 ? b == seq : (want >= before * unit && want - before * unit < t * unit)) {
+      found[0] = b;
+      found[1] = before * unit;
+    }
+    before += t;
+  }
+  __syncthreads();
+  gr.b = found[0];
+  gr.begin = found[1];
+  return total;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live) {
+  const int n = live ? 16 : 0;  // 0: the 16 bytes become zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 // D = A(16x16 bf16) * B(16x8 bf16) + C, fp32.
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -127,6 +208,7 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
 }
 // Powers of two as bf16 bits.
 constexpr uint32_t pow2_bf16(int e) { return static_cast<uint32_t>(127 + e) << 7; }
+
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
   if constexpr (N == 4)
@@ -137,496 +219,589 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
   else
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
 }
-__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
-  return v;
+__device__ __forceinline__ uint32_t lds1(uint32_t addr) {
+  uint32_t w[1];
+  lds_words<1>(w, addr);
+  return w[0];
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ bool nonfinite(uint32_t pair) {
   return (((pair & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
 }
 
-// One CTA = (sequence, kv head, group of 8 NT query rows, split of the keys).
+// One CTA = one run of tiles.
 template <int D, int GS, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_q4_kernel(Params p) {
-  using L = Layout<D, GS>;
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Params p) {
+  using L = Layout<D, GS, NT>;
   constexpr int J = L::J, NS = L::NS, BPG = GS / 32;
-  constexpr int WV = D >= 64 ? D / 64 : 1;      // V words per lane and key
+  constexpr int RB = D / 2;                     // bytes of a row of codes
+  constexpr int CH = RB / 16;                   // 16-byte chunks of it
+  constexpr int CB = CH * 2 < 4 ? CH : 2;       // chunks per ldmatrix of 16 (or 32) keys
   constexpr int MT = D / 16;                    // 16-channel tiles of O^T
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[kWarps][kStages];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  int64_t id = blockIdx.x;
-  const int split = static_cast<int>(id % p.n_splits);
-  id /= p.n_splits;
-  const int rg = static_cast<int>(id % p.n_rg);
-  const int64_t bh = id / p.n_rg;
-  const int b = static_cast<int>(bh / p.Hkv), hk = static_cast<int>(bh - int64_t(b) * p.Hkv);
+  const int per_seq = p.Hkv * p.n_rg;
 
-  int len = static_cast<int>(p.kv_len);
+  // ---- the run [lo, hi) and the group it begins in
+  Group gr;
+  int lo, hi;
   if (p.kv_lens) {
-    const int n = p.kv_lens[b];
-    if (n < 0 || n > len) {
-      if (tid == 0) report_error(p.err, DEV_ERR_INDEX, 311, b, n);
-      len = n < 0 ? 0 : len;
-    } else {
-      len = n;
+    int per = 0;
+    const int total = scan_tiles(p, -1, [&](int n) {
+      per = run_length(n, p.runs);
+      return static_cast<int>(min(int64_t(blockIdx.x) * per, int64_t(n)));
+    }, gr);
+    lo = static_cast<int>(min(int64_t(blockIdx.x) * per, int64_t(total)));
+    hi = min(lo + per, total);
+    if (blockIdx.x == 0)
+      for (int b = tid; b < p.B; b += kThreads)
+        if (p.kv_lens[b] < 0 || p.kv_lens[b] > p.kv_len)
+          report_error(p.err, DEV_ERR_INDEX, 311, b, p.kv_lens[b]);
+  } else {
+    const int all = tiles_of(p.kv_len) * per_seq;
+    lo = blockIdx.x * p.per;
+    hi = min(lo + p.per, all * p.B);
+    gr.b = lo / all;
+    gr.begin = gr.b * all;
+  }
+  if (lo >= hi) return;
+  gr.len = clamp_len(p, gr.b);
+  gr.tiles = tiles_of(gr.len);
+  gr.hg = (lo - gr.begin) / gr.tiles;
+  gr.begin += gr.hg * gr.tiles;
+  auto next_group = [&](Group &x) {
+    x.begin += x.tiles;
+    if (++x.hg == per_seq) {
+      x.hg = 0;
+      x.len = clamp_len(p, ++x.b);
+      x.tiles = tiles_of(x.len);
     }
-  }
-  const int n_tiles_all = (len + kTile - 1) / kTile;
-  const int per = (n_tiles_all + p.n_splits - 1) / p.n_splits;  // tiles of a split
-  const int tile0 = min(split * per, n_tiles_all), tile1 = min(tile0 + per, n_tiles_all);
-
-  const int64_t row0 = bh * p.cap;
-  const uint8_t *kc = reinterpret_cast<const uint8_t *>(p.c.k_codes) + row0 * (D / 2);
-  const uint8_t *vc = reinterpret_cast<const uint8_t *>(p.c.v_codes) + row0 * (D / 2);
-  const uint8_t *ks = reinterpret_cast<const uint8_t *>(p.c.k_scales) + row0 * (NS * 4);
-  const uint8_t *vs = reinterpret_cast<const uint8_t *>(p.c.v_scales) + row0 * (NS * 4);
-  const uint32_t ring = sm100::smem_u32(smem) + warp * L::kRing;
-
-  if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&bars[warp][i], 1);
-    sm100::fence_mbar_init();
-  }
-  __syncwarp();
-  // Copies tile `tl` into a stage (lane 0).  The last tile copies whole groups of
-  // 4 rows: 16-byte sizes at every scale width, inside the capacity (a multiple of 16).
-  auto issue = [&](int tl, int stage) {
-    const int r0 = tl * kTile;
-    const uint32_t n = static_cast<uint32_t>(min(kTile, (len - r0 + 3) & ~3));
-    const uint32_t dst = ring + stage * L::kStage;
-    uint64_t *bar = &bars[warp][stage];
-    sm100::mbar_arrive_expect_tx(bar, n * (D + 8 * NS));
-    bulk_load(dst, kc + int64_t(r0) * (D / 2), n * (D / 2), bar);
-    bulk_load(dst + L::kCodes, ks + int64_t(r0) * (NS * 4), n * (NS * 4), bar);
-    bulk_load(dst + L::kCodes + L::kScales, vc + int64_t(r0) * (D / 2), n * (D / 2), bar);
-    bulk_load(dst + 2 * L::kCodes + L::kScales, vs + int64_t(r0) * (NS * 4), n * (NS * 4), bar);
   };
-  if (lane == 0) {
-    for (int i = 0; i < kStages; ++i)
-      if (tile0 + warp + i * kWarps < tile1) issue(tile0 + warp + i * kWarps, i);
-  }
 
-  // Query rows: row r -> head hk G + r / Sq, position r % Sq.  Column g of an
-  // operand tile holds 8 channels of every 32; accumulator columns are 2t, 2t + 1.
-  uint32_t qf[NT][J][4];
-  uint32_t qm[NT][2];  // 2^-81 sum(Q_t) of group t in three bf16 parts
-  int lim[NT][2];      // keys the column's query sees
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = (rg * NT + nt) * 8 + g;
-    const uint16_t *src = nullptr;
-    if (r < p.R) {
-      const int h = r / p.Sq, s = r - h * p.Sq;
-      src = p.q + ((int64_t(b) * p.Hq + hk * p.G + h) * p.Sq + s) * D;
-    }
-    float sum[NS];
-#pragma unroll
-    for (int j = 0; j < NS; ++j) sum[j] = 0.f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const uint4 x = src ? *reinterpret_cast<const uint4 *>(src + 32 * j + 8 * t)
-                          : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float lo, hi;
-        unpack_bf2(xs[i], lo, hi);
-        sum[j / BPG] += lo + hi;
-        const float up = i % 2 == 0 ? 0x1p52f : 0x1p48f;
-        qf[nt][j][i] = pack_bf2(lo * up, hi * up);
+  uint32_t ring;
+  {
+    const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    ring = base + warp * L::kRing;
+  }
+  float *merge = reinterpret_cast<float *>(smem + kWarps * L::kRing);
+
+  // ---- copies: this warp's tiles lo + warp, + 4, ..., ahead of their use.  Lane i
+  // copies chunks i, i + 32, ... of the tile's codes (chunk c of row r goes to
+  // chunk c ^ swizzle(r)) and chunk i of its scales.  Rows behind the length are
+  // not read (a chunk of narrow scales may hold up to 3 of them: the capacity is
+  // a multiple of 16).
+  constexpr int kCopies = L::kCodes / 512;  // code copies per lane, of K and of V
+  const int crow = lane / CH, cch = lane % CH;
+  const int csw = D == 128 ? (crow >> 1) & 3 : D == 64 ? (crow >> 2) & 1 : 0;
+  const uint32_t cdst = crow * RB + ((cch ^ csw) << 4);
+  const int srow = lane * 4 / NS;           // first row of the lane's chunk of scales
+  Group ahead = gr;
+  int64_t arow = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
+  int next = lo + warp;
+  uint32_t next_stage = 0;  // byte offset in the ring
+  auto issue = [&]() {
+    if (next < hi) {
+      while (next >= ahead.begin + ahead.tiles || ahead.len == 0) {
+        while (next >= ahead.begin + ahead.tiles) next_group(ahead);
+        arow = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
+        if (ahead.len > 0) break;
+        next += kWarps;  // a sequence without rows: nothing to copy
+        if (next >= hi) break;
       }
     }
-    float mine = 0.f;
+    if (next < hi) {
+      const int r0 = (next - ahead.begin) * kTile;
+      const int left = ahead.len - r0;
+      const int64_t row = arow + r0;
+      const uint32_t dst = ring + next_stage;
+      const uint8_t *kc = reinterpret_cast<const uint8_t *>(p.c.k_codes) + row * RB + lane * 16;
+      const uint8_t *vc = reinterpret_cast<const uint8_t *>(p.c.v_codes) + row * RB + lane * 16;
+      if (left >= kTile) {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      float v = sum[j];
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
-      v += __shfl_xor_sync(0xffffffffu, v, 2);
-      if (j == t) mine = v * 0x1p-81f;
+        for (int i = 0; i < kCopies; ++i) {
+          copy16(dst + cdst + i * 512, kc + i * 512, true);
+          copy16(dst + L::kCodes + L::kScales + cdst + i * 512, vc + i * 512, true);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const bool live = crow + i * (32 / CH) < left;
+          copy16(dst + cdst + i * 512, live ? kc + i * 512 : kc, live);
+          copy16(dst + L::kCodes + L::kScales + cdst + i * 512, live ? vc + i * 512 : vc, live);
+        }
+      }
+      if (lane < L::kScales / 16) {
+        const int64_t off = (row * NS + lane * 4) * 4;
+        const bool live = srow < left;
+        copy16(dst + L::kCodes + lane * 16,
+               reinterpret_cast<const uint8_t *>(p.c.k_scales) + (live ? off : 0), live);
+        copy16(dst + 2 * L::kCodes + L::kScales + lane * 16,
+               reinterpret_cast<const uint8_t *>(p.c.v_scales) + (live ? off : 0), live);
+      }
+      next += kWarps;
+      next_stage = next_stage + L::kStage == L::kRing ? 0 : next_stage + L::kStage;
     }
-    const float h0 = bf2f(f2bf(mine)), h1 = bf2f(f2bf(mine - h0));
-    qm[nt][0] = pack_bf2(h0, h1);
-    qm[nt][1] = pack_bf2(mine - h0 - h1, 0.f);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int rc = (rg * NT + nt) * 8 + 2 * t + c;
-      lim[nt][c] = p.causal ? min(len, len - p.Sq + rc % p.Sq + 1) : len;
-    }
-  }
-  const int lim_all = p.causal ? min(len, len - p.Sq + 1) : len;  // keys every query sees
+    copies_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < L::kStages; ++i) issue();
 
-  float o[MT][NT][4];
-  float row_m[NT][2], row_l[NT][2];  // in units of log2; l of this lane's keys only
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    row_m[nt][0] = row_m[nt][1] = -FLT_MAX;
-    row_l[nt][0] = row_l[nt][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
-  }
-
-  const int pig = ((g >> 1) + (g >= 4 ? 4 : 0)) ^ ((g & 1) * 3);  // pi(g)
-  const int pit = t + (t >= 2 ? 4 : 0);                           // pi(2t); pi(2t + 1) = pit ^ 3
-  const int jv = D == 128 ? 2 * (g & 1) : (D == 64 ? (g & 1) : 0);  // 32-channel block of V word 0
-
+  // Addresses within a stage.  K: 4 J bytes of row g (and g + 8) per lane, words
+  // t J .. of it; V: row (lane & 7) of the 8x8 matrix lane / 8.
+  const int ksw = D == 128 ? (g >> 1) & 3 : D == 64 ? (g >> 2) & 1 : 0;
+  const uint32_t koff = g * RB + (D == 128 ? (t ^ ksw) << 4 : D == 64 ? (((t >> 1) ^ ksw) << 4) + (t & 1) * 8
+                                                                    : t * 4);
+  // matrices: D >= 64 (chunk pair, key block of 8): chunk m / 2, keys 8 (m & 1); D = 32: keys 8 m
+  const int vrow = (lane & 7) + (D == 32 ? lane & 24 : lane & 8);
+  const int vsw = D == 128 ? (vrow >> 1) & 3 : D == 64 ? (vrow >> 2) & 1 : 0;
+  const int vch = D == 32 ? 0 : lane >> 4;
+  const int gv = (D == 128 ? g >> 1 : D == 64 ? (g >> 1) & 1 : 0) / BPG;  // the lane's V scale group
+  const uint32_t vsoff = (2 * t * NS + gv) * 4;
   constexpr uint32_t kUpS = pow2_bf16(69) * 0x10001u, kDownM0 = pow2_bf16(-64) * 0x10001u,
                      kDownM1 = pow2_bf16(-60) * 0x10001u;
   const float scale_up = p.scale_log2 * 0x1p81f;
-  bool ok = true;
-  int stage = 0, phase = 0;
-  int tl = tile0 + warp;
-  for (; tl < tile1; tl += kWarps) {
-    if (!sm100::mbar_wait(&bars[warp][stage], phase)) {
-      report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 312, static_cast<int>(bh), tl);
-      ok = false;
-      break;
-    }
-    const uint32_t sk = ring + stage * L::kStage;
-    const uint32_t sks = sk + L::kCodes, sv = sks + L::kScales, svs = sv + L::kCodes;
-    const int key0 = tl * kTile;
-    const bool masked = key0 + kTile > lim_all;
+  uint32_t stage = 0;
+  int mine = lo + warp;  // this warp's next tile
 
-    // ---- S^T = K Q^T (two blocks of 16 keys), in units of log2
-    float s[2][NT][4];
+  for (int at = lo; at < hi;) {
+    // ---- one group's part of the run: tiles [at, end)
+    const int end = min(hi, gr.begin + gr.tiles);
+    const int b = gr.b, hk = gr.hg / p.n_rg, rg = gr.hg - hk * p.n_rg, len = gr.len;
+
+    // Query rows: row r -> head hk G + r / Sq, position r % Sq.  Column g of an
+    // operand tile holds 8 channels of every 32; accumulator columns are 2t, 2t + 1.
+    uint32_t qf[NT][J][4];
+    uint32_t qm[NT][2];  // 2^-81 sum(Q_t) of group t in three bf16 parts
+    int lim[NT][2];      // keys the column's query sees
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      uint32_t wl[J], wh[J], pl[NS], ph[NS], ml[1], mh[1];
-      const int kl = 16 * mt + pig;
-      lds_words<J>(wl, sk + kl * (D / 2) + t * (4 * J));
-      lds_words<J>(wh, sk + (kl + 8) * (D / 2) + t * (4 * J));
-      lds_words<NS>(pl, sks + kl * (NS * 4));
-      lds_words<NS>(ph, sks + (kl + 8) * (NS * 4));
-      lds_words<1>(ml, sks + (kl * NS + t % NS) * 4);
-      lds_words<1>(mh, sks + ((kl + 8) * NS + t % NS) * 4);
-      // minima: (m, m, m) of group t times the parts of its sum(Q)
-      const uint32_t m0 = __byte_perm(ml[0], 0u, 0x3232), m1 = __byte_perm(mh[0], 0u, 0x3232);
-      float part[NT][4];
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = (rg * NT + nt) * 8 + g;
+      const uint16_t *src = nullptr;
+      if (r < p.R) {
+        const int h = r / p.Sq, s = r - h * p.Sq;
+        src = p.q + ((int64_t(b) * p.Hq + hk * p.G + h) * p.Sq + s) * D;
+      }
+      float sum[NS];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        mma(s[mt][nt], m0, m1, m0, m1, qm[nt][0], qm[nt][1], 0.f, 0.f, 0.f, 0.f);
+      for (int j = 0; j < NS; ++j) sum[j] = 0.f;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        uint32_t a[4], c[4];
-        codes4(wl[j], a);
-        codes4(wh[j], c);
-        const int sg = j / BPG;
+        const uint4 x = src ? *reinterpret_cast<const uint4 *>(src + 32 * j + 8 * t)
+                            : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (j % BPG == 0)
-            mma(part[nt], a[0], c[0], a[1], c[1], qf[nt][j][0], qf[nt][j][1], 0.f, 0.f, 0.f, 0.f);
-          else
-            mma(part[nt], a[0], c[0], a[1], c[1], qf[nt][j][0], qf[nt][j][1], part[nt][0],
-                part[nt][1], part[nt][2], part[nt][3]);
-          mma(part[nt], a[2], c[2], a[3], c[3], qf[nt][j][2], qf[nt][j][3], part[nt][0],
-              part[nt][1], part[nt][2], part[nt][3]);
-        }
-        if (j % BPG == BPG - 1) {
-          const float s0 = __uint_as_float(pl[sg] << 16), s1 = __uint_as_float(ph[sg] << 16);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            s[mt][nt][0] = fmaf(s0, part[nt][0], s[mt][nt][0]);
-            s[mt][nt][1] = fmaf(s0, part[nt][1], s[mt][nt][1]);
-            s[mt][nt][2] = fmaf(s1, part[nt][2], s[mt][nt][2]);
-            s[mt][nt][3] = fmaf(s1, part[nt][3], s[mt][nt][3]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          float lo, hi;
+          unpack_bf2(xs[i], lo, hi);
+          sum[j / BPG] += lo + hi;
+          const float up = i % 2 == 0 ? 0x1p52f : 0x1p48f;
+          qf[nt][j][i] = pack_bf2(lo * up, hi * up);
         }
       }
+      float mine = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < NS; ++j) {
+        float v = sum[j];
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        if (j == t) mine = v * 0x1p-81f;
+      }
+      const float h0 = bf2f(f2bf(mine)), h1 = bf2f(f2bf(mine - h0));
+      qm[nt][0] = pack_bf2(h0, h1);
+      qm[nt][1] = pack_bf2(mine - h0 - h1, 0.f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][nt][e] *= scale_up;
+      for (int c = 0; c < 2; ++c) {
+        const int rc = (rg * NT + nt) * 8 + 2 * t + c;
+        lim[nt][c] = p.causal ? min(len, len - p.Sq + rc % p.Sq + 1) : len;
+      }
+    }
+    const int lim_all = p.causal ? min(len, len - p.Sq + 1) : len;  // keys every query sees
+
+    float o[MT][NT][4];
+    float row_m[NT][2], row_l[NT][2];  // in units of log2; l of this lane's keys only
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      row_m[nt][0] = row_m[nt][1] = -FLT_MAX;
+      row_l[nt][0] = row_l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
     }
 
-    if (masked) {
+    for (; mine < end; mine += kWarps) {
+      if (len == 0) continue;
+      copies_wait<L::kStages - 1>();
+      __syncwarp();
+      const uint32_t sk = ring + stage;
+      const uint32_t sks = sk + L::kCodes, sv = sks + L::kScales, svs = sv + L::kCodes;
+      const int key0 = (mine - gr.begin) * kTile;
+
+      // ---- S^T = K Q^T (two blocks of 16 keys), in units of log2
+      float s[2][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t wl[J], wh[J], pl[NS], ph[NS];
+        const int kl = 16 * mt + g;
+        lds_words<J>(wl, sk + 16 * mt * RB + koff);
+        lds_words<J>(wh, sk + (16 * mt + 8) * RB + koff);
+        lds_words<NS>(pl, sks + kl * (NS * 4));
+        lds_words<NS>(ph, sks + (kl + 8) * (NS * 4));
+        // minima: (m, m, m) of group t times the parts of its sum(Q)
+        const uint32_t m0 = __byte_perm(lds1(sks + (kl * NS + t % NS) * 4), 0u, 0x3232);
+        const uint32_t m1 = __byte_perm(lds1(sks + ((kl + 8) * NS + t % NS) * 4), 0u, 0x3232);
+        float part[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma(s[mt][nt], m0, m1, m0, m1, qm[nt][0], qm[nt][1], 0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          uint32_t a[4], c[4];
+          codes4(wl[j], a);
+          codes4(wh[j], c);
+          const int sg = j / BPG;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (j % BPG == 0)
+              mma(part[nt], a[0], c[0], a[1], c[1], qf[nt][j][0], qf[nt][j][1], 0.f, 0.f, 0.f, 0.f);
+            else
+              mma(part[nt], a[0], c[0], a[1], c[1], qf[nt][j][0], qf[nt][j][1], part[nt][0],
+                  part[nt][1], part[nt][2], part[nt][3]);
+            mma(part[nt], a[2], c[2], a[3], c[3], qf[nt][j][2], qf[nt][j][3], part[nt][0],
+                part[nt][1], part[nt][2], part[nt][3]);
+          }
+          if (j % BPG == BPG - 1) {
+            const float s0 = __uint_as_float(pl[sg] << 16), s1 = __uint_as_float(ph[sg] << 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              s[mt][nt][0] = fmaf(s0, part[nt][0], s[mt][nt][0]);
+              s[mt][nt][1] = fmaf(s0, part[nt][1], s[mt][nt][1]);
+              s[mt][nt][2] = fmaf(s1, part[nt][2], s[mt][nt][2]);
+              s[mt][nt][3] = fmaf(s1, part[nt][3], s[mt][nt][3]);
+            }
+          }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key0 + 16 * mt + pig + 8 * (e >> 1) >= lim[nt][e & 1]) s[mt][nt][e] = -INFINITY;
-      // A weight of 0 does not silence a NaN or an infinity in V: rows behind the
-      // length are cleared, and a non-finite group that some query must not see is
-      // cleared too and put into the outputs of the queries that do see it.
-      const bool behind = key0 + lane >= len;
-      uint32_t clear = behind ? (1u << NS) - 1u : 0u;  // groups of key row `lane`
-      if (!behind) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          uint32_t w[1];
-          lds_words<1>(w, svs + (lane * NS + i) * 4);
-          if (nonfinite(w[0])) clear |= 1u << i;
-        }
+          for (int e = 0; e < 4; ++e) s[mt][nt][e] *= scale_up;
       }
-      uint32_t todo = __ballot_sync(0xffffffffu, clear != 0 && !behind);
-      while (todo) {
-        const int kk = __ffs(todo) - 1;
-        todo &= todo - 1;
+
+      if (key0 + kTile > lim_all) {
 #pragma unroll
-        for (int w = 0; w < WV; ++w) {
-          uint32_t pr[1];
-          lds_words<1>(pr, svs + (kk * NS + (jv + w) / BPG) * 4);
-          if (nonfinite(pr[0])) {
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + 16 * mt + g + 8 * (e >> 1) >= lim[nt][e & 1]) s[mt][nt][e] = -INFINITY;
+        // A weight of 0 does not silence a NaN or an infinity in V: rows behind the
+        // length are cleared, and a non-finite group that some query must not see is
+        // cleared too and put into the outputs of the queries that do see it.
+        const bool behind = key0 + lane >= len;
+        uint32_t clear = behind ? (1u << NS) - 1u : 0u;  // groups of key row `lane`
+        if (!behind) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+            if (nonfinite(lds1(svs + (lane * NS + i) * 4))) clear |= 1u << i;
+        }
+        uint32_t todo = __ballot_sync(0xffffffffu, clear != 0 && !behind);
+        while (todo) {
+          const int kk = __ffs(todo) - 1;
+          todo &= todo - 1;
+          if (nonfinite(lds1(svs + (kk * NS + gv) * 4))) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int i = 0; i < MT / WV; ++i)
+              for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  if (key0 + kk < lim[nt][e & 1]) o[w * (MT / WV) + i][nt][e] = NAN;
+                  if (key0 + kk < lim[nt][e & 1]) o[i][nt][e] = NAN;
           }
         }
-      }
-      __syncwarp();
-      if (clear) {
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < NS; ++i)
           if (clear >> i & 1u)
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(svs + (lane * NS + i) * 4), "r"(0u) : "memory");
+        __syncwarp();
       }
-      __syncwarp();
-    }
 
-    // ---- softmax: the maximum is raised (and O rescaled) only when some key exceeds it
-    uint32_t pb[2][NT][2];
+      // ---- softmax: the maximum is raised (and O rescaled) only when some key exceeds it
+      uint32_t pb[2][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float mx0 = fmaxf(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[1][nt][0], s[1][nt][2]));
-      float mx1 = fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3]));
-      if (__any_sync(0xffffffffu, mx0 > row_m[nt][0] || mx1 > row_m[nt][1])) {
+      for (int nt = 0; nt < NT; ++nt) {
+        float mx0 = fmaxf(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[1][nt][0], s[1][nt][2]));
+        float mx1 = fmaxf(fmaxf(s[0][nt][1], s[0][nt][3]), fmaxf(s[1][nt][1], s[1][nt][3]));
+        if (__any_sync(0xffffffffu, mx0 > row_m[nt][0] || mx1 > row_m[nt][1])) {
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+          for (int d = 4; d < 32; d <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+          }
+          mx0 = fmaxf(mx0, row_m[nt][0]);
+          mx1 = fmaxf(mx1, row_m[nt][1]);
+          const float a0 = exp2_fast(row_m[nt][0] - mx0), a1 = exp2_fast(row_m[nt][1] - mx1);
+          row_m[nt][0] = mx0;
+          row_m[nt][1] = mx1;
+          row_l[nt][0] *= a0;
+          row_l[nt][1] *= a1;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            o[i][nt][0] *= a0;
+            o[i][nt][1] *= a1;
+            o[i][nt][2] *= a0;
+            o[i][nt][3] *= a1;
+          }
         }
-        mx0 = fmaxf(mx0, row_m[nt][0]);
-        mx1 = fmaxf(mx1, row_m[nt][1]);
-        const float a0 = exp2_fast(row_m[nt][0] - mx0), a1 = exp2_fast(row_m[nt][1] - mx1);
-        row_m[nt][0] = mx0;
-        row_m[nt][1] = mx1;
-        row_l[nt][0] *= a0;
-        row_l[nt][1] *= a1;
+        const float mu0 = row_m[nt][0], mu1 = row_m[nt][1];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          o[i][nt][0] *= a0;
-          o[i][nt][1] *= a1;
-          o[i][nt][2] *= a0;
-          o[i][nt][3] *= a1;
+        for (int mt = 0; mt < 2; ++mt) {
+          const float p0 = exp2_fast(s[mt][nt][0] - mu0), p1 = exp2_fast(s[mt][nt][1] - mu1);
+          const float p2 = exp2_fast(s[mt][nt][2] - mu0), p3 = exp2_fast(s[mt][nt][3] - mu1);
+          row_l[nt][0] += p0 + p2;
+          row_l[nt][1] += p1 + p3;
+          pb[mt][nt][0] = transpose8x8(pack_bf2(p0, p1));
+          pb[mt][nt][1] = transpose8x8(pack_bf2(p2, p3));
         }
       }
-      const float mu0 = row_m[nt][0], mu1 = row_m[nt][1];
+
+      // ---- O^T += V^T P^T
+      uint32_t u[4];
+      if constexpr (D == 32) ldsm4_t(u, sv + vrow * RB);  // keys 0-7, 8-15, 16-23, 24-31
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        const float p0 = exp2_fast(s[mt][nt][0] - mu0), p1 = exp2_fast(s[mt][nt][1] - mu1);
-        const float p2 = exp2_fast(s[mt][nt][2] - mu0), p3 = exp2_fast(s[mt][nt][3] - mu1);
-        row_l[nt][0] += p0 + p2;
-        row_l[nt][1] += p1 + p3;
-        pb[mt][nt][0] = transpose8x8(pack_bf2(p0, p1));
-        pb[mt][nt][1] = transpose8x8(pack_bf2(p2, p3));
-      }
-    }
-
-    // ---- O^T += V^T P^T
+        // scale pairs of keys (2t, 2t + 1) and (2t + 8, 2t + 9), with their powers of two
+        uint32_t s2[2], m2[2][2];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const int ka = 16 * mt + pit, kb = 16 * mt + (pit ^ 3);
-      uint32_t wa[WV], wb[WV], wa8[WV], wb8[WV];
-      if constexpr (D == 32) {
-        wa[0] = lds_u16(sv + ka * 16 + g * 2);
-        wb[0] = lds_u16(sv + kb * 16 + g * 2);
-        wa8[0] = lds_u16(sv + (ka + 8) * 16 + g * 2);
-        wb8[0] = lds_u16(sv + (kb + 8) * 16 + g * 2);
-      } else {
-        lds_words<WV>(wa, sv + ka * (D / 2) + g * (4 * WV));
-        lds_words<WV>(wb, sv + kb * (D / 2) + g * (4 * WV));
-        lds_words<WV>(wa8, sv + (ka + 8) * (D / 2) + g * (4 * WV));
-        lds_words<WV>(wb8, sv + (kb + 8) * (D / 2) + g * (4 * WV));
-      }
-      constexpr int PS = WV > BPG ? WV / BPG : 1;  // scale words per lane and key
-      uint32_t pa[PS], pbb[PS], pa8[PS], pb8[PS];
-      lds_words<PS>(pa, svs + (ka * NS + jv / BPG) * 4);
-      lds_words<PS>(pbb, svs + (kb * NS + jv / BPG) * 4);
-      lds_words<PS>(pa8, svs + ((ka + 8) * NS + jv / BPG) * 4);
-      lds_words<PS>(pb8, svs + ((kb + 8) * NS + jv / BPG) * 4);
-#pragma unroll
-      for (int w = 0; w < WV; ++w) {
-        const int sw = w * PS / WV;
-        // (key a, key b) pairs of scales and minima, with their powers of two, and of codes
-        const uint32_t s2 = mul2(__byte_perm(pa[sw], pbb[sw], 0x5410), kUpS);
-        const uint32_t m2[2] = {mul2(__byte_perm(pa[sw], pbb[sw], 0x7632), kDownM0),
-                                mul2(__byte_perm(pa[sw], pbb[sw], 0x7632), kDownM1)};
-        const uint32_t s28 = mul2(__byte_perm(pa8[sw], pb8[sw], 0x5410), kUpS);
-        const uint32_t m28[2] = {mul2(__byte_perm(pa8[sw], pb8[sw], 0x7632), kDownM0),
-                                 mul2(__byte_perm(pa8[sw], pb8[sw], 0x7632), kDownM1)};
-        uint32_t x[4], x8[4], y[4], y8[4];
-        codes4(__byte_perm(wa[w], wb[w], 0x5410), x);
-        codes4(__byte_perm(wa8[w], wb8[w], 0x5410), x8);
-        if constexpr (D > 32) {
-          codes4(__byte_perm(wa[w], wb[w], 0x7632), y);
-          codes4(__byte_perm(wa8[w], wb8[w], 0x7632), y8);
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t at0 = svs + vsoff + (16 * mt + 8 * h) * (NS * 4);
+          const uint32_t pa = lds1(at0), pc = lds1(at0 + NS * 4);
+          s2[h] = mul2(__byte_perm(pa, pc, 0x5410), kUpS);
+          const uint32_t mm = __byte_perm(pa, pc, 0x7632);
+          m2[h][0] = mul2(mm, kDownM0);
+          m2[h][1] = mul2(mm, kDownM1);
         }
-#pragma unroll
-        for (int i = 0; i < MT / WV; ++i) {
-          // channels of rows g and g + 8: fields i, i + 4 (D = 32: i, i + 2 of a half word)
-          const uint32_t a0 = fma2(x[i], s2, m2[i % 2]);
-          const uint32_t a1 = fma2(D == 32 ? x[i + 2] : y[i], s2, m2[i % 2]);
-          const uint32_t a2 = fma2(x8[i], s28, m28[i % 2]);
-          const uint32_t a3 = fma2(D == 32 ? x8[i + 2] : y8[i], s28, m28[i % 2]);
+        auto product = [&](int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int i) {
+          a0 = fma2(a0, s2[0], m2[0][i]);
+          a1 = fma2(a1, s2[0], m2[0][i]);
+          a2 = fma2(a2, s2[1], m2[1][i]);
+          a3 = fma2(a3, s2[1], m2[1][i]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float(&acc)[4] = o[w * (MT / WV) + i][nt];
+            float(&acc)[4] = o[tile][nt];
             mma(acc, a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1], acc[0], acc[1], acc[2], acc[3]);
+          }
+        };
+        if constexpr (D == 32) {
+          // rows g and g + 8 of tile i: fields i and i + 2 of the lane's unit
+          uint32_t x[4], y[4];
+          codes4(u[2 * mt], x);
+          codes4(u[2 * mt + 1], y);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) product(i, x[i], x[i + 2], y[i], y[i + 2], i);
+        } else {
+#pragma unroll
+          for (int cp = 0; cp < CH / 2; ++cp) {
+            // matrices: (chunk 2cp, keys 0-7), (2cp, 8-15), (2cp + 1, 0-7), (2cp + 1, 8-15);
+            // rows g and g + 8 of tile 4 cp + i: field i of the unit in chunks 2cp and 2cp + 1
+            ldsm4_t(u, sv + (16 * mt + vrow) * RB + (((2 * cp + vch) ^ vsw) << 4));
+            uint32_t x[4], x8[4], y[4], y8[4];
+            codes4(u[0], x);
+            codes4(u[1], x8);
+            codes4(u[2], y);
+            codes4(u[3], y8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) product(4 * cp + i, x[i], y[i], x8[i], y8[i], i % 2);
           }
         }
       }
+      __syncwarp();
+      issue();
+      stage = stage + L::kStage == L::kRing ? 0 : stage + L::kStage;
     }
-    // cleared scales (ordinary stores) before the next bulk copy into this stage
-    if (masked) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0 && tl + kStages * kWarps < tile1) issue(tl + kStages * kWarps, stage);
-    if (++stage == kStages) {
-      stage = 0;
-      phase ^= 1;
-    }
-  }
-  if (!ok) {
-    // give up: let the copies still in flight land (bounded) before the block ends
-    for (int i = 1; i < kStages; ++i) {
-      tl += kWarps;
-      if (++stage == kStages) {
-        stage = 0;
-        phase ^= 1;
-      }
-      if (tl < tile1) sm100::mbar_wait(&bars[warp][stage], phase);
-    }
-  }
 
-  // ---- join the warps: [warp][row][D channels, m, l]
+    // ---- join the warps (lane i of every warp holds the same rows and channels)
+    // and write the group's rows or its partials
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][nt][e] *= i % 2 == 0 ? 0x1p64f : 0x1p60f;
+        for (int e = 0; e < 4; ++e) o[i][nt][e] *= i % 2 == 0 ? 0x1p64f : 0x1p60f;
+    __syncthreads();
+    if (warp > 0) {
+      float *dst = merge + (warp - 1) * (L::kRegs * 32) + lane;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1)
-        row_l[nt][c] += __shfl_xor_sync(0xffffffffu, row_l[nt][c], d);
-  __syncthreads();
-  float *sm = reinterpret_cast<float *>(smem);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float *row = sm + (warp * 8 * NT + nt * 8 + 2 * t + c) * L::kRowF;
-      if constexpr (D == 32) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          row[8 * (g >> 1) + 2 * i + (g & 1)] = o[i][nt][c];
-          row[8 * (g >> 1) + 2 * (i + 2) + (g & 1)] = o[i][nt][c + 2];
+        for (int c = 0; c < 2; ++c) {
+          dst[((D / 4 + 4) * nt + c) * 32] = row_m[nt][c];
+          dst[((D / 4 + 4) * nt + 2 + c) * 32] = row_l[nt][c];
         }
-      } else {
 #pragma unroll
-        for (int w = 0; w < WV; ++w) {
-          float4 *dst = reinterpret_cast<float4 *>(row + 32 * (jv + w) + 8 * (g >> 1));
-          const int i0 = w * (MT / WV);
-          dst[0] = make_float4(o[i0][nt][c], o[i0][nt][c + 2], o[i0 + 1][nt][c], o[i0 + 1][nt][c + 2]);
-          dst[1] = make_float4(o[i0 + 2][nt][c], o[i0 + 2][nt][c + 2], o[i0 + 3][nt][c],
-                               o[i0 + 3][nt][c + 2]);
-        }
-      }
-      if (g == 0) {
-        row[D] = row_m[nt][c];
-        row[D + 1] = row_l[nt][c];
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[((D / 4 + 4) * nt + 4 + 4 * i + e) * 32] = o[i][nt][e];
       }
     }
-  __syncthreads();
-  for (int it = tid; it < 8 * NT * (D / 4); it += kThreads) {
-    const int lr = it / (D / 4), ch = (it - lr * (D / 4)) * 4;
-    const int r = rg * 8 * NT + lr;
-    if (r >= p.R) continue;
-    float M = -FLT_MAX;
+    __syncthreads();
+    if (warp == 0) {
+      const bool whole = at == gr.begin && end == gr.begin + gr.tiles;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm[(w * 8 * NT + lr) * L::kRowF + D]);
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int nt = 0; nt < NT; ++nt) {
+        const float *src = merge + (D / 4 + 4) * nt * 32 + lane;
+        float f[kWarps][2], l[2], m[2];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float *row = sm + (w * 8 * NT + lr) * L::kRowF;
-      const float f = exp2_fast(row[D] - M);
-      l += row[D + 1] * f;
-      const float4 x = *reinterpret_cast<const float4 *>(row + ch);
-      acc.x += x.x * f;
-      acc.y += x.y * f;
-      acc.z += x.z * f;
-      acc.w += x.w * f;
+        for (int c = 0; c < 2; ++c) {
+          float mw[kWarps - 1];
+          m[c] = row_m[nt][c];
+#pragma unroll
+          for (int w = 0; w < kWarps - 1; ++w) {
+            mw[w] = src[(w * L::kRegs + c) * 32];
+            m[c] = fmaxf(m[c], mw[w]);
+          }
+          f[0][c] = exp2_fast(row_m[nt][c] - m[c]);
+          l[c] = row_l[nt][c] * f[0][c];
+#pragma unroll
+          for (int w = 0; w < kWarps - 1; ++w) {
+            f[w + 1][c] = exp2_fast(mw[w] - m[c]);
+            l[c] = fmaf(src[(w * L::kRegs + 2 + c) * 32], f[w + 1][c], l[c]);
+          }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = o[i][nt][e] * f[0][e & 1];
+#pragma unroll
+            for (int w = 0; w < kWarps - 1; ++w)
+              v = fmaf(src[(w * L::kRegs + 4 + 4 * i + e) * 32], f[w + 1][e & 1], v);
+            o[i][nt][e] = v;
+          }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int lr = nt * 8 + 2 * t + c, r = rg * 8 * NT + lr;
+          const bool live = r < p.R;
+          const float inv = !whole ? 1.f : l[c] == 0.f ? 0.f : 1.0f / l[c];
+          const int h = r / p.Sq, sq = r - h * p.Sq;
+          uint16_t *dst = p.out + ((int64_t(b) * p.Sq + sq) * p.Hq + hk * p.G + h) * D;
+          const int64_t row = (2 * int64_t(blockIdx.x) + (at == gr.begin ? 1 : 0)) * (8 * NT) + lr;
+          // A unit is channels 32 j + 8 k + 2 i + (g & 1), i = 0..3: lanes g and g ^ 1 hold
+          // the even and the odd ones and trade halves, for four neighbours each.
+#pragma unroll
+          for (int un = 0; un < (D == 32 ? 1 : CH); ++un) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              x[i] = (D == 32 ? o[i % 2][nt][c + 2 * (i / 2)]
+                              : o[4 * (un / 2) + i][nt][c + 2 * (un % 2)]) * inv;
+            const bool odd = g & 1;
+            const float r0 = __shfl_xor_sync(0xffffffffu, odd ? x[0] : x[2], 4);
+            const float r1 = __shfl_xor_sync(0xffffffffu, odd ? x[1] : x[3], 4);
+            const float4 v = odd ? make_float4(r0, x[2], r1, x[3]) : make_float4(x[0], r0, x[1], r1);
+            const int j = D == 128 ? g >> 1 : D == 64 ? (g >> 1) & 1 : 0;
+            const int k = D == 128 ? un : D == 64 ? 2 * un + (g >> 2) : g >> 1;
+            const int ch = 32 * j + 8 * k + (odd ? 4 : 0);
+            if (live && whole)
+              *reinterpret_cast<uint2 *>(dst + ch) = make_uint2(pack_bf2(v.x, v.y), pack_bf2(v.z, v.w));
+            if (live && !whole) *reinterpret_cast<float4 *>(p.ws + row * D + ch) = v;
+          }
+          if (live && !whole && g == 0)
+            reinterpret_cast<float2 *>(p.ws + partial_rows(p.runs, NT) * D)[row] =
+                make_float2(m[c], l[c]);
+        }
+      }
     }
-    if (p.n_splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      const int h = r / p.Sq, sq = r - h * p.Sq;
-      uint2 v = make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
-      *reinterpret_cast<uint2 *>(p.out + ((int64_t(b) * p.Sq + sq) * p.Hq + hk * p.G + h) * D + ch) = v;
-    } else {
-      const int64_t rows = int64_t(gridDim.x) / (int64_t(p.n_splits) * p.n_rg) * p.R * p.n_splits;
-      const int64_t at = (bh * p.R + r) * p.n_splits + split;
-      *reinterpret_cast<float4 *>(p.ws + at * D + ch) = acc;
-      if (ch == 0) *reinterpret_cast<float2 *>(p.ws + rows * D + at * 2) = make_float2(M, l);
-    }
+    at = end;
+    if (at < hi) next_group(gr);
   }
+  copies_wait<0>();
 }
 
-// One warp per query row: joins the splits.
+// One CTA per query row: joins the runs that share the row's group.
 template <int D>
-__global__ void __launch_bounds__(128) attn_q4_join_kernel(Params p, int64_t rows) {
+__global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(Params p, int rows_per_group) {
   constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t gr = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (gr >= rows) return;
-  const float2 *ml = reinterpret_cast<const float2 *>(p.ws + rows * p.n_splits * D) + gr * p.n_splits;
-  const float *acc = p.ws + gr * p.n_splits * D + lane * E;
+  __shared__ float part[kWarps][D], part_l[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t gr = blockIdx.x;
+  const int64_t bh = gr / p.R;
+  const int r = static_cast<int>(gr - bh * p.R);
+  const int b = static_cast<int>(bh / p.Hkv), hk = static_cast<int>(bh - int64_t(b) * p.Hkv);
+  const int rg = r / rows_per_group, lr = r - rg * rows_per_group;
+  int per = p.per, begin;
+  const int tiles = tiles_of(clamp_len(p, b));
+  if (p.kv_lens) {
+    Group gs;
+    const int total = scan_tiles(p, b, [](int) { return 0; }, gs);
+    per = run_length(total, p.runs);
+    begin = gs.begin;
+  } else {
+    begin = b * p.Hkv * p.n_rg * tiles;
+  }
+  begin += (hk * p.n_rg + rg) * tiles;
+  const int c0 = begin / per;
+  const int n = (begin + tiles - 1) / per - c0 + 1;
+  if (n == 1) return;  // one run held the group and wrote the row
+  auto slot = [&](int i) {
+    return (2 * (int64_t(c0) + i) + (i == 0 ? 1 : 0)) * rows_per_group + lr;
+  };
+  const float2 *ml = reinterpret_cast<const float2 *>(p.ws + 2 * int64_t(p.runs) * rows_per_group * D);
   float M = -FLT_MAX;
-  for (int s = lane; s < p.n_splits; s += 32) M = fmaxf(M, ml[s].x);
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[slot(i)].x);
   M = warp_max(M);
   float l = 0.f, v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < p.n_splits; ++s) {
-    const float2 x = ml[s];
+  for (int i = warp; i < n; i += kWarps) {
+    const int64_t at = slot(i);
+    const float2 x = ml[at];
     const float f = exp2_fast(x.x - M);
     l += x.y * f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] += acc[int64_t(s) * D + e] * f;
+    for (int e = 0; e < E; ++e) v[e] = fmaf(p.ws[at * D + 32 * e + lane], f, v[e]);
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const int64_t bh = gr / p.R;
-  const int r = static_cast<int>(gr - bh * p.R);
-  const int64_t b = bh / p.Hkv;
-  const int hk = static_cast<int>(bh - b * p.Hkv), h = r / p.Sq, sq = r - h * p.Sq;
-  uint16_t *dst = p.out + ((b * p.Sq + sq) * p.Hq + hk * p.G + h) * D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = f2bf(v[e] * inv);
+  for (int e = 0; e < E; ++e) part[warp][32 * e + lane] = v[e];
+  if (lane == 0) part_l[warp] = l;
+  __syncthreads();
+  if (tid < D) {
+    const float lt = (part_l[0] + part_l[1]) + (part_l[2] + part_l[3]);
+    const float x = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+    const int h = r / p.Sq, sq = r - h * p.Sq;
+    p.out[((int64_t(b) * p.Sq + sq) * p.Hq + hk * p.G + h) * D + tid] = f2bf(x * inv);
+  }
 }
 
-// Rows per CTA and splits of the keys.
+// Query rows per CTA, and the runs the tiles are cut into.
 struct Plan {
-  int nt, n_rg, n_splits;
+  int nt, n_rg, runs, per;
+  bool join;
 };
-Plan plan(int64_t B, int Hkv, int64_t R, int64_t kv_len) {
-  Plan pl;
+int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, bool lens) {
   pl.nt = R > 8 ? 2 : 1;
-  pl.n_rg = static_cast<int>((R + 8 * pl.nt - 1) / (8 * pl.nt));
-  const int64_t groups = B * Hkv * pl.n_rg;
-  const int64_t want = (2LL * 148 * 3) / (groups > 0 ? groups : 1);
-  const int64_t most = (kv_len + 4 * kTile - 1) / (4 * kTile);
-  int64_t n = want < most ? want : most;
-  pl.n_splits = static_cast<int>(n < 1 ? 1 : n);
-  return pl;
+  const int64_t n_rg = (R + 8 * pl.nt - 1) / (8 * pl.nt);
+  const int64_t tiles = kv_len > 0 ? (kv_len + kTile - 1) / kTile : 1;
+  // all tiles, runs and rows of the list are counted in 31 bits
+  if (B >= (int64_t(1) << 31) || R >= (int64_t(1) << 31) || Hkv * n_rg >= (int64_t(1) << 31) ||
+      B * Hkv * R >= (int64_t(1) << 31) || tiles * B >= (int64_t(1) << 31) / (Hkv * n_rg))
+    return fail(Q35_ERR_SHAPE, "attn_q4: too many query rows or key tiles");
+  pl.n_rg = static_cast<int>(n_rg);
+  const int total = static_cast<int>(tiles * B * Hkv * n_rg);
+  const int slots = num_sms() * ctas_per_sm(pl.nt);
+  pl.runs = (total + kWarps - 1) / kWarps;  // at least a tile for each warp
+  if (pl.runs > slots) pl.runs = slots;
+  pl.per = run_length(total, pl.runs);
+  if (!lens) pl.runs = (total + pl.per - 1) / pl.per;
+  pl.join = pl.runs > 1 && (lens || pl.per % static_cast<int>(tiles) != 0);
+  return Q35_OK;
 }
 
 }  // namespace
@@ -637,9 +812,9 @@ using namespace q35;
 extern "C" int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                          int D) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || Sq <= 0 || D <= 0) return 0;
-  const Plan pl = plan(B, Hkv, Hq / Hkv * Sq, kv_len);
-  if (pl.n_splits == 1) return 0;
-  return B * Hq * Sq * pl.n_splits * (static_cast<int64_t>(D) + 2);
+  Plan pl;  // with kv_lens: never fewer runs than without
+  if (plan(pl, B, Hkv, Hq / Hkv * Sq, kv_len, true) != Q35_OK || !pl.join) return 0;
+  return partial_rows(pl.runs, pl.nt) * (static_cast<int64_t>(D) + 2);
 }
 
 extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_scales,
@@ -661,10 +836,11 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
   if (!aligned16(q) || !aligned16(out))
     return fail(Q35_ERR_ALIGN, "attn_q4: q, out not 16-byte aligned");
   const int64_t R = Hq / Hkv * Sq;
-  if (R >= (int64_t(1) << 30)) return fail(Q35_ERR_SHAPE, "attn_q4: %lld query rows", (long long)R);
-  const Plan pl = plan(B, Hkv, R, kv_len);
-  if (pl.n_splits > 1 && !workspace) return fail(Q35_ERR_INVALID, "attn_q4: no workspace");
-  if (pl.n_splits > 1 && !aligned16(workspace))
+  Plan pl;
+  const int ps = plan(pl, B, Hkv, R, kv_len, kv_lens != nullptr);
+  if (ps) return ps;
+  if (pl.join && !workspace) return fail(Q35_ERR_INVALID, "attn_q4: no workspace");
+  if (pl.join && !aligned16(workspace))
     return fail(Q35_ERR_ALIGN, "attn_q4: workspace not 16-byte aligned");
   int *err = device_error_word();
   if (!err) return fail(Q35_ERR_CUDA, "attn_q4: no device error word");
@@ -684,24 +860,24 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
   p.Sq = static_cast<int>(Sq);
   p.R = static_cast<int>(R);
   p.n_rg = pl.n_rg;
-  p.n_splits = pl.n_splits;
+  p.B = static_cast<int>(B);
+  p.runs = pl.runs;
+  p.per = pl.per;
   p.causal = causal ? 1 : 0;
-  p.kv_len = kv_len;
+  p.kv_len = static_cast<int>(kv_len);
   p.cap = cap;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const int64_t blocks = B * Hkv * pl.n_rg * pl.n_splits, rows = B * Hkv * R;
-  if (blocks >= (int64_t(1) << 31) || rows >= (int64_t(1) << 32))
-    return fail(Q35_ERR_SHAPE, "attn_q4: too many rows");
+  const int64_t rows = B * Hkv * R;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto d, auto gs, auto nt) -> int {
     auto *kern = &attn_q4_kernel<d(), gs(), nt()>;
-    constexpr int smem = Layout<d(), gs()>::smem(nt());
+    constexpr int smem = Layout<d(), gs(), nt()>::kSmem;
     const int e = ensure_smem_attr(reinterpret_cast<const void *>(kern), smem);
     if (e) return e;
-    kern<<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(p);
+    kern<<<pl.runs, kThreads, smem, s>>>(p);
     Q35_LAUNCH_CHECK("attn_q4 launch");
-    if (pl.n_splits > 1) {
-      attn_q4_join_kernel<d()><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, s>>>(p, rows);
+    if (pl.join) {
+      attn_q4_join_kernel<d()><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(p, 8 * nt());
       Q35_LAUNCH_CHECK("attn_q4 join launch");
     }
     return Q35_OK;
