@@ -37,17 +37,19 @@
 // keys, the unit of its column, so its eight V channels per 16-byte chunk pair
 // come without a byte permutation and belong to one scale group.
 //
-// Work.  The 32-key tiles of all (sequence, kv head, group of 8 NT query rows)
-// form one list that is cut into equal runs, one per resident CTA; a run may end
-// one group, take several whole and begin another.  Nothing depends on the
-// lengths being alike, and the rings below never drain between groups.  A group
-// that one run holds whole is written at once, the others leave (max, sum, O)
-// partials that a second kernel joins; a run leaves at most two.
+// Work.  A group is a (sequence, kv head, 8 NT query rows); its 32-key tiles go in
+// rounds of four, one tile per warp.  The rounds of all groups form one list, each
+// group headed by one more round for what it costs to begin and end it, and the
+// list is cut into equal runs, one per resident CTA; a run may end one group, take
+// several whole and begin another.  Nothing depends on the lengths being alike,
+// and the rings below do not drain between groups.  A group that one run holds
+// whole is written at once, the others leave (max, sum, O) partials that a second
+// kernel joins; a run leaves at most two.
 //
-// Each warp takes every fourth tile of the run through a private ring of
-// asynchronous 16-byte copies, so warps meet only at the end of a group.  The
-// 16-byte chunks of a row are XOR-swizzled by the row so that both the 16-byte
-// reads of K and the 8-row reads of V touch every bank once.
+// Each warp keeps its tiles coming through a private ring of asynchronous 16-byte
+// copies, so warps meet only at the end of a group.  The 16-byte chunks of a row
+// are XOR-swizzled by the row, so that both the 16-byte reads of K and the 8-row
+// reads of V touch every bank once.
 #include <float.h>
 
 #include <type_traits>
@@ -75,8 +77,9 @@ struct Params {
   const int32_t *kv_lens;
   int *err;
   int B, Hq, Hkv, G, Sq, R, n_rg, causal;
-  int runs;  // CTAs of the main kernel
-  int per;   // tiles of a run (without kv_lens)
+  int runs;   // CTAs of the main kernel
+  int per;    // rounds of a run (unless scan)
+  int scan;   // runs are cut by the sequences' own lengths (kv_lens)
   int kv_len;
   int64_t cap;
   float scale_log2;
@@ -102,31 +105,27 @@ __device__ __forceinline__ int clamp_len(const Params &p, int b) {
   if (!p.kv_lens) return p.kv_len;
   return max(0, min(p.kv_lens[b], p.kv_len));
 }
-// Tiles of a group; a sequence without rows counts as one tile, so that some CTA
-// writes its zeros.
-__host__ __device__ __forceinline__ int tiles_of(int len) {
-  return len > 0 ? (len + kTile - 1) / kTile : 1;
-}
-__host__ __device__ __forceinline__ int run_length(int total, int runs) {
-  const int per = (total + runs - 1) / runs;
-  return (per + kWarps - 1) / kWarps * kWarps;  // whole rounds of the four warps
+// Rounds of a group in the list: its tiles by fours (a sequence without rows counts
+// one, so that some CTA writes its zeros) behind one for its start and end.
+__host__ __device__ __forceinline__ int rounds_of(int len) {
+  return 1 + (len > 0 ? (len + kWarps * kTile - 1) / (kWarps * kTile) : 1);
 }
 
 // A group of the list: its sequence, its (kv head, row group) index, its first
-// tile, the sequence's length in keys and tiles.
+// round, the sequence's length in keys and rounds.
 struct Group {
-  int b, hg, begin, len, tiles;
+  int b, hg, begin, len, rounds;
 };
-// Prefix sums over the sequences' tiles by the whole CTA.  Returns the tiles of
-// all groups; finds the sequence that holds tile at(total) (or, if seq >= 0,
-// looks at that sequence) and sets its first tile.
-template <typename At>
+// Prefix sums over the sequences' rounds by the whole CTA.  Returns the rounds of
+// all groups; finds the sequence that holds round at(total) (or, if seq >= 0,
+// looks at that sequence) and sets its first round.
+template <int THREADS, typename At>
 __device__ __forceinline__ int scan_tiles(const Params &p, int seq, At &&at, Group &gr) {
-  __shared__ int warp_sum[kWarps], found[2];
+  __shared__ int warp_sum[THREADS / 32], found[2];
   const int tid = threadIdx.x, lane = tid & 31;
-  const int each = (p.B + kThreads - 1) / kThreads, b0 = tid * each, b1 = min(b0 + each, p.B);
+  const int each = (p.B + THREADS - 1) / THREADS, b0 = tid * each, b1 = min(b0 + each, p.B);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(clamp_len(p, b));
+  for (int b = b0; b < b1; ++b) mine += rounds_of(clamp_len(p, b));
   int incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -137,7 +136,7 @@ __device__ __forceinline__ int scan_tiles(const Params &p, int seq, At &&at, Gro
   __syncthreads();
   int total = 0, before = incl - mine;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     if (w < (tid >> 5)) before += warp_sum[w];
     total += warp_sum[w];
   }
@@ -145,7 +144,7 @@ __device__ __forceinline__ int scan_tiles(const Params &p, int seq, At &&at, Gro
   total *= unit;
   const int want = at(total);
   for (int b = b0; b < b1; ++b) {
-    const int t = tiles_of(clamp_len(p, b));
+    const int t = rounds_of(clamp_len(p, b));
     if (seq >= 0 ? b == seq : (want >= before * unit && want - before * unit < t * unit)) {
       found[0] = b;
       found[1] = before * unit;
@@ -246,39 +245,40 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_seq = p.Hkv * p.n_rg;
 
-  // ---- the run [lo, hi) and the group it begins in
+  // ---- the run [lo, hi) of rounds and the group it begins in
   Group gr;
   int lo, hi;
-  if (p.kv_lens) {
+  if (p.scan) {
     int per = 0;
-    const int total = scan_tiles(p, -1, [&](int n) {
-      per = run_length(n, p.runs);
+    const int total = scan_tiles<kThreads>(p, -1, [&](int n) {
+      per = (n + p.runs - 1) / p.runs;
       return static_cast<int>(min(int64_t(blockIdx.x) * per, int64_t(n)));
     }, gr);
     lo = static_cast<int>(min(int64_t(blockIdx.x) * per, int64_t(total)));
     hi = min(lo + per, total);
-    if (blockIdx.x == 0)
-      for (int b = tid; b < p.B; b += kThreads)
-        if (p.kv_lens[b] < 0 || p.kv_lens[b] > p.kv_len)
-          report_error(p.err, DEV_ERR_INDEX, 311, b, p.kv_lens[b]);
   } else {
-    const int all = tiles_of(p.kv_len) * per_seq;
+    const int all = rounds_of(p.kv_len) * per_seq;
     lo = blockIdx.x * p.per;
     hi = min(lo + p.per, all * p.B);
     gr.b = lo / all;
     gr.begin = gr.b * all;
   }
+  if (p.kv_lens && blockIdx.x == 0)
+    for (int b = tid; b < p.B; b += kThreads)
+      if (p.kv_lens[b] < 0 || p.kv_lens[b] > p.kv_len)
+        report_error(p.err, DEV_ERR_INDEX, 311, b, p.kv_lens[b]);
   if (lo >= hi) return;
+  auto seq_rounds = [&](int len) { return rounds_of(p.scan ? len : p.kv_len); };
   gr.len = clamp_len(p, gr.b);
-  gr.tiles = tiles_of(gr.len);
-  gr.hg = (lo - gr.begin) / gr.tiles;
-  gr.begin += gr.hg * gr.tiles;
+  gr.rounds = seq_rounds(gr.len);
+  gr.hg = (lo - gr.begin) / gr.rounds;
+  gr.begin += gr.hg * gr.rounds;
   auto next_group = [&](Group &x) {
-    x.begin += x.tiles;
+    x.begin += x.rounds;
     if (++x.hg == per_seq) {
       x.hg = 0;
       x.len = clamp_len(p, ++x.b);
-      x.tiles = tiles_of(x.len);
+      x.rounds = seq_rounds(x.len);
     }
   };
 
@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   }
   float *merge = reinterpret_cast<float *>(smem + kWarps * L::kRing);
 
-  // ---- copies: this warp's tiles lo + warp, + 4, ..., ahead of their use.  Lane i
-  // copies chunks i, i + 32, ... of the tile's codes (chunk c of row r goes to
+  // ---- copies: this warp's tiles (tile 4 r + warp of round r of a group), ahead of
+  // their use.  Lane i copies chunks i, i + 32, ... of the tile's codes (chunk c of row r goes to
   // chunk c ^ swizzle(r)) and chunk i of its scales.  Rows behind the length are
   // not read (a chunk of narrow scales may hold up to 3 of them: the capacity is
   // a multiple of 16).
@@ -301,20 +301,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   const int srow = lane * 4 / NS;           // first row of the lane's chunk of scales
   Group ahead = gr;
   int64_t arow = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
-  int next = lo + warp;
+  int next = lo;
   uint32_t next_stage = 0;  // byte offset in the ring
   auto issue = [&]() {
-    if (next < hi) {
-      while (next >= ahead.begin + ahead.tiles || ahead.len == 0) {
-        while (next >= ahead.begin + ahead.tiles) next_group(ahead);
+    int r0 = 0;
+    for (; next < hi; ++next) {  // to the next round with a tile for this warp
+      if (next >= ahead.begin + ahead.rounds) {
+        next_group(ahead);
         arow = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
-        if (ahead.len > 0) break;
-        next += kWarps;  // a sequence without rows: nothing to copy
-        if (next >= hi) break;
       }
+      r0 = ((next - ahead.begin - 1) * kWarps + warp) * kTile;
+      if (next > ahead.begin && r0 < ahead.len) break;
     }
     if (next < hi) {
-      const int r0 = (next - ahead.begin) * kTile;
       const int left = ahead.len - r0;
       const int64_t row = arow + r0;
       const uint32_t dst = ring + next_stage;
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
         copy16(dst + 2 * L::kCodes + L::kScales + lane * 16,
                reinterpret_cast<const uint8_t *>(p.c.v_scales) + (live ? off : 0), live);
       }
-      next += kWarps;
+      ++next;
       next_stage = next_stage + L::kStage == L::kRing ? 0 : next_stage + L::kStage;
     }
     copies_commit();
@@ -365,12 +364,18 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
                      kDownM1 = pow2_bf16(-60) * 0x10001u;
   const float scale_up = p.scale_log2 * 0x1p81f;
   uint32_t stage = 0;
-  int mine = lo + warp;  // this warp's next tile
 
   for (int at = lo; at < hi;) {
-    // ---- one group's part of the run: tiles [at, end)
-    const int end = min(hi, gr.begin + gr.tiles);
+    // ---- one group's part of the run: its rounds [at, end), the first round of the
+    // group being only a mark
+    const int end = min(hi, gr.begin + gr.rounds);
     const int b = gr.b, hk = gr.hg / p.n_rg, rg = gr.hg - hk * p.n_rg, len = gr.len;
+    const bool begins = at <= gr.begin + 1, whole = begins && end == gr.begin + gr.rounds;
+    if (end == gr.begin + 1) {
+      at = end;
+      if (at < hi) next_group(gr);
+      continue;
+    }
 
     // Query rows: row r -> head hk G + r / Sq, position r % Sq.  Column g of an
     // operand tile holds 8 channels of every 32; accumulator columns are 2t, 2t + 1.
@@ -431,13 +436,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
       for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
     }
 
-    for (; mine < end; mine += kWarps) {
-      if (len == 0) continue;
+    for (int round = max(at, gr.begin + 1); round < end; ++round) {
+      const int key0 = ((round - gr.begin - 1) * kWarps + warp) * kTile;
+      if (key0 >= len) break;
       copies_wait<L::kStages - 1>();
       __syncwarp();
       const uint32_t sk = ring + stage;
       const uint32_t sks = sk + L::kCodes, sv = sks + L::kScales, svs = sv + L::kCodes;
-      const int key0 = (mine - gr.begin) * kTile;
 
       // ---- S^T = K Q^T (two blocks of 16 keys), in units of log2
       float s[2][NT][4];
@@ -649,7 +654,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
     }
     __syncthreads();
     if (warp == 0) {
-      const bool whole = at == gr.begin && end == gr.begin + gr.tiles;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float *src = merge + (D / 4 + 4) * nt * 32 + lane;
@@ -690,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
           const float inv = !whole ? 1.f : l[c] == 0.f ? 0.f : 1.0f / l[c];
           const int h = r / p.Sq, sq = r - h * p.Sq;
           uint16_t *dst = p.out + ((int64_t(b) * p.Sq + sq) * p.Hq + hk * p.G + h) * D;
-          const int64_t row = (2 * int64_t(blockIdx.x) + (at == gr.begin ? 1 : 0)) * (8 * NT) + lr;
+          const int64_t row = (2 * int64_t(blockIdx.x) + (begins ? 1 : 0)) * (8 * NT) + lr;
           // A unit is channels 32 j + 8 k + 2 i + (g & 1), i = 0..3: lanes g and g ^ 1 hold
           // the even and the odd ones and trade halves, for four neighbours each.
 #pragma unroll
@@ -724,29 +728,31 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
 }
 
 // One CTA per query row: joins the runs that share the row's group.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(Params p, int rows_per_group) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_q4_join_kernel(Params p, int rows_per_group) {
   constexpr int E = D / 32;
-  __shared__ float part[kWarps][D], part_l[kWarps];
+  __shared__ float part[kJoinWarps][D], part_l[kJoinWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t gr = blockIdx.x;
   const int64_t bh = gr / p.R;
   const int r = static_cast<int>(gr - bh * p.R);
   const int b = static_cast<int>(bh / p.Hkv), hk = static_cast<int>(bh - int64_t(b) * p.Hkv);
   const int rg = r / rows_per_group, lr = r - rg * rows_per_group;
-  int per = p.per, begin;
-  const int tiles = tiles_of(clamp_len(p, b));
-  if (p.kv_lens) {
+  int per = p.per, begin, rounds;
+  if (p.scan) {
     Group gs;
-    const int total = scan_tiles(p, b, [](int) { return 0; }, gs);
-    per = run_length(total, p.runs);
+    const int total = scan_tiles<kJoinWarps * 32>(p, b, [](int) { return 0; }, gs);
+    per = (total + p.runs - 1) / p.runs;
+    rounds = rounds_of(clamp_len(p, b));
     begin = gs.begin;
   } else {
-    begin = b * p.Hkv * p.n_rg * tiles;
+    rounds = rounds_of(p.kv_len);
+    begin = b * p.Hkv * p.n_rg * rounds;
   }
-  begin += (hk * p.n_rg + rg) * tiles;
-  const int c0 = begin / per;
-  const int n = (begin + tiles - 1) / per - c0 + 1;
+  begin += (hk * p.n_rg + rg) * rounds;
+  const int c0 = (begin + 1) / per;  // the run with the group's first keys
+  const int n = (begin + rounds - 1) / per - c0 + 1;
   if (n == 1) return;  // one run held the group and wrote the row
   auto slot = [&](int i) {
     return (2 * (int64_t(c0) + i) + (i == 0 ? 1 : 0)) * rows_per_group + lr;
@@ -759,7 +765,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(Params p, int ro
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 4
-  for (int i = warp; i < n; i += kWarps) {
+  for (int i = warp; i < n; i += kJoinWarps) {
     const int64_t at = slot(i);
     const float2 x = ml[at];
     const float f = exp2_fast(x.x - M);
@@ -772,35 +778,43 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(Params p, int ro
   if (lane == 0) part_l[warp] = l;
   __syncthreads();
   if (tid < D) {
-    const float lt = (part_l[0] + part_l[1]) + (part_l[2] + part_l[3]);
-    const float x = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    float lt = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      lt += part_l[w];
+      x += part[w][tid];
+    }
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
     const int h = r / p.Sq, sq = r - h * p.Sq;
     p.out[((int64_t(b) * p.Sq + sq) * p.Hq + hk * p.G + h) * D + tid] = f2bf(x * inv);
   }
 }
 
-// Query rows per CTA, and the runs the tiles are cut into.
+// Query rows per CTA, and the runs the rounds are cut into.
 struct Plan {
   int nt, n_rg, runs, per;
-  bool join;
+  bool scan, join;
 };
+// What the second kernel costs, in rounds: it pays from about there on to cut a
+// group into runs although whole groups would fill the CTAs.
+constexpr int kJoinRounds = 4;
 int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, bool lens) {
   pl.nt = R > 8 ? 2 : 1;
   const int64_t n_rg = (R + 8 * pl.nt - 1) / (8 * pl.nt);
-  const int64_t tiles = kv_len > 0 ? (kv_len + kTile - 1) / kTile : 1;
-  // all tiles, runs and rows of the list are counted in 31 bits
-  if (B >= (int64_t(1) << 31) || R >= (int64_t(1) << 31) || Hkv * n_rg >= (int64_t(1) << 31) ||
-      B * Hkv * R >= (int64_t(1) << 31) || tiles * B >= (int64_t(1) << 31) / (Hkv * n_rg))
+  const int rounds = rounds_of(static_cast<int>(kv_len));
+  const int64_t lim = int64_t(1) << 31;  // rounds and rows of the list are counted in 31 bits
+  if (B >= lim || R >= lim || Hkv * n_rg >= lim || B * Hkv >= lim / R ||
+      rounds * B >= lim / (Hkv * n_rg))
     return fail(Q35_ERR_SHAPE, "attn_q4: too many query rows or key tiles");
   pl.n_rg = static_cast<int>(n_rg);
-  const int total = static_cast<int>(tiles * B * Hkv * n_rg);
+  const int groups = static_cast<int>(B * Hkv * n_rg), total = groups * rounds;
   const int slots = num_sms() * ctas_per_sm(pl.nt);
-  pl.runs = (total + kWarps - 1) / kWarps;  // at least a tile for each warp
-  if (pl.runs > slots) pl.runs = slots;
-  pl.per = run_length(total, pl.runs);
-  if (!lens) pl.runs = (total + pl.per - 1) / pl.per;
-  pl.join = pl.runs > 1 && (lens || pl.per % static_cast<int>(tiles) != 0);
+  const int cut = total < slots ? total : slots;
+  const int cut_per = (total + cut - 1) / cut, whole = (groups + slots - 1) / slots * rounds;
+  pl.join = cut_per + kJoinRounds < whole;
+  pl.scan = pl.join && lens;
+  pl.per = pl.join ? cut_per : whole;
+  pl.runs = pl.scan ? cut : (total + pl.per - 1) / pl.per;
   return Q35_OK;
 }
 
@@ -813,7 +827,9 @@ extern "C" int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq,
                                          int D) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || Sq <= 0 || D <= 0) return 0;
   Plan pl;  // with kv_lens: never fewer runs than without
-  if (plan(pl, B, Hkv, Hq / Hkv * Sq, kv_len, true) != Q35_OK || !pl.join) return 0;
+  if (kv_len < 0 || kv_len >= (int64_t(1) << 31) - 256 ||
+      plan(pl, B, Hkv, Hq / Hkv * Sq, kv_len, true) != Q35_OK || !pl.join)
+    return 0;
   return partial_rows(pl.runs, pl.nt) * (static_cast<int64_t>(D) + 2);
 }
 
@@ -863,6 +879,7 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
   p.B = static_cast<int>(B);
   p.runs = pl.runs;
   p.per = pl.per;
+  p.scan = pl.scan ? 1 : 0;
   p.causal = causal ? 1 : 0;
   p.kv_len = static_cast<int>(kv_len);
   p.cap = cap;
@@ -877,7 +894,7 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
     kern<<<pl.runs, kThreads, smem, s>>>(p);
     Q35_LAUNCH_CHECK("attn_q4 launch");
     if (pl.join) {
-      attn_q4_join_kernel<d()><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(p, 8 * nt());
+      attn_q4_join_kernel<d()><<<static_cast<unsigned>(rows), kJoinWarps * 32, 0, s>>>(p, 8 * nt());
       Q35_LAUNCH_CHECK("attn_q4 join launch");
     }
     return Q35_OK;
