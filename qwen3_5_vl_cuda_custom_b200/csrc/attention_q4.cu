@@ -64,9 +64,10 @@ using q4::Cache;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;  // keys per tile
-// CTAs per SM, and tiles in flight per warp: what registers and shared memory
-// (40 KB of rings and 13.5 KB to join the warps at D = 128, NT = 1) allow.
-constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : 2; }
+// CTAs per SM, and tiles in flight per warp.  At D = 128, NT = 1 the registers
+// allow 3 CTAs; 4 of 128 registers (spills) measured 70.5 us against 68.0 at 64 x
+// 8193 keys, 3 tiles in flight 68.6.
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 constexpr int stages(int d, int nt) { return d == 128 && nt == 1 ? 2 : 4; }
 
 struct Params {

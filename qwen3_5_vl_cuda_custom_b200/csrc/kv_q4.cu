@@ -8,9 +8,12 @@
 // the smallest bf16) stores codes of 0.  A group that holds a NaN or an infinity
 // stores s = m = NaN and reads back as NaN.
 //
-// Both kernels move bytes: a thread owns the eight channels of one 32-bit code
-// word (16 bytes of bf16), group statistics go over the group/8 neighbouring
-// threads by shuffles, K and V share one launch.
+// Both kernels move bytes: a thread owns the eight channels of a 32-bit code word
+// (16 bytes of bf16) in each of two rows, group statistics go over the group/8
+// neighbouring threads by shuffles, K and V share one launch.  At 20 bytes per word
+// HBM feeds about 1.2 words per SM and clock, so about 100 instructions per word
+// are what a word may cost: hence paired fp32 arithmetic, one shuffle a step for
+// minimum and maximum together, and a multiplication for each division by S or Hkv.
 #include <type_traits>
 
 #include "kv_q4.cuh"
@@ -21,10 +24,28 @@ namespace {
 using q4::Cache;
 
 constexpr int kThreads = 256;
+constexpr int kWords = 2;  // code words per thread
 
 struct Rows {
   int64_t sb, sh, ss;  // element strides of batch, head, position
 };
+
+// n / d for 0 <= n < 2^31 by multiplication (Granlund and Montgomery): with
+// L = ceil(log2 d) and m = floor(2^32 (2^L - d) / d) + 1, n / d = (mulhi(m, n) + n) >> L.
+struct Divisor {
+  uint32_t d, m, shift;
+};
+Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  const uint64_t m = ((uint64_t(1) << 32) * ((uint64_t(1) << l) - d)) / d + 1;
+  return {d, static_cast<uint32_t>(m), l};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor &v, uint32_t &rest) {
+  const uint32_t q = (__umulhi(v.m, n) + n) >> v.shift;
+  rest = n - q * v.d;
+  return q;
+}
 
 __device__ __forceinline__ uint32_t bf2_min(uint32_t a, uint32_t b) {
   __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162 *>(&a),
@@ -57,32 +78,30 @@ __device__ __noinline__ uint32_t code_exact(float x, float lo, float s) {
 // Eight channels x (bf16 pairs) of a group -> their code word; `pair` receives
 // the group's (scale, minimum).  The threads of a group are neighbours.
 //
-// The fp32 quotient (x - m) * (1/s) is off by less than 3 * 2^-24 * 15 = 2.7e-6,
-// so a code can only differ from the 64-bit rule when the quotient lies within
-// 1e-5 of a half; those (about one in 10^5) are decided in 64 bits, as are
-// scales within 4 fp32 steps of a bf16 border and groups outside the range in
-// which 1/s and M - m are finite.
+// With r within 2^-23 of 1/s the fp32 value y = x r + (-m r) is off by less than
+// 15 * 2^-23 (r), 2^-24 |m| r (the rounded -m r) and 2^-20 (the sum): a code can only
+// differ from the 64-bit rule when y lies within 1e-5 + 2^-23 |m| r of a half.  Those
+// are decided in 64 bits, as are scales within 4 fp32 steps of a bf16 border and
+// groups outside the range in which 1/s and M - m are normal numbers.
 template <int GT>  // threads per group: 4, 8 or 16
 __device__ __forceinline__ uint32_t quantise8(uint4 x, uint32_t &pair) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t mn = bf2_min(bf2_min(w[0], w[1]), bf2_min(w[2], w[3]));
-  uint32_t mx = bf2_max(bf2_max(w[0], w[1]), bf2_max(w[2], w[3]));
+  const uint32_t mn = bf2_min(bf2_min(w[0], w[1]), bf2_min(w[2], w[3]));
+  const uint32_t mx = bf2_max(bf2_max(w[0], w[1]), bf2_max(w[2], w[3]));
   uint32_t bad = 0;  // an exponent of all ones carries into bit 15 / 31
 #pragma unroll
   for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f807f80u) + 0x00800080u;
-  bad &= 0x80008000u;
+  // (minimum, -maximum) as a pair: one minimum per step serves both
+  uint32_t ext = __byte_perm(mn, mx ^ 0x80008000u, 0x5410);
+  ext = bf2_min(ext, __byte_perm(mn, mx ^ 0x80008000u, 0x7632));
 #pragma unroll
-  for (int o = 1; o < GT; o <<= 1) {
-    mn = bf2_min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-    mx = bf2_max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-  }
-  float a, b, lo, hi;
-  unpack_bf2(mn, a, b);
-  lo = fminf(a, b);
-  unpack_bf2(mx, a, b);
-  hi = fmaxf(a, b);
-  if (bad) {
+  for (int o = 1; o < GT; o <<= 1) ext = bf2_min(ext, __shfl_xor_sync(0xffffffffu, ext, o));
+  const uint32_t any_bad = __ballot_sync(0xffffffffu, (bad & 0x80008000u) != 0);
+  const uint32_t lane = threadIdx.x & 31;
+  float lo, hi;
+  unpack_bf2(ext, lo, hi);
+  hi = -hi;
+  if (any_bad >> (lane & ~(GT - 1u)) & ((1u << GT) - 1u)) {
     pair = 0x7fc07fc0u;
     return 0u;
   }
@@ -92,31 +111,30 @@ __device__ __forceinline__ uint32_t quantise8(uint4 x, uint32_t &pair) {
   // 2^-100 <= s32 <= 2^120: 1/s and x - m stay normal numbers
   const bool plain = s32 >= 7.8886091e-31f && s32 <= 1.3292280e36f;
   const uint32_t low = (su & 0xffffu) - (0x8000u - 4u);
-  const uint16_t sb = (d == 0.f) ? uint16_t(0)
-                      : (plain && low > 8u) ? f2bf(s32)
-                                            : scale_exact(lo, hi);
+  uint16_t sb = f2bf(s32);
+  if (!plain || low <= 8u) sb = d == 0.f ? uint16_t(0) : scale_exact(lo, hi);
   const float s = bf2f(sb);
-  pair = static_cast<uint32_t>(sb) | (__float_as_uint(lo) & 0xffff0000u);
+  pair = static_cast<uint32_t>(sb) | ext << 16;
   if (s == 0.f) return 0u;
-  const float r = 1.0f / s;
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+  const float c = -lo * r;
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
-  uint32_t word = 0;
-  bool border = !plain;
+  const float2 r2 = make_float2(r, r), c2 = make_float2(c, c), up = make_float2(kRound, kRound),
+               down = make_float2(-kRound, -kRound), neg = make_float2(-1.f, -1.f);
+  float2 q[4];
+  float off = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float v[2];
-    unpack_bf2(w[i], v[0], v[1]);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float y = (v[h] - lo) * r;
-      const float t = y + kRound;
-      border |= fabsf(y - (t - kRound)) > 0.49999f;
-      const uint32_t c = min(__float_as_uint(t) - __float_as_uint(kRound), 15u);
-      word |= c << (4 * (i + 4 * h));
-    }
+    float2 v;
+    unpack_bf2(w[i], v.x, v.y);
+    const float2 y = __ffma2_rn(v, r2, c2);
+    q[i] = __fadd2_rn(__fadd2_rn(y, up), down);
+    const float2 e = __ffma2_rn(q[i], neg, y);
+    off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
   }
-  if (border) {
-    word = 0;
+  if (!plain || !(off < 0.49999f - fabsf(c) * 1.1920929e-7f)) {
+    uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float v0, v1;
@@ -124,74 +142,102 @@ __device__ __forceinline__ uint32_t quantise8(uint4 x, uint32_t &pair) {
       word |= code_exact(v0, lo, s) << (4 * i);
       word |= code_exact(v1, lo, s) << (4 * (i + 4));
     }
+    return word;
   }
-  return word;
+  // (even channels, odd channels): sums of 16^i code_i are integers below 2^16, which
+  // 2^23 puts into the low bits
+  const float2 k16 = make_float2(16.f, 16.f), k23 = make_float2(8388608.f, 8388608.f);
+  float2 f = __ffma2_rn(q[3], k16, q[2]);
+  f = __ffma2_rn(f, k16, q[1]);
+  f = __fadd2_rn(__ffma2_rn(f, k16, q[0]), k23);
+  return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410);
 }
 
-// One thread per code word; blockIdx.y picks K or V.
+// blockIdx.y picks K or V.
 template <int D, int GROUP>
 __global__ void __launch_bounds__(kThreads) kv_append_q4_kernel(
     const uint16_t *__restrict__ k, const uint16_t *__restrict__ v, Rows rk, Rows rv, Cache c,
-    int64_t words, int Hkv, int64_t S, int64_t cap, int64_t offset,
+    uint32_t rows, Divisor by_s, Divisor by_h, int64_t cap, int64_t offset,
     const int32_t *__restrict__ offsets, int *err) {
   constexpr int W = D / 8, J = D / 32, GT = GROUP / 8, NS = D / GROUP;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  constexpr int kRows = kThreads / W;  // rows of a CTA's step
   const bool is_v = blockIdx.y != 0;
   const uint16_t *src = is_v ? v : k;
   const Rows rs = is_v ? rv : rk;
-  const bool live = i < words;
-  const int64_t row = live ? i / W : 0;
-  const int ch = static_cast<int>(i & (W - 1));  // channels 8 ch ..
-  const int64_t bh = row / S, s = row - bh * S;
-  const int64_t b = bh / Hkv, h = bh - b * Hkv;
-  uint4 x = make_uint4(0u, 0u, 0u, 0u);
-  if (live)
-    x = *reinterpret_cast<const uint4 *>(src + b * rs.sb + h * rs.sh + s * rs.ss + 8 * ch);
-  uint32_t pair;
-  const uint32_t word = quantise8<GT>(x, pair);
-  if (!live) return;
-  const int64_t dst = (offsets ? static_cast<int64_t>(offsets[b]) : offset) + s;
-  if (dst < 0 || dst >= cap) {
-    report_error(err, DEV_ERR_INDEX, 105, static_cast<int>(b), static_cast<int>(dst));
-    return;
+  const int ch = threadIdx.x & (W - 1);  // channels 8 ch ..
+  uint4 x[kWords];
+  uint32_t bh[kWords], b[kWords], s[kWords];
+  bool live[kWords];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    const uint32_t row = (blockIdx.x * kWords + i) * kRows + threadIdx.x / W;
+    live[i] = row < rows;
+    bh[i] = divide(live[i] ? row : 0u, by_s, s[i]);
+    uint32_t h;
+    b[i] = divide(bh[i], by_h, h);
+    x[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (live[i])
+      x[i] = *reinterpret_cast<const uint4 *>(src + b[i] * rs.sb + h * rs.sh + s[i] * rs.ss + 8 * ch);
   }
-  const int64_t out = bh * cap + dst;
-  (is_v ? c.v_codes : c.k_codes)[out * W + (ch & 3) * J + (ch >> 2)] = word;
-  if (ch % GT == 0) (is_v ? c.v_scales : c.k_scales)[out * NS + ch / GT] = pair;
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    uint32_t pair;
+    const uint32_t word = quantise8<GT>(x[i], pair);
+    if (!live[i]) continue;
+    const int64_t dst = (offsets ? static_cast<int64_t>(offsets[b[i]]) : offset) + s[i];
+    if (dst < 0 || dst >= cap) {
+      report_error(err, DEV_ERR_INDEX, 105, static_cast<int>(b[i]), static_cast<int>(dst));
+      continue;
+    }
+    const int64_t out = bh[i] * cap + dst;
+    (is_v ? c.v_codes : c.k_codes)[out * W + (ch & 3) * J + (ch >> 2)] = word;
+    if (ch % GT == 0) (is_v ? c.v_scales : c.k_scales)[out * NS + ch / GT] = pair;
+  }
 }
 
-// Rows [start, start + n) as bf16 [B, Hkv, out_cap, D]; rows n .. out_cap are
-// zeros.  One thread per code word.
+// Rows [start, start + n) as bf16 [B, Hkv, out_cap, D]; rows n .. out_cap are zeros.
 template <int D, int GROUP>
 __global__ void __launch_bounds__(kThreads) kv_read_q4_kernel(
-    Cache c, uint16_t *__restrict__ k, uint16_t *__restrict__ v, int64_t words, int Hkv, int64_t n,
-    int64_t out_cap, int64_t cap, int64_t start, const int32_t *__restrict__ starts, int *err) {
+    Cache c, uint16_t *__restrict__ k, uint16_t *__restrict__ v, uint32_t rows, Divisor by_out,
+    Divisor by_h, uint32_t n, int64_t cap, int64_t start, const int32_t *__restrict__ starts,
+    int *err) {
   constexpr int W = D / 8, J = D / 32, GT = GROUP / 8, NS = D / GROUP;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= words) return;
+  constexpr int kRows = kThreads / W;
   const bool is_v = blockIdx.y != 0;
-  const int64_t row = i / W;
-  const int ch = static_cast<int>(i & (W - 1));
-  const int64_t bh = row / out_cap, r = row - bh * out_cap;
-  uint4 x = make_uint4(0u, 0u, 0u, 0u);
-  if (r < n) {
-    const int64_t b = bh / Hkv;
-    const int64_t src = (starts ? static_cast<int64_t>(starts[b]) : start) + r;
-    if (src < 0 || src >= cap) {
-      report_error(err, DEV_ERR_INDEX, 106, static_cast<int>(b), static_cast<int>(src));
-    } else {
-      const int64_t at = bh * cap + src;
-      const uint32_t word = (is_v ? c.v_codes : c.k_codes)[at * W + (ch & 3) * J + (ch >> 2)];
-      const uint32_t pair = (is_v ? c.v_scales : c.k_scales)[at * NS + ch / GT];
-      uint32_t o[4];
+  const uint32_t *codes = is_v ? c.v_codes : c.k_codes, *scales = is_v ? c.v_scales : c.k_scales;
+  const int ch = threadIdx.x & (W - 1);
+  uint32_t word[kWords], pair[kWords], row[kWords];
+  bool live[kWords];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o[e] = pack_bf2(q4::value(q4::code_of(word, 2 * e), pair),
-                        q4::value(q4::code_of(word, 2 * e + 1), pair));
-      x = make_uint4(o[0], o[1], o[2], o[3]);
+  for (int i = 0; i < kWords; ++i) {
+    row[i] = (blockIdx.x * kWords + i) * kRows + threadIdx.x / W;
+    uint32_t r, h;
+    const uint32_t bh = divide(row[i] < rows ? row[i] : 0u, by_out, r);
+    live[i] = row[i] < rows && r < n;
+    word[i] = pair[i] = 0u;  // a scale and a minimum of 0: the value 0
+    if (live[i]) {
+      const int64_t src =
+          (starts ? static_cast<int64_t>(starts[divide(bh, by_h, h)]) : start) + r;
+      if (src < 0 || src >= cap) {
+        report_error(err, DEV_ERR_INDEX, 106, static_cast<int>(bh / by_h.d), static_cast<int>(src));
+      } else {
+        const int64_t at = bh * cap + src;
+        word[i] = codes[at * W + (ch & 3) * J + (ch >> 2)];
+        pair[i] = scales[at * NS + ch / GT];
+      }
     }
   }
-  *reinterpret_cast<uint4 *>((is_v ? v : k) + row * D + 8 * ch) = x;
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    if (row[i] >= rows) continue;
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = pack_bf2(q4::value(q4::code_of(word[i], 2 * e), pair[i]),
+                      q4::value(q4::code_of(word[i], 2 * e + 1), pair[i]));
+    *reinterpret_cast<uint4 *>((is_v ? v : k) + int64_t(row[i]) * D + 8 * ch) =
+        make_uint4(o[0], o[1], o[2], o[3]);
+  }
 }
 
 template <typename F>
@@ -233,18 +279,19 @@ extern "C" int q35_kv_append_q4(const void *k_new, const void *v_new, const int6
       return fail(Q35_ERR_ALIGN, "kv_append_q4: strides not multiples of 8 elements");
   int *err = device_error_word();
   if (!err) return fail(Q35_ERR_CUDA, "kv_append_q4: no device error word");
-  const int64_t words = B * Hkv * S * (D / 8);
-  const int64_t blocks = (words + kThreads - 1) / kThreads;
-  if (blocks >= (int64_t(1) << 31)) return fail(Q35_ERR_SHAPE, "kv_append_q4: too many rows");
+  const int64_t rows = B * Hkv * S, step = kWords * kThreads / (D / 8);
+  if (B >= (int64_t(1) << 31) / Hkv || rows >= (int64_t(1) << 31) - step)
+    return fail(Q35_ERR_SHAPE, "kv_append_q4: too many rows");
   const Cache c{static_cast<uint32_t *>(k_codes), static_cast<uint32_t *>(k_scales),
                 static_cast<uint32_t *>(v_codes), static_cast<uint32_t *>(v_scales)};
   const Rows rk{k_strides[0], k_strides[1], k_strides[2]};
   const Rows rv{v_strides[0], v_strides[1], v_strides[2]};
   by_shape(D, group, [&](auto d, auto g) {
-    kv_append_q4_kernel<d(), g()><<<dim3(static_cast<unsigned>(blocks), 2), kThreads, 0,
+    kv_append_q4_kernel<d(), g()><<<dim3(static_cast<unsigned>((rows + step - 1) / step), 2), kThreads, 0,
                                     reinterpret_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint16_t *>(k_new), static_cast<const uint16_t *>(v_new), rk, rv, c,
-        words, Hkv, S, cap, offset, offsets, err);
+        static_cast<uint32_t>(rows), divisor(static_cast<uint32_t>(S)), divisor(Hkv), cap, offset,
+        offsets, err);
     return 0;
   });
   Q35_LAUNCH_CHECK("kv_append_q4 launch");
@@ -269,18 +316,21 @@ extern "C" int q35_kv_read_q4(const void *k_codes, const void *k_scales, const v
     return fail(Q35_ERR_ALIGN, "kv_read_q4: outputs not 16-byte aligned");
   int *err = device_error_word();
   if (!err) return fail(Q35_ERR_CUDA, "kv_read_q4: no device error word");
-  const int64_t words = B * Hkv * out_cap * (D / 8);
-  const int64_t blocks = (words + kThreads - 1) / kThreads;
-  if (blocks >= (int64_t(1) << 31)) return fail(Q35_ERR_SHAPE, "kv_read_q4: too many rows");
+  if (out_cap >= (int64_t(1) << 31))
+    return fail(Q35_ERR_SHAPE, "kv_read_q4: %lld rows", (long long)out_cap);
+  const int64_t rows = B * Hkv * out_cap, step = kWords * kThreads / (D / 8);
+  if (B >= (int64_t(1) << 31) / Hkv || rows >= (int64_t(1) << 31) - step)
+    return fail(Q35_ERR_SHAPE, "kv_read_q4: too many rows");
   const Cache c{static_cast<uint32_t *>(const_cast<void *>(k_codes)),
                 static_cast<uint32_t *>(const_cast<void *>(k_scales)),
                 static_cast<uint32_t *>(const_cast<void *>(v_codes)),
                 static_cast<uint32_t *>(const_cast<void *>(v_scales))};
   by_shape(D, group, [&](auto d, auto g) {
-    kv_read_q4_kernel<d(), g()><<<dim3(static_cast<unsigned>(blocks), 2), kThreads, 0,
+    kv_read_q4_kernel<d(), g()><<<dim3(static_cast<unsigned>((rows + step - 1) / step), 2), kThreads, 0,
                                   reinterpret_cast<cudaStream_t>(stream)>>>(
-        c, static_cast<uint16_t *>(k_out), static_cast<uint16_t *>(v_out), words, Hkv, n, out_cap,
-        cap, start, starts, err);
+        c, static_cast<uint16_t *>(k_out), static_cast<uint16_t *>(v_out),
+        static_cast<uint32_t>(rows), divisor(static_cast<uint32_t>(out_cap)), divisor(Hkv),
+        static_cast<uint32_t>(n), cap, start, starts, err);
     return 0;
   });
   Q35_LAUNCH_CHECK("kv_read_q4 launch");
