@@ -70,9 +70,20 @@ __device__ __noinline__ uint16_t scale_exact(float lo, float hi) {
   }
   return f2bf(__uint_as_float(u));
 }
-__device__ __noinline__ uint32_t code_exact(float x, float lo, float s) {
+__device__ __noinline__ float code_exact(float x, float lo, float s) {
   const double y = (static_cast<double>(x) - static_cast<double>(lo)) / static_cast<double>(s);
-  return static_cast<uint32_t>(fmin(rint(y), 15.0));
+  return static_cast<float>(fmin(rint(y), 15.0));
+}
+// The same for a quotient y known to lie next to a half, in fp32: n + 1/2 is the
+// border, (n + 1/2) s has at most 13 significant bits, x - lo = d + err exactly
+// (Knuth's two-sum), and d lies next to the border, so the differences are exact.
+__device__ __forceinline__ float code_at_border(float x, float lo, float s, float y) {
+  const float n = rintf(y - 0.5f), border = (n + 0.5f) * s;
+  const float d = x - lo, z = d - x;
+  const float err = (x - (d - z)) + (-lo - z);
+  const float u = (d - border) + err;
+  const bool odd = static_cast<int>(n) & 1;
+  return (u > 0.f || (u == 0.f && odd)) ? n + 1.f : n;
 }
 
 // Eight channels x (bf16 pairs) of a group -> their code word; `pair` receives
@@ -80,9 +91,11 @@ __device__ __noinline__ uint32_t code_exact(float x, float lo, float s) {
 //
 // With r within 2^-23 of 1/s the fp32 value y = x r + (-m r) is off by less than
 // 15 * 2^-23 (r), 2^-24 |m| r (the rounded -m r) and 2^-20 (the sum): a code can only
-// differ from the 64-bit rule when y lies within 1e-5 + 2^-23 |m| r of a half.  Those
-// are decided in 64 bits, as are scales within 4 fp32 steps of a bf16 border and
-// groups outside the range in which 1/s and M - m are normal numbers.
+// differ from the 64-bit rule when y lies within 1e-5 + 2^-23 |m| r of a half.  Exact
+// halves are common (x - m and s have few bits: about one channel in 300), so those
+// channels are decided on their own in exact fp32 steps.  64 bits decide scales
+// within 4 fp32 steps of a bf16 border and groups outside the range in which 1/s and
+// M - m are normal numbers.
 template <int GT>  // threads per group: 4, 8 or 16
 __device__ __forceinline__ uint32_t quantise8(uint4 x, uint32_t &pair) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -133,16 +146,20 @@ __device__ __forceinline__ uint32_t quantise8(uint4 x, uint32_t &pair) {
     const float2 e = __ffma2_rn(q[i], neg, y);
     off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
   }
-  if (!plain || !(off < 0.49999f - fabsf(c) * 1.1920929e-7f)) {
-    uint32_t word = 0;
+  const float near = 0.49999f - fabsf(c) * 1.1920929e-7f;
+  if (!plain || !(off < near)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float v0, v1;
-      unpack_bf2(w[i], v0, v1);
-      word |= code_exact(v0, lo, s) << (4 * i);
-      word |= code_exact(v1, lo, s) << (4 * (i + 4));
+      float2 v;
+      unpack_bf2(w[i], v.x, v.y);
+      if (!plain) {
+        q[i] = make_float2(code_exact(v.x, lo, s), code_exact(v.y, lo, s));
+      } else {
+        const float2 y = __ffma2_rn(v, r2, c2);
+        if (!(fabsf(y.x - q[i].x) < near)) q[i].x = code_at_border(v.x, lo, s, y.x);
+        if (!(fabsf(y.y - q[i].y) < near)) q[i].y = code_at_border(v.y, lo, s, y.y);
+      }
     }
-    return word;
   }
   // (even channels, odd channels): sums of 16^i code_i are integers below 2^16, which
   // 2^23 puts into the low bits
