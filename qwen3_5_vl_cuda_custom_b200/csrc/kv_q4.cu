@@ -8,12 +8,12 @@
 // the smallest bf16) stores codes of 0.  A group that holds a NaN or an infinity
 // stores s = m = NaN and reads back as NaN.
 //
-// Both kernels move bytes: a thread owns the eight channels of a 32-bit code word
-// (16 bytes of bf16) in each of two rows, group statistics go over the group/8
+// Both kernels move bytes.  A thread writes two code words of a row (16 channels),
+// or reads one in each of two rows; group statistics go over the group/16
 // neighbouring threads by shuffles, K and V share one launch.  At 20 bytes per word
-// HBM feeds about 1.2 words per SM and clock, so about 100 instructions per word
-// are what a word may cost: hence paired fp32 arithmetic, one shuffle a step for
-// minimum and maximum together, and a multiplication for each division by S or Hkv.
+// HBM feeds about 1.2 words per SM and clock, so about 100 instructions are what a
+// word may cost: hence paired fp32 arithmetic, one shuffle a step for minimum and
+// maximum together, and a multiplication for each division by S or Hkv.
 #include <type_traits>
 
 #include "kv_q4.cuh"
@@ -24,7 +24,8 @@ namespace {
 using q4::Cache;
 
 constexpr int kThreads = 256;
-constexpr int kWords = 2;  // code words per thread
+constexpr int kAppendThreads = 128, kAppendCtas = 7;
+constexpr int kWords = 2;  // code words per thread of the read
 
 struct Rows {
   int64_t sb, sh, ss;  // element strides of batch, head, position
@@ -47,20 +48,21 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor &v, uint32_
   return q;
 }
 
+// Minimum and maximum of bf16 pairs; a NaN stays.
 __device__ __forceinline__ uint32_t bf2_min(uint32_t a, uint32_t b) {
-  __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162 *>(&a),
-                             *reinterpret_cast<__nv_bfloat162 *>(&b));
-  return *reinterpret_cast<uint32_t *>(&r);
+  uint32_t d;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 __device__ __forceinline__ uint32_t bf2_max(uint32_t a, uint32_t b) {
-  __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162 *>(&a),
-                             *reinterpret_cast<__nv_bfloat162 *>(&b));
-  return *reinterpret_cast<uint32_t *>(&r);
+  uint32_t d;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
 // bf16((M - m) / 15) in one rounding, from 64 bits: a quotient that fp32 rounds
 // onto a border between two bf16 numbers is put back on its own side.
-__device__ __noinline__ uint16_t scale_exact(float lo, float hi) {
+__device__ __forceinline__ uint16_t scale_exact(float lo, float hi) {
   const double s = (static_cast<double>(hi) - static_cast<double>(lo)) / 15.0;
   float f = static_cast<float>(s);
   uint32_t u = __float_as_uint(f);
@@ -70,7 +72,18 @@ __device__ __noinline__ uint16_t scale_exact(float lo, float hi) {
   }
   return f2bf(__uint_as_float(u));
 }
-__device__ __noinline__ float code_exact(float x, float lo, float s) {
+// The rounding of a quotient s32 next to a border, in fp32: 15 times the border has
+// at most 13 significant bits, M - m = d + err exactly (Knuth's two-sum), and 15
+// borders lie next to d.
+__device__ __forceinline__ uint16_t scale_at_border(float lo, float hi, float s32) {
+  const uint32_t below = __float_as_uint(s32) >> 16;
+  const float border = __uint_as_float(below << 16 | 0x8000u);
+  const float d = hi - lo, z = d - hi;
+  const float err = (hi - (d - z)) + (-lo - z);
+  const float u = fmaf(border, -15.f, d) + err;
+  return static_cast<uint16_t>(below + ((u > 0.f || (u == 0.f && (below & 1u))) ? 1u : 0u));
+}
+__device__ __forceinline__ float code_exact(float x, float lo, float s) {
   const double y = (static_cast<double>(x) - static_cast<double>(lo)) / static_cast<double>(s);
   return static_cast<float>(fmin(rint(y), 15.0));
 }
@@ -86,37 +99,37 @@ __device__ __forceinline__ float code_at_border(float x, float lo, float s, floa
   return (u > 0.f || (u == 0.f && odd)) ? n + 1.f : n;
 }
 
-// Eight channels x (bf16 pairs) of a group -> their code word; `pair` receives
-// the group's (scale, minimum).  The threads of a group are neighbours.
+// 16 channels w (bf16 pairs) of a group -> their code words; `pair` receives the
+// group's (scale, minimum).  The threads of a group are neighbours.
 //
 // With r within 2^-23 of 1/s the fp32 value y = x r + (-m r) is off by less than
 // 15 * 2^-23 (r), 2^-24 |m| r (the rounded -m r) and 2^-20 (the sum): a code can only
 // differ from the 64-bit rule when y lies within 1e-5 + 2^-23 |m| r of a half.  Exact
-// halves are common (x - m and s have few bits: about one channel in 300), so those
-// channels are decided on their own in exact fp32 steps.  64 bits decide scales
-// within 4 fp32 steps of a bf16 border and groups outside the range in which 1/s and
-// M - m are normal numbers.
-template <int GT>  // threads per group: 4, 8 or 16
-__device__ __forceinline__ uint32_t quantise8(uint4 x, uint32_t &pair) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  const uint32_t mn = bf2_min(bf2_min(w[0], w[1]), bf2_min(w[2], w[3]));
-  const uint32_t mx = bf2_max(bf2_max(w[0], w[1]), bf2_max(w[2], w[3]));
-  uint32_t bad = 0;  // an exponent of all ones carries into bit 15 / 31
+// halves are common (x - m and s have few bits: one channel in 500), so those channels
+// are decided on their own in exact fp32 steps, as are scales within 4 fp32 steps of
+// a bf16 border.  Groups outside the range in which 1/s and M - m are normal numbers
+// take 64 bits.
+template <int GT>  // threads per group: 2, 4 or 8
+__device__ __forceinline__ void quantise16(const uint32_t (&w)[8], uint32_t (&word)[2],
+                                           uint32_t &pair) {
+  uint32_t mn = w[0], mx = w[0];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f807f80u) + 0x00800080u;
+  for (int i = 1; i < 8; ++i) {
+    mn = bf2_min(mn, w[i]);
+    mx = bf2_max(mx, w[i]);
+  }
   // (minimum, -maximum) as a pair: one minimum per step serves both
   uint32_t ext = __byte_perm(mn, mx ^ 0x80008000u, 0x5410);
   ext = bf2_min(ext, __byte_perm(mn, mx ^ 0x80008000u, 0x7632));
 #pragma unroll
   for (int o = 1; o < GT; o <<= 1) ext = bf2_min(ext, __shfl_xor_sync(0xffffffffu, ext, o));
-  const uint32_t any_bad = __ballot_sync(0xffffffffu, (bad & 0x80008000u) != 0);
-  const uint32_t lane = threadIdx.x & 31;
   float lo, hi;
   unpack_bf2(ext, lo, hi);
   hi = -hi;
-  if (any_bad >> (lane & ~(GT - 1u)) & ((1u << GT) - 1u)) {
+  word[0] = word[1] = 0u;
+  if (((ext & 0x7f807f80u) + 0x00800080u) & 0x80008000u) {  // an infinity or a NaN
     pair = 0x7fc07fc0u;
-    return 0u;
+    return;
   }
   const float d = hi - lo;
   const float s32 = d * (1.0f / 15.0f);
@@ -125,90 +138,113 @@ __device__ __forceinline__ uint32_t quantise8(uint4 x, uint32_t &pair) {
   const bool plain = s32 >= 7.8886091e-31f && s32 <= 1.3292280e36f;
   const uint32_t low = (su & 0xffffu) - (0x8000u - 4u);
   uint16_t sb = f2bf(s32);
-  if (!plain || low <= 8u) sb = d == 0.f ? uint16_t(0) : scale_exact(lo, hi);
+  if (!plain) sb = d == 0.f ? uint16_t(0) : scale_exact(lo, hi);
+  else if (low <= 8u) sb = scale_at_border(lo, hi, s32);
   const float s = bf2f(sb);
   pair = static_cast<uint32_t>(sb) | ext << 16;
-  if (s == 0.f) return 0u;
+  if (s == 0.f) return;
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
   const float c = -lo * r;
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
   const float2 r2 = make_float2(r, r), c2 = make_float2(c, c), up = make_float2(kRound, kRound),
                down = make_float2(-kRound, -kRound), neg = make_float2(-1.f, -1.f);
-  float2 q[4];
-  float off = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 v;
-    unpack_bf2(w[i], v.x, v.y);
-    const float2 y = __ffma2_rn(v, r2, c2);
-    q[i] = __fadd2_rn(__fadd2_rn(y, up), down);
-    const float2 e = __ffma2_rn(q[i], neg, y);
-    off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
-  }
+  const float2 k16 = make_float2(16.f, 16.f), k23 = make_float2(8388608.f, 8388608.f);
   const float near = 0.49999f - fabsf(c) * 1.1920929e-7f;
-  if (!plain || !(off < near)) {
+  uint32_t todo = 0;  // channels to decide on their own
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float2 q[4], e[4];
+    float off = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 v;
-      unpack_bf2(w[i], v.x, v.y);
-      if (!plain) {
-        q[i] = make_float2(code_exact(v.x, lo, s), code_exact(v.y, lo, s));
-      } else {
-        const float2 y = __ffma2_rn(v, r2, c2);
-        if (!(fabsf(y.x - q[i].x) < near)) q[i].x = code_at_border(v.x, lo, s, y.x);
-        if (!(fabsf(y.y - q[i].y) < near)) q[i].y = code_at_border(v.y, lo, s, y.y);
+      unpack_bf2(w[4 * h + i], v.x, v.y);
+      const float2 y = __ffma2_rn(v, r2, c2);
+      q[i] = __fadd2_rn(__fadd2_rn(y, up), down);
+      e[i] = __ffma2_rn(q[i], neg, y);
+      off = fmaxf(fmaxf(off, fabsf(e[i].x)), fabsf(e[i].y));
+    }
+    if (!(off < near)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!(fabsf(e[i].x) < near)) todo |= 1u << (8 * h + 2 * i);
+        if (!(fabsf(e[i].y) < near)) todo |= 2u << (8 * h + 2 * i);
       }
     }
+    // (even channels, odd channels): sums of 16^i code_i are integers below 2^16, which
+    // 2^23 puts into the low bits
+    float2 f = __ffma2_rn(q[3], k16, q[2]);
+    f = __ffma2_rn(f, k16, q[1]);
+    f = __fadd2_rn(__ffma2_rn(f, k16, q[0]), k23);
+    word[h] = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410);
   }
-  // (even channels, odd channels): sums of 16^i code_i are integers below 2^16, which
-  // 2^23 puts into the low bits
-  const float2 k16 = make_float2(16.f, 16.f), k23 = make_float2(8388608.f, 8388608.f);
-  float2 f = __ffma2_rn(q[3], k16, q[2]);
-  f = __ffma2_rn(f, k16, q[1]);
-  f = __fadd2_rn(__ffma2_rn(f, k16, q[0]), k23);
-  return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410);
+  if (!plain) todo = 0xffffu;
+#pragma unroll 1
+  while (todo) {
+    const int k = __ffs(todo) - 1, i = k >> 1;  // channel k of the 16
+    todo &= todo - 1;
+    const uint32_t a0 = i & 1 ? w[1] : w[0], a1 = i & 1 ? w[3] : w[2], a2 = i & 1 ? w[5] : w[4],
+                   a3 = i & 1 ? w[7] : w[6];
+    const uint32_t b0 = i & 2 ? a1 : a0, b1 = i & 2 ? a3 : a2, two = i & 4 ? b1 : b0;
+    const float x = __uint_as_float(k & 1 ? two & 0xffff0000u : two << 16);
+    const uint32_t code = static_cast<uint32_t>(
+        plain ? code_at_border(x, lo, s, fmaf(x, r, c)) : code_exact(x, lo, s));
+    const int at = 4 * ((i & 3) + 4 * (k & 1));
+    const uint32_t keep = ~(15u << at), put = code << at;
+    if (k < 8) word[0] = (word[0] & keep) | put;
+    else word[1] = (word[1] & keep) | put;
+  }
 }
 
 // blockIdx.y picks K or V.
 template <int D, int GROUP>
-__global__ void __launch_bounds__(kThreads) kv_append_q4_kernel(
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) kv_append_q4_kernel(
     const uint16_t *__restrict__ k, const uint16_t *__restrict__ v, Rows rk, Rows rv, Cache c,
     uint32_t rows, Divisor by_s, Divisor by_h, int64_t cap, int64_t offset,
     const int32_t *__restrict__ offsets, int *err) {
-  constexpr int W = D / 8, J = D / 32, GT = GROUP / 8, NS = D / GROUP;
-  constexpr int kRows = kThreads / W;  // rows of a CTA's step
+  constexpr int W = D / 8, J = D / 32, GT = GROUP / 16, NS = D / GROUP;
+  constexpr int T = D / 16;  // threads per row
   const bool is_v = blockIdx.y != 0;
-  const uint16_t *src = is_v ? v : k;
   const Rows rs = is_v ? rv : rk;
-  const int ch = threadIdx.x & (W - 1);  // channels 8 ch ..
-  uint4 x[kWords];
-  uint32_t bh[kWords], b[kWords], s[kWords];
-  bool live[kWords];
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    const uint32_t row = (blockIdx.x * kWords + i) * kRows + threadIdx.x / W;
-    live[i] = row < rows;
-    bh[i] = divide(live[i] ? row : 0u, by_s, s[i]);
+  const int ch = threadIdx.x & (T - 1);  // channels 16 ch ..
+  const uint16_t *src = (is_v ? v : k) + 16 * ch;
+  // words 2 ch and 2 ch + 1 in channel order: (t, j) = (2 ch % 4, ch / 2) and the next t
+  uint32_t *codes = (is_v ? c.v_codes : c.k_codes) + (2 * ch & 3) * J + (ch >> 1);
+  uint32_t *scales = (is_v ? c.v_scales : c.k_scales) + ch / GT;
+  constexpr uint32_t kStep = kAppendThreads / T;  // rows of a CTA's step
+  const uint32_t stride = gridDim.x * kStep;
+  uint32_t row = blockIdx.x * kStep + threadIdx.x / T, bh = 0, b = 0, s = 0;
+  uint32_t w[8] = {};
+  auto load = [&](uint32_t r) {  // the row's channels, ahead of their use
     uint32_t h;
-    b[i] = divide(bh[i], by_h, h);
-    x[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (live[i])
-      x[i] = *reinterpret_cast<const uint4 *>(src + b[i] * rs.sb + h * rs.sh + s[i] * rs.ss + 8 * ch);
-  }
+    bh = divide(r, by_s, s);
+    b = divide(bh, by_h, h);
+    const uint4 *at = reinterpret_cast<const uint4 *>(src + b * rs.sb + h * rs.sh + s * rs.ss);
+    const uint4 x = at[0], y = at[1];
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+  };
+  if (row < rows) load(row);
+  // every thread of a warp takes the same number of steps: the shuffles need them all
+  for (uint32_t base = blockIdx.x * kStep; base < rows; base += stride, row += stride) {
+    uint32_t now[8];
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    uint32_t pair;
-    const uint32_t word = quantise8<GT>(x[i], pair);
-    if (!live[i]) continue;
-    const int64_t dst = (offsets ? static_cast<int64_t>(offsets[b[i]]) : offset) + s[i];
+    for (int i = 0; i < 8; ++i) now[i] = w[i];
+    const uint32_t bh0 = bh, b0 = b, s0 = s;
+    if (row + stride < rows) load(row + stride);
+    uint32_t word[2], pair;
+    quantise16<GT>(now, word, pair);
+    if (row >= rows) continue;
+    const int64_t dst = (offsets ? static_cast<int64_t>(offsets[b0]) : offset) + s0;
     if (dst < 0 || dst >= cap) {
-      report_error(err, DEV_ERR_INDEX, 105, static_cast<int>(b[i]), static_cast<int>(dst));
+      report_error(err, DEV_ERR_INDEX, 105, static_cast<int>(b0), static_cast<int>(dst));
       continue;
     }
-    const int64_t out = bh[i] * cap + dst;
-    (is_v ? c.v_codes : c.k_codes)[out * W + (ch & 3) * J + (ch >> 2)] = word;
-    if (ch % GT == 0) (is_v ? c.v_scales : c.k_scales)[out * NS + ch / GT] = pair;
+    const int64_t out = bh0 * cap + dst;
+    codes[out * W] = word[0];
+    codes[out * W + J] = word[1];
+    if (ch % GT == 0) scales[out * NS] = pair;
   }
 }
 
@@ -296,15 +332,18 @@ extern "C" int q35_kv_append_q4(const void *k_new, const void *v_new, const int6
       return fail(Q35_ERR_ALIGN, "kv_append_q4: strides not multiples of 8 elements");
   int *err = device_error_word();
   if (!err) return fail(Q35_ERR_CUDA, "kv_append_q4: no device error word");
-  const int64_t rows = B * Hkv * S, step = kWords * kThreads / (D / 8);
-  if (B >= (int64_t(1) << 31) / Hkv || rows >= (int64_t(1) << 31) - step)
+  const int64_t rows = B * Hkv * S, step = kAppendThreads / (D / 16);
+  if (B >= (int64_t(1) << 31) / Hkv || rows >= (int64_t(1) << 30))
     return fail(Q35_ERR_SHAPE, "kv_append_q4: too many rows");
+  int64_t ctas = (rows + step - 1) / step;  // per K and V; at most the resident ones
+  const int64_t most = (int64_t(num_sms()) * kAppendCtas + 1) / 2;
+  if (ctas > most) ctas = most;
   const Cache c{static_cast<uint32_t *>(k_codes), static_cast<uint32_t *>(k_scales),
                 static_cast<uint32_t *>(v_codes), static_cast<uint32_t *>(v_scales)};
   const Rows rk{k_strides[0], k_strides[1], k_strides[2]};
   const Rows rv{v_strides[0], v_strides[1], v_strides[2]};
   by_shape(D, group, [&](auto d, auto g) {
-    kv_append_q4_kernel<d(), g()><<<dim3(static_cast<unsigned>((rows + step - 1) / step), 2), kThreads, 0,
+    kv_append_q4_kernel<d(), g()><<<dim3(static_cast<unsigned>(ctas), 2), kAppendThreads, 0,
                                     reinterpret_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint16_t *>(k_new), static_cast<const uint16_t *>(v_new), rk, rv, c,
         static_cast<uint32_t>(rows), divisor(static_cast<uint32_t>(S)), divisor(Hkv), cap, offset,
