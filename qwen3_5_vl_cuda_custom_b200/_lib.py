@@ -179,6 +179,9 @@ def sections_arg(sections) -> ctypes.Array:
     return arr
 
 
-def strides_arg(t) -> ctypes.Array:
-    """Element strides of all dims but the last of a 4-D tensor, as int64[3]."""
-    return (c_int64 * 3)(*t.stride()[:3])
+_I64x3 = c_int64 * 3
+
+
+def strides_arg(strides) -> ctypes.Array:
+    """The first three of a tensor's element strides as int64[3]."""
+    return _I64x3(strides[0], strides[1], strides[2])

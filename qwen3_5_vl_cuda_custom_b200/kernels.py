@@ -23,7 +23,9 @@ _BF16 = torch.bfloat16
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """Handle of the current stream of t's device (without building a Stream
+    object: 0.1 instead of 2.2 us, a good part of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -601,16 +603,17 @@ def _same_device(t: torch.Tensor, name: str, device) -> torch.Tensor:
     return t
 
 
-def _strided_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+def _strided_rows(t: torch.Tensor, name: str, device) -> torch.Tensor:
     """t [B, Hkv, S, D] as the append kernel can address it: contiguous channels,
     16-byte aligned rows (a transposed view of a token-major tensor needs no copy)."""
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
         raise TypeError(f"{name}: expected a 4-D tensor")
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:3])
-    if ok and t.is_cuda and t.dtype == _BF16:
-        return t
-    t = _require(t, name)
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    st = t.stride()
+    if (t.dtype != _BF16 or t.device != device or st[3] != 1 or (st[0] | st[1] | st[2]) & 7
+            or t.data_ptr() & 15):
+        t = _same_device(_require(t, name), name, device)
+        t = t.clone() if t.data_ptr() & 15 else t
+    return t
 
 
 def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
@@ -627,17 +630,22 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
     out and recorded as a device error.  k and v may be strided views."""
     B, Hkv, cap, D, group = _cache_q4("kv_append_q4", k_codes, k_scales, v_codes, v_scales)
     dev = k_codes.device
-    k = _same_device(_strided_rows(k, "kv_append_q4.k"), "kv_append_q4.k", dev)
-    v = _same_device(_strided_rows(v, "kv_append_q4.v"), "kv_append_q4.v", dev)
-    S = k.shape[2]
-    if tuple(k.shape) != (B, Hkv, S, D) or v.shape != k.shape:
+    k, v = _strided_rows(k, "kv_append_q4.k", dev), _strided_rows(v, "kv_append_q4.v", dev)
+    shape = k.shape
+    S = shape[2]
+    if shape != v.shape or shape != (B, Hkv, S, D):
         raise RuntimeError(f"kv_append_q4: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of "
                            f"{(B, Hkv, cap, D)}")
-    rows = _per_sequence(offset, "kv_append_q4.offset", B, dev) if isinstance(offset, torch.Tensor) else None
-    _call_on(dev, "q35_kv_append_q4", k.data_ptr(), v.data_ptr(), _lib.strides_arg(k),
-             _lib.strides_arg(v), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-             v_scales.data_ptr(), B, Hkv, S, D, group, cap, 0 if rows is not None else int(offset),
-             _ptr(rows), _stream(k_codes))
+    if isinstance(offset, torch.Tensor):
+        rows, first = _per_sequence(offset, "kv_append_q4.offset", B, dev).data_ptr(), 0
+    else:
+        rows, first = None, int(offset)
+    ks, vs = k.stride(), v.stride()
+    k_strides = _lib.strides_arg(ks)
+    _call_on(dev, "q35_kv_append_q4", k.data_ptr(), v.data_ptr(), k_strides,
+             k_strides if ks == vs else _lib.strides_arg(vs), k_codes.data_ptr(), k_scales.data_ptr(),
+             v_codes.data_ptr(), v_scales.data_ptr(), B, Hkv, S, D, group, cap, first, rows,
+             _stream(k_codes))
 
 
 def _read_q4(cache, shape, start: int, starts, n: int, out_cap: int):
