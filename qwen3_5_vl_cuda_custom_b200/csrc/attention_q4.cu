@@ -232,6 +232,16 @@ __device__ __forceinline__ bool nonfinite(uint32_t pair) {
   return (((pair & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
 }
 
+// Programmatic dependent launch: the kernels below are launched before the one in
+// front of them in the stream has finished; nothing is read or written before
+// wait_for_earlier().
+__device__ __forceinline__ void wait_for_earlier() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // One CTA = one run of tiles.
 template <int D, int GS, int NT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Params p) {
@@ -246,6 +256,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_seq = p.Hkv * p.n_rg;
 
+  if (p.kv_lens) wait_for_earlier();
+  let_next_launch();
   // ---- the run [lo, hi) of rounds and the group it begins in
   Group gr;
   int lo, hi;
@@ -347,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
     }
     copies_commit();
   };
+  if (!p.kv_lens) wait_for_earlier();
 #pragma unroll 1
   for (int i = 0; i < L::kStages; ++i) issue();
 
@@ -728,22 +741,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   copies_wait<0>();
 }
 
-// One CTA per query row: joins the runs that share the row's group.
-constexpr int kJoinWarps = 8;
-template <int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_q4_join_kernel(Params p, int rows_per_group) {
+// One CTA per query row: joins the runs that share the row's group.  Each warp joins
+// the partials it loads, U at once, by their own maximum.
+template <int D, int WARPS, int U>
+__global__ void __launch_bounds__(WARPS * 32) attn_q4_join_kernel(Params p, int rows_per_group) {
   constexpr int E = D / 32;
-  __shared__ float part[kJoinWarps][D], part_l[kJoinWarps];
+  __shared__ float part[WARPS][D], part_m[WARPS], part_l[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t gr = blockIdx.x;
-  const int64_t bh = gr / p.R;
-  const int r = static_cast<int>(gr - bh * p.R);
-  const int b = static_cast<int>(bh / p.Hkv), hk = static_cast<int>(bh - int64_t(b) * p.Hkv);
+  const int gr = blockIdx.x, bh = gr / p.R, r = gr - bh * p.R;
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int rg = r / rows_per_group, lr = r - rg * rows_per_group;
+  wait_for_earlier();
+  let_next_launch();
   int per = p.per, begin, rounds;
   if (p.scan) {
     Group gs;
-    const int total = scan_tiles<kJoinWarps * 32>(p, b, [](int) { return 0; }, gs);
+    const int total = scan_tiles<WARPS * 32>(p, b, [](int) { return 0; }, gs);
     per = (total + p.runs - 1) / p.runs;
     rounds = rounds_of(clamp_len(p, b));
     begin = gs.begin;
@@ -759,35 +772,56 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_q4_join_kernel(Params p,
     return (2 * (int64_t(c0) + i) + (i == 0 ? 1 : 0)) * rows_per_group + lr;
   };
   const float2 *ml = reinterpret_cast<const float2 *>(p.ws + 2 * int64_t(p.runs) * rows_per_group * D);
-  float M = -FLT_MAX;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[slot(i)].x);
-  M = warp_max(M);
-  float l = 0.f, v[E];
+  float m = -FLT_MAX, l = 0.f, v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < n; i += kJoinWarps) {
-    const int64_t at = slot(i);
-    const float2 x = ml[at];
-    const float f = exp2_fast(x.x - M);
-    l += x.y * f;
+  for (int i0 = warp; i0 < n; i0 += U * WARPS) {
+    float x[U][E];
+    float2 w[U];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = fmaf(p.ws[at * D + 32 * e + lane], f, v[e]);
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * WARPS;
+      const int64_t at = slot(i < n ? i : 0);
+      w[u] = i < n ? ml[at] : make_float2(-FLT_MAX, 0.f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[u][e] = i < n ? p.ws[at * D + 32 * e + lane] : 0.f;
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, w[u].x);
+    const float keep = exp2_fast(m - top);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] *= keep;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float f = exp2_fast(w[u].x - m);
+      l = fmaf(w[u].y, f, l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = fmaf(x[u][e], f, v[e]);
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) part[warp][32 * e + lane] = v[e];
-  if (lane == 0) part_l[warp] = l;
+  if (lane == 0) {
+    part_m[warp] = m;
+    part_l[warp] = l;
+  }
   __syncthreads();
-  if (tid < D) {
-    float lt = 0.f, x = 0.f;
+  for (int d = tid; d < D; d += WARPS * 32) {
+    float top = -FLT_MAX, lt = 0.f, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      lt += part_l[w];
-      x += part[w][tid];
+    for (int i = 0; i < WARPS; ++i) top = fmaxf(top, part_m[i]);
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      const float f = exp2_fast(part_m[i] - top);
+      lt = fmaf(part_l[i], f, lt);
+      sum = fmaf(part[i][d], f, sum);
     }
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
     const int h = r / p.Sq, sq = r - h * p.Sq;
-    p.out[((int64_t(b) * p.Sq + sq) * p.Hq + hk * p.G + h) * D + tid] = f2bf(x * inv);
+    p.out[((int64_t(b) * p.Sq + sq) * p.Hq + hk * p.G + h) * D + d] = f2bf(sum * inv);
   }
 }
 
@@ -892,10 +926,28 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
     constexpr int smem = Layout<d(), gs(), nt()>::kSmem;
     const int e = ensure_smem_attr(reinterpret_cast<const void *>(kern), smem);
     if (e) return e;
-    kern<<<pl.runs, kThreads, smem, s>>>(p);
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    cfg.stream = s;
+    cfg.gridDim = dim3(pl.runs);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    Q35_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
     Q35_LAUNCH_CHECK("attn_q4 launch");
     if (pl.join) {
-      attn_q4_join_kernel<d()><<<static_cast<unsigned>(rows), kJoinWarps * 32, 0, s>>>(p, 8 * nt());
+      // about runs / groups partials a row: 1 or 2, around a dozen, a hundred
+      const int64_t each = pl.runs / (B * Hkv * pl.n_rg);
+      auto *join = each < 4    ? &attn_q4_join_kernel<d(), 2, 2>
+                   : each < 32 ? &attn_q4_join_kernel<d(), 8, 2>
+                               : &attn_q4_join_kernel<d(), 16, 8>;
+      cfg.gridDim = dim3(static_cast<unsigned>(rows));
+      cfg.blockDim = dim3(each < 4 ? 64 : each < 32 ? 8 * 32 : 512);
+      cfg.dynamicSmemBytes = 0;
+      Q35_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join, p, 8 * nt()));
       Q35_LAUNCH_CHECK("attn_q4 join launch");
     }
     return Q35_OK;
