@@ -98,8 +98,9 @@ struct Layout {
   static constexpr int kSmem = kWarps * kRing + (kWarps - 1) * kRegs * 128;
 };
 
-// Partials: [2 runs][8 NT rows][D] floats, then [2 runs][8 NT rows] (m, l).
-// Slot 2 r holds the group that run r continues, 2 r + 1 the one it begins.
+// Workspace: [2 runs][8 NT rows][D] floats and [2 runs][8 NT rows] (m, l) of partials
+// (slot 2 r holds the group that run r continues, 2 r + 1 the one it begins), then
+// with kv_lens the first round of every sequence and the number of all rounds.
 constexpr int64_t partial_rows(int64_t runs, int nt) { return 2 * runs * 8 * nt; }
 
 __device__ __forceinline__ int clamp_len(const Params &p, int b) {
@@ -118,13 +119,13 @@ struct Group {
   int b, hg, begin, len, rounds;
 };
 // Prefix sums over the sequences' rounds by the whole CTA.  Returns the rounds of
-// all groups; finds the sequence that holds round at(total) (or, if seq >= 0,
-// looks at that sequence) and sets its first round.
-template <int THREADS, typename At>
-__device__ __forceinline__ int scan_tiles(const Params &p, int seq, At &&at, Group &gr) {
-  __shared__ int warp_sum[THREADS / 32], found[2];
+// all groups; finds the sequence that holds round at(total) and sets its first
+// round.  `table` (or null) receives every sequence's first round and the total.
+template <typename At>
+__device__ __forceinline__ int scan_rounds(const Params &p, At &&at, Group &gr, int *table) {
+  __shared__ int warp_sum[kWarps], found[2];
   const int tid = threadIdx.x, lane = tid & 31;
-  const int each = (p.B + THREADS - 1) / THREADS, b0 = tid * each, b1 = min(b0 + each, p.B);
+  const int each = (p.B + kThreads - 1) / kThreads, b0 = tid * each, b1 = min(b0 + each, p.B);
   int mine = 0;
   for (int b = b0; b < b1; ++b) mine += rounds_of(clamp_len(p, b));
   int incl = mine;
@@ -137,7 +138,7 @@ __device__ __forceinline__ int scan_tiles(const Params &p, int seq, At &&at, Gro
   __syncthreads();
   int total = 0, before = incl - mine;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w < (tid >> 5)) before += warp_sum[w];
     total += warp_sum[w];
   }
@@ -146,12 +147,14 @@ __device__ __forceinline__ int scan_tiles(const Params &p, int seq, At &&at, Gro
   const int want = at(total);
   for (int b = b0; b < b1; ++b) {
     const int t = rounds_of(clamp_len(p, b));
-    if (seq >= 0 ? b == seq : (want >= before * unit && want - before * unit < t * unit)) {
+    if (want >= before * unit && want - before * unit < t * unit) {
       found[0] = b;
       found[1] = before * unit;
     }
+    if (table) table[b] = before * unit;
     before += t;
   }
+  if (table && tid == 0) table[p.B] = total;
   __syncthreads();
   gr.b = found[0];
   gr.begin = found[1];
@@ -234,7 +237,8 @@ __device__ __forceinline__ bool nonfinite(uint32_t pair) {
 
 // Programmatic dependent launch: the kernels below are launched before the one in
 // front of them in the stream has finished; nothing is read or written before
-// wait_for_earlier().
+// wait_for_earlier(), and the next launch is let in only behind it (else several
+// kernels in a row pile up and crowd some SMs).
 __device__ __forceinline__ void wait_for_earlier() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
@@ -257,16 +261,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   const int per_seq = p.Hkv * p.n_rg;
 
   if (p.kv_lens) wait_for_earlier();
-  let_next_launch();
   // ---- the run [lo, hi) of rounds and the group it begins in
   Group gr;
   int lo, hi;
   if (p.scan) {
     int per = 0;
-    const int total = scan_tiles<kThreads>(p, -1, [&](int n) {
+    int *table = reinterpret_cast<int *>(p.ws + partial_rows(p.runs, NT) * (D + 2));
+    const int total = scan_rounds(p, [&](int n) {
       per = (n + p.runs - 1) / p.runs;
       return static_cast<int>(min(int64_t(blockIdx.x) * per, int64_t(n)));
-    }, gr);
+    }, gr, blockIdx.x == 0 ? table : nullptr);
     lo = static_cast<int>(min(int64_t(blockIdx.x) * per, int64_t(total)));
     hi = min(lo + per, total);
   } else {
@@ -360,6 +364,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
     copies_commit();
   };
   if (!p.kv_lens) wait_for_earlier();
+  let_next_launch();
 #pragma unroll 1
   for (int i = 0; i < L::kStages; ++i) issue();
 
@@ -755,11 +760,10 @@ __global__ void __launch_bounds__(WARPS * 32) attn_q4_join_kernel(Params p, int 
   let_next_launch();
   int per = p.per, begin, rounds;
   if (p.scan) {
-    Group gs;
-    const int total = scan_tiles<WARPS * 32>(p, b, [](int) { return 0; }, gs);
-    per = (total + p.runs - 1) / p.runs;
+    const int *table = reinterpret_cast<const int *>(p.ws + 2 * int64_t(p.runs) * rows_per_group * (D + 2));
+    begin = table[b];
     rounds = rounds_of(clamp_len(p, b));
-    begin = gs.begin;
+    per = (table[p.B] + p.runs - 1) / p.runs;
   } else {
     rounds = rounds_of(p.kv_len);
     begin = b * p.Hkv * p.n_rg * rounds;
@@ -830,10 +834,16 @@ struct Plan {
   int nt, n_rg, runs, per;
   bool scan, join;
 };
-// What the second kernel costs, in rounds: it pays from about there on to cut a
-// group into runs although whole groups would fill the CTAs.
-constexpr int kJoinRounds = 4;
-int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, bool lens) {
+// When to cut groups: a round at D = 128 takes about 0.72 us while every CTA has an SM
+// to itself and 1.4 once some SMs hold two or three; the second kernel adds 3.8 us and
+// 0.011 us per query row, 1.7 more when lengths on the device cut the runs.  In tenths
+// of a lone round (8 sequences x 4 kv heads: 512 keys whole 6.3, cut 6.5 us; 1024 keys
+// 9.2 and 7.9; 256 sequences: 1024 keys 43 and 47, 4096 keys 139 and 122).
+int round_cost(int64_t ctas, int D) {
+  return (ctas <= num_sms() ? 10 : 20) * (D + 128) / 256;
+}
+int64_t join_cost(int64_t rows, bool lens) { return 53 + rows / 64 + (lens ? 24 : 0); }
+int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, int D, bool lens) {
   pl.nt = R > 8 ? 2 : 1;
   const int64_t n_rg = (R + 8 * pl.nt - 1) / (8 * pl.nt);
   const int rounds = rounds_of(static_cast<int>(kv_len));
@@ -844,9 +854,10 @@ int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, bool lens) {
   pl.n_rg = static_cast<int>(n_rg);
   const int groups = static_cast<int>(B * Hkv * n_rg), total = groups * rounds;
   const int slots = num_sms() * ctas_per_sm(pl.nt);
-  const int cut = total < slots ? total : slots;
-  const int cut_per = (total + cut - 1) / cut, whole = (groups + slots - 1) / slots * rounds;
-  pl.join = cut_per + kJoinRounds < whole;
+  const int cut = total < slots ? total : slots, cut_per = (total + cut - 1) / cut;
+  const int each = (groups + slots - 1) / slots, whole = each * rounds;
+  pl.join = int64_t(cut_per) * round_cost(cut, D) + join_cost(B * Hkv * R, lens) <
+            int64_t(whole) * round_cost((groups + each - 1) / each, D);
   pl.scan = pl.join && lens;
   pl.per = pl.join ? cut_per : whole;
   pl.runs = pl.scan ? cut : (total + pl.per - 1) / pl.per;
@@ -861,11 +872,15 @@ using namespace q35;
 extern "C" int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                          int D) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || Sq <= 0 || D <= 0) return 0;
-  Plan pl;  // with kv_lens: never fewer runs than without
-  if (kv_len < 0 || kv_len >= (int64_t(1) << 31) - 256 ||
-      plan(pl, B, Hkv, Hq / Hkv * Sq, kv_len, true) != Q35_OK || !pl.join)
-    return 0;
-  return partial_rows(pl.runs, pl.nt) * (static_cast<int64_t>(D) + 2);
+  if (kv_len < 0 || kv_len >= (int64_t(1) << 31) - 256) return 0;
+  int64_t most = 0;  // of the calls with and without kv_lens
+  for (int lens = 0; lens < 2; ++lens) {
+    Plan pl;
+    if (plan(pl, B, Hkv, Hq / Hkv * Sq, kv_len, D, lens != 0) != Q35_OK || !pl.join) continue;
+    const int64_t n = partial_rows(pl.runs, pl.nt) * (static_cast<int64_t>(D) + 2) + B + 1;
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_scales,
@@ -888,7 +903,7 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
     return fail(Q35_ERR_ALIGN, "attn_q4: q, out not 16-byte aligned");
   const int64_t R = Hq / Hkv * Sq;
   Plan pl;
-  const int ps = plan(pl, B, Hkv, R, kv_len, kv_lens != nullptr);
+  const int ps = plan(pl, B, Hkv, R, kv_len, D, kv_lens != nullptr);
   if (ps) return ps;
   if (pl.join && !workspace) return fail(Q35_ERR_INVALID, "attn_q4: no workspace");
   if (pl.join && !aligned16(workspace))
