@@ -497,8 +497,7 @@ Q35_API int q35_kv_read_q4(const void *k_codes, const void *k_scales, const void
 /* Attention over the first kv_len rows (kv_lens[b] <= kv_len rows of sequence b
  * when kv_lens, device int32 [B], is not NULL): q bf16 [B, Hq, Sq, D], out bf16
  * token-major [B, Sq, Hq*D], any Hq/Hkv and Sq.  Meant for few query rows per
- * kv head (a decode step, drafted tokens); for a chunk of a prompt read the rows
- * back and call q35_attn_prefill_cache_fwd.  causal != 0: query s sees keys
+ * kv head (a decode step, drafted tokens).  causal != 0: query s sees keys
  * <= s + len - Sq.  A query that sees no key gives zeros.  A kv_lens entry
  * outside [0, kv_len] is clamped and recorded as a device error (code 2, site
  * 311).  workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.      */
@@ -509,6 +508,19 @@ Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_sc
                             int Hq, int Hkv, int64_t Sq, int64_t kv_len, const int32_t *kv_lens,
                             int64_t cap, int D, int group, float scale, int causal,
                             float *workspace, q35_stream_t stream);
+
+/* The same for many query rows per kv head (a chunk of a prompt), all sequences of
+ * kv_len >= 1 rows: the rows go through scaled fp16 copies in the workspace
+ * (q35_attn_q4_chunk_workspace(...) bytes, 16-byte aligned) and the tensor-memory
+ * attention kernels.  B * Hq <= 65535.  A key or value that is not finite may reach
+ * all rows that share its 128-key tile, as in q35_attn_prefill_cache_fwd.     */
+Q35_API int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64_t Sq,
+                                            int64_t kv_len, int D);
+Q35_API int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const void *k_scales,
+                                  const void *v_codes, const void *v_scales, void *out,
+                                  int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
+                                  int64_t cap, int D, int group, float scale, int causal,
+                                  void *workspace, q35_stream_t stream);
 
 /* ---- Vision-tower operators (bf16, fp32 math) -------------------------- */
 /* LayerNorm over the last dim: (x - mean) * rsqrt(var + eps) * w (+ b); b may

@@ -23,6 +23,15 @@
 //                   arithmetic.  At the end: O / l, bf16, token-major store.
 // Every mbarrier wait is bounded (sm100::mbar_wait); on timeout the kernel
 // records DEV_ERR_WAIT_TIMEOUT and unwinds.
+//
+// Both kernels also come with fp16 operands (kF16), for rows read back from a 4-bit
+// cache (attention_q4_chunk.cu): same tiles, P in fp16, the key tiles optionally cut
+// into splits that leave fp32 partials, a power of two per kv head on the scores and
+// on the output, head_dim 32 and 64 zero-padded to 128.
+#include <cuda_fp16.h>
+#include <float.h>
+
+#include "attention_tc.cuh"
 #include "sm100.cuh"
 
 namespace q35 {
@@ -96,8 +105,69 @@ struct AttnParams {
   uint16_t *out;
   float *lse;
   int *err;
+  F16Extra x;  // kF16 only
 };
 
+// P as the operand type of the products.
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack_p(float a, float b) {
+  if constexpr (kF16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    return pack_bf2(a, b);
+  }
+}
+// The key tiles [j0, j0 + n) of this CTA's split.
+__device__ __forceinline__ int split_tiles(const AttnParams &p, int split, int n_all, int &j0) {
+  j0 = split * p.x.tiles_per_split;
+  return max(0, min(n_all - j0, p.x.tiles_per_split));
+}
+// kF16 epilogue of one query row: D columns of O (read 32 at a time from TMEM by the
+// whole warp) as bf16, or as an fp32 partial with its (max in log2 units, sum).
+__device__ __forceinline__ void store_row_f16(const AttnParams &p, uint32_t o_tm, bool some,
+                                              bool valid, int b, int h, int64_t qi, int split,
+                                              float m_log2, float l, float f) {
+  const int64_t rows = p.x.rows;
+  const int64_t row = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq + qi;
+  const int64_t slot = row * p.x.splits + split;
+  const float inv = p.x.part ? f : (l > 0.f ? f / l : 0.f);
+#pragma unroll 1
+  for (int c = 0; c < p.x.D / 32; ++c) {
+    uint32_t r[32];
+    if (some) {
+      sm100::tmem_ld32(o_tm + c * 32, r);
+      sm100::tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = 0u;
+    }
+    if (!valid) continue;
+    if (p.x.part) {
+      float4 *dst = reinterpret_cast<float4 *>(p.x.part + slot * p.x.D + c * 32);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        dst[i] = make_float4(__uint_as_float(r[4 * i]) * inv, __uint_as_float(r[4 * i + 1]) * inv,
+                             __uint_as_float(r[4 * i + 2]) * inv, __uint_as_float(r[4 * i + 3]) * inv);
+    } else {
+      uint4 *dst = reinterpret_cast<uint4 *>(
+          p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * p.x.D + c * 32);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          u[k] = pack_bf2(__uint_as_float(r[8 * i + 2 * k]) * inv,
+                          __uint_as_float(r[8 * i + 2 * k + 1]) * inv);
+        dst[i] = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+    }
+  }
+  if (valid && p.x.part)
+    reinterpret_cast<float2 *>(p.x.part + rows * p.x.splits * p.x.D)[slot] = make_float2(m_log2, l);
+}
+
+template <bool kF16>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
                    const __grid_constant__ CUtensorMap tmK,
@@ -124,7 +194,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t diag = p.Skv - p.Sq;
   int64_t kv_end = p.Skv;
   if (p.causal) kv_end = min(p.Skv, m0 + kTile + diag);
-  const int n_tiles = kv_end > 0 ? static_cast<int>((kv_end + kTile - 1) / kTile) : 0;
+  int n_tiles = kv_end > 0 ? static_cast<int>((kv_end + kTile - 1) / kTile) : 0;
+  int j0 = 0;
+  float sl2 = p.sl2, f_out = 1.f;
+  if constexpr (kF16) {
+    n_tiles = split_tiles(p, blockIdx.z, n_tiles, j0);
+    const float2 f = p.x.fac[static_cast<int64_t>(b) * p.Hkv + hk];
+    sl2 *= f.x;
+    f_out = f.y;
+  }
   const int32_t q_row = static_cast<int32_t>((static_cast<int64_t>(b) * p.Hq + h) * p.Sq + m0);
   const int32_t kv_row = static_cast<int32_t>((static_cast<int64_t>(b) * p.Hkv + hk) * p.kv_cap);
 
@@ -162,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       uint8_t *sk = smem + kKOff + st * 2 * kHalfBytes;
       uint8_t *sv = smem + kVOff + st * 2 * kHalfBytes;
-      const int32_t r = kv_row + j * kTile;
+      const int32_t r = kv_row + (j0 + j) * kTile;
       sm100::mbar_arrive_expect_tx(&kv_full[st], 4 * kHalfBytes);
       sm100::tma_load_2d(sk, &tmK, &kv_full[st], 0, r);
       sm100::tma_load_2d(sk + kHalfBytes, &tmK, &kv_full[st], 64, r);
@@ -171,8 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1 && lane == 0) {
     // ------------------------------------------------ MMA issuer
-    constexpr uint32_t idesc_s = sm100::idesc_bf16_f32(kTile, kTile);
-    constexpr uint32_t idesc_pv = sm100::idesc_bf16_f32(kTile, 128, 0, 1);
+    constexpr uint32_t idesc_s = sm100::idesc_bf16_f32(kTile, kTile, 0, 0, kF16);
+    constexpr uint32_t idesc_pv = sm100::idesc_bf16_f32(kTile, 128, 0, 1, kF16);
     bool ok = n_tiles > 0;
     if (ok && !sm100::mbar_wait(q_full, 0)) {
       report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 302, 0, 0);
@@ -251,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(r[i]);
       }
-      const int64_t n0 = static_cast<int64_t>(j) * kTile;
+      const int64_t n0 = static_cast<int64_t>(j0 + j) * kTile;
       const int64_t lim = p.causal ? min(qi + diag, p.Skv - 1) : p.Skv - 1;
       if (n0 + kTile - 1 > lim) {
 #pragma unroll
@@ -266,14 +344,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * p.sl2 > 8.f) {
+      } else if ((m_new - m_used) * sl2 > 8.f) {
         need = true;
-        alpha = exp2f((m_used - m_new) * p.sl2);
+        alpha = exp2f((m_used - m_new) * sl2);
         m_used = m_new;
         l *= alpha;
       }
       const float mu = (m_used == -INFINITY) ? 0.f : m_used;
-      const float mus = mu * p.sl2;
+      const float mus = mu * sl2;
       // O may only be touched once PV_{j-1} has finished.
       if (j >= 1 && !sm100::mbar_wait(o_done, (j - 1) & 1)) {
         report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 307, j, row);
@@ -298,10 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float a = exp2_mufu(fmaf(s[half * 64 + 2 * i], p.sl2, -mus));
-          const float b2 = exp2_fma(fmaf(s[half * 64 + 2 * i + 1], p.sl2, -mus));
+          const float a = exp2_mufu(fmaf(s[half * 64 + 2 * i], sl2, -mus));
+          const float b2 = exp2_fma(fmaf(s[half * 64 + 2 * i + 1], sl2, -mus));
           l += a + b2;
-          pk[i] = pack_bf2(a, b2);
+          pk[i] = pack_p<kF16>(a, b2);
         }
         sm100::tmem_st32(sb + half * 32, pk);
       }
@@ -311,6 +389,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // ---- epilogue: O / l -> bf16, out[b, qi, h*128 + d]
     const bool valid = qi < p.Sq;
+    if constexpr (kF16) {
+      bool done = n_tiles > 0 && ok;
+      if (done && !sm100::mbar_wait(o_done, (n_tiles - 1) & 1)) {
+        report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 309, n_tiles, row);
+        done = false;
+      }
+      done = __all_sync(0xffffffffu, done);
+      sm100::tc_fence_after();
+      const bool seen = done && m_used != -INFINITY;
+      store_row_f16(p, tmem + lane_base, done, valid, b, h, qi, blockIdx.z,
+                    seen ? m_used * sl2 : -FLT_MAX, seen ? l : 0.f, seen ? f_out : 0.f);
+    } else {
     uint16_t *orow = p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * 128;
     if (n_tiles > 0 && ok) {
       if (!sm100::mbar_wait(o_done, (n_tiles - 1) & 1)) {
@@ -342,6 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (valid && p.lse)
       p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + qi] =
           l > 0.f ? m_used * p.scale + logf(l) : -INFINITY;
+    }
   }
 
   sm100::tc_fence_before();
@@ -387,7 +478,7 @@ constexpr uint32_t kPolyPattern() {
   return kPoly == 2 ? 0x22u : kPoly == 3 ? 0x52u : kPoly == 4 ? 0xAAu : kPoly == 5 ? 0xADu : 0x00u;
 }
 
-template <int kPoly>
+template <int kPoly, bool kF16>
 __global__ void __launch_bounds__(kThreads2, 1)
     attn_tc2_kernel(const __grid_constant__ CUtensorMap tmQ,
                     const __grid_constant__ CUtensorMap tmK,
@@ -422,7 +513,15 @@ __global__ void __launch_bounds__(kThreads2, 1)
   const int64_t diag = p.Skv - p.Sq;
   int64_t kv_end = p.Skv;
   if (p.causal) kv_end = min(p.Skv, m0 + kTile + diag);
-  const int n_tiles = kv_end > 0 ? static_cast<int>((kv_end + kTile - 1) / kTile) : 0;
+  int n_tiles = kv_end > 0 ? static_cast<int>((kv_end + kTile - 1) / kTile) : 0;
+  int j0 = 0;
+  float sl2 = p.sl2, f_out = 1.f;
+  if constexpr (kF16) {
+    n_tiles = split_tiles(p, blockIdx.y, n_tiles, j0);
+    const float2 f = p.x.fac[static_cast<int64_t>(b) * p.Hkv + hk];
+    sl2 *= f.x;
+    f_out = f.y;
+  }
   const int32_t kv_row = static_cast<int32_t>((static_cast<int64_t>(b) * p.Hkv + hk) * p.kv_cap);
 
   if (threadIdx.x == 0) {
@@ -463,7 +562,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
       const uint32_t ph = ((j >> 1) & 1) ^ 1;
       uint8_t *sk = smem + kK2Off + st * 2 * kHalfBytes;
       uint8_t *sv = smem + kV2Off + st * 2 * kHalfBytes;
-      const int32_t r = kv_row + j * kTile;
+      const int32_t r = kv_row + (j0 + j) * kTile;
       if (!sm100::mbar_wait(&k_empty[st], ph)) {
         report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 321, j, 0);
         break;
@@ -481,8 +580,8 @@ __global__ void __launch_bounds__(kThreads2, 1)
     }
   } else if (warp == 1 && lane == 0) {
     // ------------------------------------------------ MMA issuer
-    constexpr uint32_t idesc_s = sm100::idesc_bf16_f32(kTile, kTile);
-    constexpr uint32_t idesc_pv = sm100::idesc_bf16_f32(kTile, 128, 0, 1);
+    constexpr uint32_t idesc_s = sm100::idesc_bf16_f32(kTile, kTile, 0, 0, kF16);
+    constexpr uint32_t idesc_pv = sm100::idesc_bf16_f32(kTile, 128, 0, 1, kF16);
     bool ok = n_tiles > 0;
     if (ok && !sm100::mbar_wait(q_full, 0)) {
       report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 322, 0, 0);
@@ -569,7 +668,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
         break;
       }
       sm100::tc_fence_after();
-      const int64_t n0 = static_cast<int64_t>(j) * kTile;
+      const int64_t n0 = static_cast<int64_t>(j0 + j) * kTile;
       const bool masked = n0 + kTile - 1 > lim_c;
       // the whole score row in two 64-column loads, one wait
       uint32_t sr[kTile];
@@ -595,17 +694,17 @@ __global__ void __launch_bounds__(kThreads2, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * p.sl2 > 8.f) {
+      } else if ((m_new - m_used) * sl2 > 8.f) {
         need = true;
-        alpha = exp2f((m_used - m_new) * p.sl2);
+        alpha = exp2f((m_used - m_new) * sl2);
         m_used = m_new;
         l *= alpha;
       }
-      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * p.sl2;
+      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * sl2;
       // exponentials, bf16 P over the first 64 S columns.  Score pairs are
       // scaled with one f32x2 FMA; pairs alternate between the MUFU unit
       // (ex2.approx) and the paired FMA polynomial; row sums in f32x2.
-      const float2 sl2v = make_float2(p.sl2, p.sl2), nmus = make_float2(-mus, -mus);
+      const float2 sl2v = make_float2(sl2, sl2), nmus = make_float2(-mus, -mus);
       float2 lsum0 = make_float2(0.f, 0.f), lsum1 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int qtr = 0; qtr < 4; ++qtr) {
@@ -624,7 +723,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
           }
           if (i & 2) lsum1 = __fadd2_rn(lsum1, e);
           else lsum0 = __fadd2_rn(lsum0, e);
-          pk[i] = pack_bf2(e.x, e.y);
+          pk[i] = pack_p<kF16>(e.x, e.y);
         }
         sm100::tmem_st16(s_tm + qtr * 16, pk);
       }
@@ -648,6 +747,18 @@ __global__ void __launch_bounds__(kThreads2, 1)
     }
     // ---- epilogue: O / l -> bf16, out[b, qi, h*128 + d]
     const bool valid = qi < p.Sq;
+    if constexpr (kF16) {
+      bool done = n_tiles > 0 && ok;
+      if (done && !sm100::mbar_wait(o_done, 0)) {
+        report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 330, n_tiles, row);
+        done = false;
+      }
+      done = __all_sync(0xffffffffu, done);
+      sm100::tc_fence_after();
+      const bool seen = done && m_used != -INFINITY;
+      store_row_f16(p, o_tm, done, valid, b, h, qi, blockIdx.y, seen ? m_used * sl2 : -FLT_MAX,
+                    seen ? l : 0.f, seen ? f_out : 0.f);
+    } else {
     uint16_t *orow = p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * 128;
     if (n_tiles > 0 && ok) {
       if (!sm100::mbar_wait(o_done, 0)) {
@@ -681,6 +792,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
     if (valid && p.lse)
       p.lse[(static_cast<int64_t>(b) * p.Hq + h) * p.Sq + qi] =
           (l > 0.f && m_used != -INFINITY) ? m_used * p.scale + logf(l) : -INFINITY;
+    }
   }
 
   sm100::tc_fence_before();
@@ -697,40 +809,28 @@ __global__ void __launch_bounds__(kThreads2, 1)
 
 using namespace q35;
 
-// Prefill attention for head_dim 128 on tcgen05 (called by
-// q35_attn_prefill_fwd; same arguments and layouts).
-int q35_attn_prefill_tc(const void *q, const void *k, const void *v, void *out,
-                        float *lse, int64_t B, int Hq, int Hkv, int64_t Sq,
-                        int64_t Skv, int64_t kv_cap, float scale, int causal,
-                        q35_stream_t stream) {
-  const int64_t qrows = B * Hq * Sq, kvrows = B * Hkv * kv_cap;
+namespace {
+// The launches both entry points share; `splits` CTAs per query block.
+template <bool kF16>
+int launch_tc(const void *q, const void *k, const void *v, AttnParams &p, int64_t B, int splits,
+              q35_stream_t stream) {
+  const int64_t qrows = B * p.Hq * p.Sq, kvrows = B * p.Hkv * p.kv_cap;
   if (qrows >= (int64_t(1) << 31) || kvrows >= (int64_t(1) << 31))
     return fail(Q35_ERR_SHAPE, "attn_prefill_tc: too many rows for TMA coordinates");
-  int *err = device_error_word();
-  if (!err) return fail(Q35_ERR_CUDA, "attn_prefill_tc: no device error word");
-  CUtensorMap tq, tk, tv;
+  p.err = device_error_word();
+  if (!p.err) return fail(Q35_ERR_CUDA, "attn_prefill_tc: no device error word");
+  CUtensorMap tq, tk, tv;  // (16-bit elements either way)
   int st = make_tmap_bf16_2d(&tq, q, 128, qrows, 256, 64, kTile);
   if (st) return st;
   st = make_tmap_bf16_2d(&tk, k, 128, kvrows, 256, 64, kTile);
   if (st) return st;
   st = make_tmap_bf16_2d(&tv, v, 128, kvrows, 256, 64, kTile);
   if (st) return st;
-  AttnParams p{};
-  p.Hq = Hq;
-  p.Hkv = Hkv;
-  p.Sq = Sq;
-  p.Skv = Skv;
-  p.kv_cap = kv_cap;
-  p.n_mblocks = static_cast<int>((Sq + kTile - 1) / kTile);
-  p.scale = scale;
-  p.sl2 = scale * 1.4426950408889634f;
-  p.causal = causal ? 1 : 0;
-  p.out = static_cast<uint16_t *>(out);
-  p.lse = lse;
-  p.err = err;
-  if ((Hq / Hkv) % 2 == 0) {
+  p.n_mblocks = static_cast<int>((p.Sq + kTile - 1) / kTile);
+  p.sl2 = p.scale * 1.4426950408889634f;
+  if ((p.Hq / p.Hkv) % 2 == 0) {
     // GQA with an even group: two heads per CTA share each K/V tile.
-    dim3 grid2(static_cast<unsigned>(p.n_mblocks * B * Hq / 2));
+    dim3 grid2(static_cast<unsigned>(p.n_mblocks * B * p.Hq / 2), splits);
     constexpr int np = 3;  // 3 of 8 score pairs on the FMA-pipe exp2 (measured best of 2..5)
     auto go = [&](auto kern) -> int {
       const int st2 = ensure_smem_attr(reinterpret_cast<const void *>(kern), kSmem2);
@@ -749,14 +849,60 @@ int q35_attn_prefill_tc(const void *q, const void *k, const void *v, void *out,
       kern<<<grid2, kThreads2, kSmem2, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tv, p);
       return 0;
     };
-    int st3 = go(attn_tc2_kernel<np>);
+    int st3 = go(attn_tc2_kernel<np, kF16>);
     if (st3) return st3;
     Q35_LAUNCH_CHECK("attn_prefill_tc2 launch");
     return Q35_OK;
   }
-  { const int _st = ensure_smem_attr(reinterpret_cast<const void *>(attn_tc_kernel), kSmem); if (_st) return _st; }
-  dim3 grid(p.n_mblocks, static_cast<unsigned>(B * Hq));
-  attn_tc_kernel<<<grid, kThreads, kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tv, p);
+  { const int _st = ensure_smem_attr(reinterpret_cast<const void *>(attn_tc_kernel<kF16>), kSmem); if (_st) return _st; }
+  dim3 grid(p.n_mblocks, static_cast<unsigned>(B * p.Hq), splits);
+  attn_tc_kernel<kF16><<<grid, kThreads, kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tv, p);
   Q35_LAUNCH_CHECK("attn_prefill_tc launch");
   return Q35_OK;
 }
+}  // namespace
+
+// Prefill attention for head_dim 128 on tcgen05 (called by
+// q35_attn_prefill_fwd; same arguments and layouts).
+int q35_attn_prefill_tc(const void *q, const void *k, const void *v, void *out,
+                        float *lse, int64_t B, int Hq, int Hkv, int64_t Sq,
+                        int64_t Skv, int64_t kv_cap, float scale, int causal,
+                        q35_stream_t stream) {
+  AttnParams p{};
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.Sq = Sq;
+  p.Skv = Skv;
+  p.kv_cap = kv_cap;
+  p.scale = scale;
+  p.causal = causal ? 1 : 0;
+  p.out = static_cast<uint16_t *>(out);
+  p.lse = lse;
+  return launch_tc<false>(q, k, v, p, B, 1, stream);
+}
+
+namespace q35 {
+
+int attn_tc_ctas(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t *tile_rows) {
+  *tile_rows = kTile;
+  const int64_t blocks = (Sq + kTile - 1) / kTile * B * Hq;
+  return static_cast<int>((Hq / Hkv) % 2 == 0 ? blocks / 2 : blocks);
+}
+
+int attn_tc_f16(const void *q, const void *k, const void *v, void *out, int64_t B, int Hq, int Hkv,
+                int64_t Sq, int64_t Skv, int64_t kv_cap, float scale, int causal,
+                const F16Extra &x, q35_stream_t stream) {
+  AttnParams p{};
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.Sq = Sq;
+  p.Skv = Skv;
+  p.kv_cap = kv_cap;
+  p.scale = scale;
+  p.causal = causal ? 1 : 0;
+  p.out = static_cast<uint16_t *>(out);
+  p.x = x;
+  return launch_tc<true>(q, k, v, p, B, x.splits, stream);
+}
+
+}  // namespace q35

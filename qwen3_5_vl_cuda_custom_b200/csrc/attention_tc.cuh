@@ -1,0 +1,25 @@
+// The fp16-operand form of the tensor-memory attention kernels (attention_tc.cu),
+// which attention over rows read back from a 4-bit cache runs on.
+#pragma once
+
+#include "common.cuh"
+
+namespace q35 {
+
+struct F16Extra {
+  const float2 *fac;    // per (sequence, kv head): factors of the scores and of the output
+  float *part;          // fp32 partials [rows, splits, D], then (m, l) [rows, splits]; or null
+  int64_t rows;         // B * Hq * Sq
+  int splits, tiles_per_split, D;
+};
+
+// CTAs of one pass over all key tiles, and the rows of a query or key tile.
+int attn_tc_ctas(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t *tile_rows);
+
+// q [B,Hq,Sq,128], k / v [B,Hkv,kv_cap,128] fp16 (channels behind D zero, rows behind
+// Skv finite), out token-major bf16 [B,Sq,Hq*D] unless x.part takes partials.
+int attn_tc_f16(const void *q, const void *k, const void *v, void *out, int64_t B, int Hq, int Hkv,
+                int64_t Sq, int64_t Skv, int64_t kv_cap, float scale, int causal,
+                const F16Extra &x, q35_stream_t stream);
+
+}  // namespace q35

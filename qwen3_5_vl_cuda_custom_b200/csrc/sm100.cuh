@@ -292,14 +292,15 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr,
   return d;
 }
 
-// Instruction descriptor of tcgen05.mma kind::f16: bf16 A/B, fp32 D,
+// Instruction descriptor of tcgen05.mma kind::f16: bf16 (or fp16) A/B, fp32 D,
 // both operands K-major unless a_mn / b_mn, shape M x N.
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N,
                                                       int a_mn = 0,
-                                                      int b_mn = 0) {
+                                                      int b_mn = 0,
+                                                      bool fp16 = false) {
   return (1u << 4)                                  // D format F32
-         | (1u << 7)                                // A format BF16
-         | (1u << 10)                               // B format BF16
+         | ((fp16 ? 0u : 1u) << 7)                  // A format BF16 (0: F16)
+         | ((fp16 ? 0u : 1u) << 10)                 // B format BF16 (0: F16)
          | (static_cast<uint32_t>(a_mn) << 15)      // A major
          | (static_cast<uint32_t>(b_mn) << 16)      // B major
          | (static_cast<uint32_t>(N >> 3) << 17)    // N / 8

@@ -671,9 +671,9 @@ def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Ten
     return _read_q4(cache, shape, 0 if starts is not None else int(start), starts, int(length), int(length))
 
 
-# Query rows per kv head from which attention_cache_q4 reads the rows back and
-# runs the bf16 prefill kernel instead of attending over the codes.
-_Q4_PREFILL_ROWS = 256
+# Query rows per kv head from which attention_cache_q4 takes the form for chunks of
+# a prompt instead of attending over the codes.
+_Q4_CHUNK_ROWS = 256
 
 
 def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
@@ -687,8 +687,9 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     is read on the device, so such a call can be captured once and replayed as
     the lengths grow.  Causal masking is aligned to each sequence's last row; a
     query that sees no row gives zeros.  Decode-shaped calls run on the codes;
-    with an int ``kv_len`` a chunk of a prompt reads the rows back into a
-    temporary bf16 copy and runs the prefill kernel."""
+    with an int ``kv_len`` a chunk of a prompt goes through a temporary fp16 copy
+    of the rows (256 bytes of K and V each per row) and the tensor-memory
+    attention kernels."""
     cache = (k_codes, k_scales, v_codes, v_scales)
     shape = _cache_q4("attention_cache_q4", *cache)
     B, Hkv, cap, D, group = shape
@@ -707,13 +708,12 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     if n < 0 or n > cap:
         raise RuntimeError(f"attention_cache_q4: {n} rows exceed the capacity {cap}")
     out = torch.empty(B, Sq, Hq * D, device=q.device, dtype=q.dtype)
-    if lens is None and (Hq // Hkv) * Sq >= _Q4_PREFILL_ROWS and n > 0:
-        # whole key tiles, zero-filled: the prefill kernel reads (and masks) to the end of one
-        pad = -(-n // 128) * 128
-        k, v = _read_q4(cache, shape, 0, None, n, pad)
-        _call_on(q.device, "q35_attn_prefill_cache_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                 out.data_ptr(), None, B, Hq, Hkv, Sq, n, pad, D, float(scale), 1 if causal else 0,
-                 _stream(q))
+    if lens is None and (Hq // Hkv) * Sq >= _Q4_CHUNK_ROWS and n > 0:
+        w = _lib.query("q35_attn_q4_chunk_workspace", B, Hq, Hkv, Sq, n, D)
+        ws = torch.empty(max(w, 16), device=q.device, dtype=torch.uint8)
+        _call_on(q.device, "q35_attn_q4_chunk_fwd", q.data_ptr(), *[t.data_ptr() for t in cache],
+                 out.data_ptr(), B, Hq, Hkv, Sq, n, cap, D, group, float(scale), 1 if causal else 0,
+                 ws.data_ptr(), _stream(q))
     else:
         w = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, n, D)
         ws = torch.empty(w, device=q.device, dtype=torch.float32) if w > 0 else None
