@@ -5,8 +5,9 @@
 // attention of a 512-token chunk (32 heads, 8704 keys).  But rounding the keys to
 // bf16 on the way shows: a score moves by 2^-9 of its terms, 3 times the error of all
 // other roundings together.  So the operands are fp16, whose 11 bits make it vanish,
-// scaled per sequence and kv head by powers of two to a largest value in
-// [2^13, 2^14): the range that bf16 has and fp16 has not.
+// scaled per sequence and kv head by powers of two, for the range that bf16 has and
+// fp16 has not: v to a largest value in [2^13, 2^14), q and k against one another to
+// largest values of like size, so that the scores stay what they are.
 //
 //   1. attn_q4_absmax_kernel: largest |q|, |k|, |v| of each kv head (k, v from the
 //      scales alone, a fifth of the cache's bytes).
@@ -27,18 +28,20 @@ namespace {
 using q4::Cache;
 
 constexpr int kThreads = 256;
-constexpr int kSlices = 16;  // CTAs per kv head of the largest values
-constexpr int kPad = 128;    // rows of a key tile, channels of an operand row
+constexpr int kMaxSlices = 64;  // CTAs per kv head of the largest values, at most
+constexpr int kPad = 128;       // rows of a key tile, channels of an operand row
+constexpr int kRows = 4;        // operand rows of a thread
 
 struct Chunk {
   const uint16_t *q;
   Cache c;
-  float4 *maxima;  // [kSlices][B * Hkv] (|q|, |k|, |v|)
-  float2 *fac;     // [B * Hkv]
+  float4 *maxima;  // [slices][B * Hkv] (|q|, |k|, |v|)
+  float *v_scale;  // [B * Hkv]
   __half *qo, *ko, *vo;
   int D, group, q_rows;  // q_rows = Hq / Hkv * Sq
   int64_t cap;
   int len, pad;          // keys, and their rows in ko / vo
+  int slices;
 };
 
 __device__ __forceinline__ float largest(float a, float x) {
@@ -49,10 +52,11 @@ __device__ __forceinline__ float largest(float a, float x) {
 __global__ void __launch_bounds__(kThreads) attn_q4_absmax_kernel(Chunk p) {
   const int64_t bh = blockIdx.y;
   const int ns = p.D / p.group, tid = blockIdx.x * kThreads + threadIdx.x;
-  constexpr int step = kSlices * kThreads;
+  const int step = p.slices * kThreads;
   float m[3] = {0.f, 0.f, 0.f};
   const uint4 *q = reinterpret_cast<const uint4 *>(p.q + bh * p.q_rows * p.D);
   const int64_t nq = int64_t(p.q_rows) * p.D / 8;
+#pragma unroll 4
   for (int64_t i = tid; i < nq; i += step) {
     const uint4 x = q[i];
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -64,6 +68,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_absmax_kernel(Chunk p) {
     }
   }
   const int64_t base = bh * p.cap * ns, n = int64_t(p.len) * ns;
+#pragma unroll 4
   for (int64_t i = tid; i < n; i += step) {
     const uint32_t k = p.c.k_scales[base + i], v = p.c.v_scales[base + i];
     m[1] = largest(largest(m[1], q4::value(0.f, k)), q4::value(15.f, k));
@@ -84,12 +89,11 @@ __global__ void __launch_bounds__(kThreads) attn_q4_absmax_kernel(Chunk p) {
   }
 }
 
-// e with 2^-e * a in [2^13, 2^14); 0 for a = 0.
+// Exponent of a > 0: a = f 2^e, f in [0.5, 1); 0 for a = 0.
 __device__ __forceinline__ int exponent(float a) {
-  if (a == 0.f) return 0;
-  int e;
-  frexpf(a, &e);  // a = f 2^e, f in [0.5, 1)
-  return max(-100, min(e - 14, 126));
+  int e = 0;
+  if (a > 0.f) frexpf(a, &e);
+  return e;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
@@ -97,88 +101,109 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// A thread writes 8 of the 128 channels of an operand row; rows: keys, values, queries.
+// A thread writes 8 of the 128 channels of kRows operand rows; rows: keys, values,
+// queries.  What it reads is on its way before the scales are known.
 __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
   const int64_t bh = blockIdx.y;
   __shared__ float scale[3];
+  const int ch = threadIdx.x & 15, W = p.D / 8;
+  const int64_t r0 = int64_t(blockIdx.x) * (kRows * kThreads / 16) + threadIdx.x / 16;
+  uint4 x[kRows];  // 8 channels of q, or (code word, scale pair)
+  int which[kRows];
+  int64_t row[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t r = r0 + i * (kThreads / 16);
+    which[i] = r < p.pad ? 1 : r < 2 * int64_t(p.pad) ? 2 : 0;
+    row[i] = which[i] == 1 ? r : which[i] == 2 ? r - p.pad : r - 2 * int64_t(p.pad);
+    x[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (ch >= W) continue;
+    if (which[i] == 0) {
+      if (row[i] < p.q_rows)
+        x[i] = *reinterpret_cast<const uint4 *>(p.q + (bh * p.q_rows + row[i]) * p.D + 8 * ch);
+    } else if (row[i] < p.len) {
+      const int64_t at = bh * p.cap + row[i];
+      const bool v = which[i] == 2;
+      x[i].x = (v ? p.c.v_codes : p.c.k_codes)[at * W + (ch & 3) * (p.D / 32) + (ch >> 2)];
+      x[i].y = (v ? p.c.v_scales : p.c.k_scales)[at * (p.D / p.group) + 8 * ch / p.group];
+    }
+  }
   if (threadIdx.x < 32) {
     float m[3] = {0.f, 0.f, 0.f};
-    if (threadIdx.x < kSlices) {
-      const float4 x = p.maxima[int64_t(threadIdx.x) * gridDim.y + bh];
-      m[0] = x.x, m[1] = x.y, m[2] = x.z;
+    for (int s = threadIdx.x; s < p.slices; s += 32) {
+      const float4 y = p.maxima[int64_t(s) * gridDim.y + bh];
+      m[0] = fmaxf(m[0], y.x), m[1] = fmaxf(m[1], y.y), m[2] = fmaxf(m[2], y.z);
     }
     int e[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) e[i] = exponent(warp_max(m[i]));
     if (threadIdx.x == 0) {
-#pragma unroll
-      for (int i = 0; i < 3; ++i) scale[i] = pow2(-e[i]);
-      if (blockIdx.x == 0) p.fac[bh] = make_float2(ldexpf(1.f, e[0] + e[1]), pow2(e[2]));
+      const int a = max(-100, min((e[0] - e[1]) / 2, 100)), v = max(-100, min(e[2] - 14, 100));
+      scale[0] = pow2(-a);
+      scale[1] = pow2(a);
+      scale[2] = pow2(-v);
+      if (blockIdx.x == 0) p.v_scale[bh] = pow2(v);
     }
   }
   __syncthreads();
-  const int ch = threadIdx.x & 15, W = p.D / 8;
-  const int64_t r = int64_t(blockIdx.x) * (kThreads / 16) + threadIdx.x / 16;
-  const int which = r < p.pad ? 1 : r < 2 * int64_t(p.pad) ? 2 : 0;
-  const int64_t row = which == 1 ? r : which == 2 ? r - p.pad : r - 2 * int64_t(p.pad);
-  if (which == 0 && row >= p.q_rows) return;
-  const float f = scale[which];
-  uint32_t o[4] = {0u, 0u, 0u, 0u};
-  if (ch < W) {
-    if (which == 0) {
-      const uint4 x = *reinterpret_cast<const uint4 *>(p.q + (bh * p.q_rows + row) * p.D + 8 * ch);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kRows; ++i) {
+    if (which[i] == 0 && row[i] >= p.q_rows) continue;
+    const float f = scale[which[i]];
+    uint32_t o[4];
+    if (which[i] == 0) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
         float a, b;
-        unpack_bf2(w[i], a, b);
-        o[i] = pack_h2(a * f, b * f);
+        unpack_bf2(w[k], a, b);
+        o[k] = pack_h2(a * f, b * f);
       }
-    } else if (row < p.len) {
-      const int64_t at = bh * p.cap + row;
-      const uint32_t word = (which == 2 ? p.c.v_codes : p.c.k_codes)[at * W + (ch & 3) * (p.D / 32) + (ch >> 2)];
-      const uint32_t pair = (which == 2 ? p.c.v_scales : p.c.k_scales)[at * (p.D / p.group) + 8 * ch / p.group];
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o[i] = pack_h2(q4::value(q4::code_of(word, 2 * i), pair) * f,
-                       q4::value(q4::code_of(word, 2 * i + 1), pair) * f);
+      for (int k = 0; k < 4; ++k)
+        o[k] = pack_h2(q4::value(q4::code_of(x[i].x, 2 * k), x[i].y) * f,
+                       q4::value(q4::code_of(x[i].x, 2 * k + 1), x[i].y) * f);
     }
+    __half *dst = which[i] == 0 ? p.qo + (bh * p.q_rows + row[i]) * kPad
+                                : (which[i] == 2 ? p.vo : p.ko) + (bh * p.pad + row[i]) * kPad;
+    reinterpret_cast<uint4 *>(dst)[ch] = make_uint4(o[0], o[1], o[2], o[3]);
   }
-  __half *dst = which == 0 ? p.qo + (bh * p.q_rows + row) * kPad
-                           : (which == 2 ? p.vo : p.ko) + (bh * p.pad + row) * kPad;
-  reinterpret_cast<uint4 *>(dst)[ch] = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// One warp per query row: joins the splits.
+// Joins the splits; a thread owns 4 channels of a query row.
 __global__ void __launch_bounds__(kThreads) attn_q4_splits_kernel(F16Extra x, uint16_t *out, int Hq,
                                                                   int64_t Sq) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t row = i / (x.D / 4);
+  const int ch = static_cast<int>(i - row * (x.D / 4)) * 4;
   if (row >= x.rows) return;
   const float2 *ml = reinterpret_cast<const float2 *>(x.part + x.rows * x.splits * x.D) + row * x.splits;
-  const float *part = x.part + row * x.splits * x.D;
-  float top = -FLT_MAX, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  const float *part = x.part + row * x.splits * x.D + ch;
+  float top = -FLT_MAX, l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s = 0; s < x.splits; ++s) top = fmaxf(top, ml[s].x);
+#pragma unroll 2
   for (int s = 0; s < x.splits; ++s) {
     const float2 w = ml[s];
+    const float4 o = *reinterpret_cast<const float4 *>(part + int64_t(s) * x.D);
     const float f = exp2f(w.x - top);
     l = fmaf(w.y, f, l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (32 * e < x.D) v[e] = fmaf(part[int64_t(s) * x.D + 32 * e + lane], f, v[e]);
+    v.x = fmaf(o.x, f, v.x);
+    v.y = fmaf(o.y, f, v.y);
+    v.z = fmaf(o.z, f, v.z);
+    v.w = fmaf(o.w, f, v.w);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t b = row / (Hq * Sq), h = row / Sq % Hq, s = row % Sq;
-  uint16_t *dst = out + ((b * Sq + s) * Hq + h) * x.D + lane;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (32 * e < x.D) dst[32 * e] = f2bf(v[e] * inv);
+  const int64_t bh = row / Sq, sq = row - bh * Sq, b = bh / Hq, h = bh - b * Hq;
+  *reinterpret_cast<uint2 *>(out + ((b * Sq + sq) * Hq + h) * x.D + ch) =
+      make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
 }
 
 // Splits of the key tiles and the workspace's parts, in bytes.
 struct Plan {
-  int splits, tiles_per_split, pad;
-  int64_t fac, ko, vo, qo, part, bytes;
+  int splits, tiles_per_split, pad, slices;
+  int64_t v_scale, ko, vo, qo, part, bytes;
 };
 Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   Plan pl{};
@@ -194,8 +219,11 @@ Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   pl.splits = (tiles + pl.tiles_per_split - 1) / pl.tiles_per_split;
   pl.pad = static_cast<int>(tiles * tile);
   const int64_t bh = B * Hkv, rows = B * Hq * Sq;
-  pl.fac = kSlices * bh * int64_t(sizeof(float4));
-  pl.ko = pl.fac + (bh * int64_t(sizeof(float2)) + 15) / 16 * 16;
+  // about four CTAs per SM read for the largest values
+  const int64_t slices = 4 * int64_t(num_sms()) / bh;
+  pl.slices = static_cast<int>(slices < 2 ? 2 : slices > kMaxSlices ? kMaxSlices : slices);
+  pl.v_scale = pl.slices * bh * int64_t(sizeof(float4));
+  pl.ko = pl.v_scale + (bh * int64_t(sizeof(float)) + 15) / 16 * 16;
   pl.vo = pl.ko + bh * pl.pad * kPad * 2;
   pl.qo = pl.vo + bh * pl.pad * kPad * 2;
   pl.part = pl.qo + rows * kPad * 2;
@@ -249,7 +277,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
               static_cast<uint32_t *>(const_cast<void *>(v_codes)),
               static_cast<uint32_t *>(const_cast<void *>(v_scales))};
   c.maxima = reinterpret_cast<float4 *>(ws);
-  c.fac = reinterpret_cast<float2 *>(ws + pl.fac);
+  c.v_scale = reinterpret_cast<float *>(ws + pl.v_scale);
   c.ko = reinterpret_cast<__half *>(ws + pl.ko);
   c.vo = reinterpret_cast<__half *>(ws + pl.vo);
   c.qo = reinterpret_cast<__half *>(ws + pl.qo);
@@ -259,15 +287,16 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   c.cap = cap;
   c.len = static_cast<int>(kv_len);
   c.pad = pl.pad;
+  c.slices = pl.slices;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const unsigned bh = static_cast<unsigned>(B * Hkv);
-  attn_q4_absmax_kernel<<<dim3(kSlices, bh), kThreads, 0, s>>>(c);
+  attn_q4_absmax_kernel<<<dim3(pl.slices, bh), kThreads, 0, s>>>(c);
   Q35_LAUNCH_CHECK("attn_q4 absmax launch");
-  const int64_t rows = 2 * int64_t(c.pad) + c.q_rows;
-  attn_q4_operands_kernel<<<dim3(static_cast<unsigned>((rows + 15) / 16), bh), kThreads, 0, s>>>(c);
+  const int64_t rows = 2 * int64_t(c.pad) + c.q_rows, step = kRows * kThreads / 16;
+  attn_q4_operands_kernel<<<dim3(static_cast<unsigned>((rows + step - 1) / step), bh), kThreads, 0, s>>>(c);
   Q35_LAUNCH_CHECK("attn_q4 operands launch");
   F16Extra x{};
-  x.fac = c.fac;
+  x.v_scale = c.v_scale;
   x.rows = B * Hq * Sq;
   x.splits = pl.splits;
   x.tiles_per_split = pl.tiles_per_split;
@@ -276,7 +305,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   st = attn_tc_f16(c.qo, c.ko, c.vo, out, B, Hq, Hkv, Sq, kv_len, c.pad, scale, causal, x, stream);
   if (st) return st;
   if (pl.splits > 1) {
-    attn_q4_splits_kernel<<<static_cast<unsigned>((x.rows + 7) / 8), kThreads, 0, s>>>(
+    attn_q4_splits_kernel<<<static_cast<unsigned>((x.rows * (D / 4) + kThreads - 1) / kThreads), kThreads, 0, s>>>(
         x, static_cast<uint16_t *>(out), Hq, Sq);
     Q35_LAUNCH_CHECK("attn_q4 splits launch");
   }

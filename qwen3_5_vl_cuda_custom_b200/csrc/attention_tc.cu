@@ -196,13 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (p.causal) kv_end = min(p.Skv, m0 + kTile + diag);
   int n_tiles = kv_end > 0 ? static_cast<int>((kv_end + kTile - 1) / kTile) : 0;
   int j0 = 0;
-  float sl2 = p.sl2, f_out = 1.f;
-  if constexpr (kF16) {
-    n_tiles = split_tiles(p, blockIdx.z, n_tiles, j0);
-    const float2 f = p.x.fac[static_cast<int64_t>(b) * p.Hkv + hk];
-    sl2 *= f.x;
-    f_out = f.y;
-  }
+  if constexpr (kF16) n_tiles = split_tiles(p, blockIdx.z, n_tiles, j0);
   const int32_t q_row = static_cast<int32_t>((static_cast<int64_t>(b) * p.Hq + h) * p.Sq + m0);
   const int32_t kv_row = static_cast<int32_t>((static_cast<int64_t>(b) * p.Hkv + hk) * p.kv_cap);
 
@@ -329,8 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(r[i]);
       }
-      const int64_t n0 = static_cast<int64_t>(j0 + j) * kTile;
-      const int64_t lim = p.causal ? min(qi + diag, p.Skv - 1) : p.Skv - 1;
+      const int64_t n0 = static_cast<int64_t>(j) * kTile;
+      const int64_t lim = (p.causal ? min(qi + diag, p.Skv - 1) : p.Skv - 1) -
+                          static_cast<int64_t>(j0) * kTile;  // of the split's own keys
       if (n0 + kTile - 1 > lim) {
 #pragma unroll
         for (int c = 0; c < kTile; ++c)
@@ -344,14 +339,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * sl2 > 8.f) {
+      } else if ((m_new - m_used) * p.sl2 > 8.f) {
         need = true;
-        alpha = exp2f((m_used - m_new) * sl2);
+        alpha = exp2f((m_used - m_new) * p.sl2);
         m_used = m_new;
         l *= alpha;
       }
       const float mu = (m_used == -INFINITY) ? 0.f : m_used;
-      const float mus = mu * sl2;
+      const float mus = mu * p.sl2;
       // O may only be touched once PV_{j-1} has finished.
       if (j >= 1 && !sm100::mbar_wait(o_done, (j - 1) & 1)) {
         report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 307, j, row);
@@ -376,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float a = exp2_mufu(fmaf(s[half * 64 + 2 * i], sl2, -mus));
-          const float b2 = exp2_fma(fmaf(s[half * 64 + 2 * i + 1], sl2, -mus));
+          const float a = exp2_mufu(fmaf(s[half * 64 + 2 * i], p.sl2, -mus));
+          const float b2 = exp2_fma(fmaf(s[half * 64 + 2 * i + 1], p.sl2, -mus));
           l += a + b2;
           pk[i] = pack_p<kF16>(a, b2);
         }
@@ -399,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::tc_fence_after();
       const bool seen = done && m_used != -INFINITY;
       store_row_f16(p, tmem + lane_base, done, valid, b, h, qi, blockIdx.z,
-                    seen ? m_used * sl2 : -FLT_MAX, seen ? l : 0.f, seen ? f_out : 0.f);
+                    seen ? m_used * p.sl2 : -FLT_MAX, seen ? l : 0.f,
+                    seen ? p.x.v_scale[static_cast<int64_t>(b) * p.Hkv + hk] : 0.f);
     } else {
     uint16_t *orow = p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * 128;
     if (n_tiles > 0 && ok) {
@@ -515,13 +511,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
   if (p.causal) kv_end = min(p.Skv, m0 + kTile + diag);
   int n_tiles = kv_end > 0 ? static_cast<int>((kv_end + kTile - 1) / kTile) : 0;
   int j0 = 0;
-  float sl2 = p.sl2, f_out = 1.f;
-  if constexpr (kF16) {
-    n_tiles = split_tiles(p, blockIdx.y, n_tiles, j0);
-    const float2 f = p.x.fac[static_cast<int64_t>(b) * p.Hkv + hk];
-    sl2 *= f.x;
-    f_out = f.y;
-  }
+  if constexpr (kF16) n_tiles = split_tiles(p, blockIdx.y, n_tiles, j0);
   const int32_t kv_row = static_cast<int32_t>((static_cast<int64_t>(b) * p.Hkv + hk) * p.kv_cap);
 
   if (threadIdx.x == 0) {
@@ -658,7 +648,8 @@ __global__ void __launch_bounds__(kThreads2, 1)
     const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t o_tm = tmem + lane_base + hh * 256;
     const uint32_t s_tm = o_tm + 128;
-    const int64_t lim_c = p.causal ? min(qi + diag, p.Skv - 1) : p.Skv - 1;
+    const int64_t lim_c = (p.causal ? min(qi + diag, p.Skv - 1) : p.Skv - 1) -
+                          static_cast<int64_t>(j0) * kTile;  // of the split's own keys
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
@@ -668,7 +659,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
         break;
       }
       sm100::tc_fence_after();
-      const int64_t n0 = static_cast<int64_t>(j0 + j) * kTile;
+      const int64_t n0 = static_cast<int64_t>(j) * kTile;
       const bool masked = n0 + kTile - 1 > lim_c;
       // the whole score row in two 64-column loads, one wait
       uint32_t sr[kTile];
@@ -694,17 +685,17 @@ __global__ void __launch_bounds__(kThreads2, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * sl2 > 8.f) {
+      } else if ((m_new - m_used) * p.sl2 > 8.f) {
         need = true;
-        alpha = exp2f((m_used - m_new) * sl2);
+        alpha = exp2f((m_used - m_new) * p.sl2);
         m_used = m_new;
         l *= alpha;
       }
-      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * sl2;
+      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * p.sl2;
       // exponentials, bf16 P over the first 64 S columns.  Score pairs are
       // scaled with one f32x2 FMA; pairs alternate between the MUFU unit
       // (ex2.approx) and the paired FMA polynomial; row sums in f32x2.
-      const float2 sl2v = make_float2(sl2, sl2), nmus = make_float2(-mus, -mus);
+      const float2 sl2v = make_float2(p.sl2, p.sl2), nmus = make_float2(-mus, -mus);
       float2 lsum0 = make_float2(0.f, 0.f), lsum1 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int qtr = 0; qtr < 4; ++qtr) {
@@ -756,8 +747,8 @@ __global__ void __launch_bounds__(kThreads2, 1)
       done = __all_sync(0xffffffffu, done);
       sm100::tc_fence_after();
       const bool seen = done && m_used != -INFINITY;
-      store_row_f16(p, o_tm, done, valid, b, h, qi, blockIdx.y, seen ? m_used * sl2 : -FLT_MAX,
-                    seen ? l : 0.f, seen ? f_out : 0.f);
+      store_row_f16(p, o_tm, done, valid, b, h, qi, blockIdx.y, seen ? m_used * p.sl2 : -FLT_MAX,
+                    seen ? l : 0.f, seen ? p.x.v_scale[static_cast<int64_t>(b) * p.Hkv + hk] : 0.f);
     } else {
     uint16_t *orow = p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * 128;
     if (n_tiles > 0 && ok) {

@@ -7,7 +7,7 @@
 namespace q35 {
 
 struct F16Extra {
-  const float2 *fac;    // per (sequence, kv head): factors of the scores and of the output
+  const float *v_scale; // [B * Hkv]: what the output is multiplied by
   float *part;          // fp32 partials [rows, splits, D], then (m, l) [rows, splits]; or null
   int64_t rows;         // B * Hq * Sq
   int splits, tiles_per_split, D;
