@@ -500,7 +500,8 @@ Q35_API int q35_kv_read_q4(const void *k_codes, const void *k_scales, const void
  * kv head (a decode step, drafted tokens).  causal != 0: query s sees keys
  * <= s + len - Sq.  A query that sees no key gives zeros.  A kv_lens entry
  * outside [0, kv_len] is clamped and recorded as a device error (code 2, site
- * 311).  workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.      */
+ * 311).  Exact in its scaling for |q| < 2^75 and |v| between 2^-60 and 2^58 (beyond:
+ * infinite, or rounded to 0).  workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.      */
 Q35_API int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D);
 Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_scales,
@@ -514,6 +515,8 @@ Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_sc
  * (q35_attn_q4_chunk_workspace(...) bytes, 16-byte aligned) and the tensor-memory
  * attention kernels.  B * Hq <= 65535.  A key or value that is not finite may reach
  * all rows that share its 128-key tile, as in q35_attn_prefill_cache_fwd.     */
+Q35_API int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
+                                      int D); /* 1: estimated faster than q35_attn_q4_fwd */
 Q35_API int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64_t Sq,
                                             int64_t kv_len, int D);
 Q35_API int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const void *k_scales,

@@ -125,6 +125,7 @@ _SIGS = {
     "q35_attn_q4_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                 c_int, c_int, c_int64, c_int64, c_void_p, c_int64, c_int, c_int,
                                 c_float, c_int, c_void_p, c_void_p]),
+    "q35_attn_q4_prefers_chunk": (c_int, [c_int64, c_int, c_int, c_int64, c_int64, c_int]),
     "q35_attn_q4_chunk_workspace": (c_int64, [c_int64, c_int, c_int, c_int64, c_int64, c_int]),
     "q35_attn_q4_chunk_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                       c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int,

@@ -42,6 +42,7 @@ struct Chunk {
   int64_t cap;
   int len, pad;          // keys, and their rows in ko / vo
   int slices;
+  float q_sign;          // of the scale: the attention kernels want it positive
 };
 
 __device__ __forceinline__ float largest(float a, float x) {
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
     for (int i = 0; i < 3; ++i) e[i] = exponent(warp_max(m[i]));
     if (threadIdx.x == 0) {
       const int a = max(-100, min((e[0] - e[1]) / 2, 100)), v = max(-100, min(e[2] - 14, 100));
-      scale[0] = pow2(-a);
+      scale[0] = pow2(-a) * p.q_sign;
       scale[1] = pow2(a);
       scale[2] = pow2(-v);
       if (blockIdx.x == 0) p.v_scale[bh] = pow2(v);
@@ -248,6 +249,27 @@ extern "C" int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64
   return plan(B, Hq, Hkv, Sq, kv_len, D).bytes;
 }
 
+// Fitted to 542 shapes (head_dim 64 and 128, 8 to 32 heads on 1 to 8, 1 to 16
+// sequences, 4 to 512 queries, 512 to 32768 keys); its choice costs 0.8 % on average
+// over the better of the two measured times, a fixed limit of 256 rows 14 %.  In
+// microseconds: on the codes 16 query rows pass over all keys at a time; in chunks
+// a 128-key tile takes 2 in each of the CTAs the GPU holds, and the operands move at
+// 3.7 TB/s.  (512 queries x 32 heads, 8704 keys: 354 on the codes, 102 in chunks;
+// 16 queries x 32 heads, 8192 keys: 21 and 46.)
+extern "C" int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
+                                         int D) {
+  if (!plannable(B, Hq, Hkv, Sq, kv_len) || Hq % Hkv != 0 || B * Hq > 65535) return 0;
+  const Plan pl = plan(B, Hq, Hkv, Sq, kv_len, D);
+  int64_t tile;
+  const double ctas = static_cast<double>(attn_tc_ctas(B, Hq, Hkv, Sq, &tile)) * pl.splits;
+  const double waves = static_cast<double>((static_cast<int64_t>(ctas) + num_sms() - 1) / num_sms());
+  const double rows = static_cast<double>(Hq / Hkv * Sq), keys = static_cast<double>(B) * Hkv * kv_len;
+  const double bytes = keys * (1.25 * D + 1024) + static_cast<double>(B) * Hq * Sq * 768;
+  const double chunk = 14 + 2 * waves * pl.tiles_per_split + bytes * 0.27e-6;
+  const double codes = 9.4 + keys * ((rows + 15) / 16) * (D + 64) * 0.227e-6;
+  return chunk < codes ? 1 : 0;
+}
+
 extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const void *k_scales,
                                      const void *v_codes, const void *v_scales, void *out,
                                      int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
@@ -288,6 +310,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   c.len = static_cast<int>(kv_len);
   c.pad = pl.pad;
   c.slices = pl.slices;
+  c.q_sign = scale < 0.f ? -1.f : 1.f;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const unsigned bh = static_cast<unsigned>(B * Hkv);
   attn_q4_absmax_kernel<<<dim3(pl.slices, bh), kThreads, 0, s>>>(c);
@@ -302,7 +325,9 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   x.tiles_per_split = pl.tiles_per_split;
   x.D = D;
   x.part = pl.splits > 1 ? reinterpret_cast<float *>(ws + pl.part) : nullptr;
-  st = attn_tc_f16(c.qo, c.ko, c.vo, out, B, Hq, Hkv, Sq, kv_len, c.pad, scale, causal, x, stream);
+  // (a scale of 0 would turn masked scores into 0 * inf)
+  st = attn_tc_f16(c.qo, c.ko, c.vo, out, B, Hq, Hkv, Sq, kv_len, c.pad, fmaxf(fabsf(scale), 1e-30f),
+                   causal, x, stream);
   if (st) return st;
   if (pl.splits > 1) {
     attn_q4_splits_kernel<<<static_cast<unsigned>((x.rows * (D / 4) + kThreads - 1) / kThreads), kThreads, 0, s>>>(

@@ -671,9 +671,11 @@ def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Ten
     return _read_q4(cache, shape, 0 if starts is not None else int(start), starts, int(length), int(length))
 
 
-# Query rows per kv head from which attention_cache_q4 takes the form for chunks of
-# a prompt instead of attending over the codes.
-_Q4_CHUNK_ROWS = 256
+def _q4_chunk(B: int, Hq: int, Hkv: int, Sq: int, kv_len: int, D: int) -> bool:
+    """Whether attention_cache_q4 takes the form for chunks of a prompt (a cost
+    estimate; up to 16 query rows per kv head never do)."""
+    return (Hq // Hkv) * Sq > 16 and kv_len > 0 and bool(
+        _lib.query("q35_attn_q4_prefers_chunk", B, Hq, Hkv, Sq, kv_len, D))
 
 
 def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
@@ -708,7 +710,7 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     if n < 0 or n > cap:
         raise RuntimeError(f"attention_cache_q4: {n} rows exceed the capacity {cap}")
     out = torch.empty(B, Sq, Hq * D, device=q.device, dtype=q.dtype)
-    if lens is None and (Hq // Hkv) * Sq >= _Q4_CHUNK_ROWS and n > 0:
+    if lens is None and _q4_chunk(B, Hq, Hkv, Sq, n, D):
         w = _lib.query("q35_attn_q4_chunk_workspace", B, Hq, Hkv, Sq, n, D)
         ws = torch.empty(max(w, 16), device=q.device, dtype=torch.uint8)
         _call_on(q.device, "q35_attn_q4_chunk_fwd", q.data_ptr(), *[t.data_ptr() for t in cache],

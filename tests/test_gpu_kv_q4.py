@@ -194,6 +194,7 @@ def check_attention(out, q, kv, vv, lens, scale, causal, group, chunk=False):
     # per key at most: values lie in [m, m + 15 s], so s <= 2/15 max|k| and |m| <= max|k|
     ka = kv.abs().amax(dim=(0, 1, 2)) if kv.numel() else torch.zeros_like(qa)
     groups = ka.view(-1, group).amax(-1).repeat_interleave(group)
+    scale = abs(scale)
     d = 2.0 ** -19 * scale * float((qa * groups).sum()) * (128 * 2 / 15 + 1)
     if chunk:
         d += 2.0 ** -8 * scale * float((qa * ka).sum()) + 2.0 ** -13
@@ -256,6 +257,68 @@ def test_attention_of_a_chunk(Hq, Hkv, D, group, Sq, kv, causal):
     q = rows((B, Hq, Sq, D), 53, 0.5)
     out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, causal)
     check_attention(out, q, kk, vv, [kv] * B, D ** -0.5, causal, group, chunk=True)
+
+
+@pytest.mark.parametrize("D,group,B,Hq,Hkv,Sq,kv,causal", [
+    (128, 32, 1, 32, 4, 33, 1000, True),           # splits of the key tiles, joined
+    (128, 128, 2, 6, 2, 130, 257, True),           # one head per CTA, two query blocks
+    (128, 64, 1, 16, 1, 20, 5000, False),
+    (64, 32, 2, 8, 2, 70, 700, True), (64, 64, 1, 8, 8, 128, 128, True),
+    (32, 32, 3, 4, 2, 129, 90, True),              # queries that see nothing
+    (32, 32, 1, 7, 7, 5, 1, False), (128, 32, 2, 4, 4, 1, 131, True),
+])
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1.0, 1.0, 1.0), (1e-9, 1e9, 1e30), (3e4, 2e-5, 1e-30)])
+def test_attention_of_a_chunk_at_any_size_of_values(monkeypatch, D, group, B, Hq, Hkv, Sq, kv, causal,
+                                                    q_scale, k_scale, v_scale):
+    """The fp16 operands are scaled: values far outside fp16's range, and far apart.
+    Bounds: weights and values rounded to fp16 (2^-11 each); scores off by d from the
+    keys' rounding 2^-11 scale sum |q_d k_d| (bf16 queries are exact in fp16) and the
+    exponential's 2^-13; the output's rounding 2^-8."""
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: True)
+    cache, kk, vv = filled_cache(B, Hkv, -(-kv // 16) * 16, D, group, 55, 0.5)
+    codes = list(cache)
+    codes[1], codes[3] = (cache[1].double() * k_scale).bfloat16(), (cache[3].double() * v_scale).bfloat16()
+    kk = R.values(codes[0], codes[1])
+    vv = R.values(codes[2], codes[3])
+    q = (rows((B, Hq, Sq, D), 57, 0.5).double() * q_scale).bfloat16()
+    scale = D ** -0.5 / (q_scale * k_scale)
+    out = K().attention_cache_q4(q.to(DEV), *codes, kv, scale, causal).double().cpu()
+    ref, A = R.attention(q, kk, vv, [kv] * B, scale, causal)
+    d = 2.0 ** -11 * scale * float((q.double().abs().amax((0, 1, 2)) * kk.abs().amax((0, 1, 2))).sum())
+    tol = A * (2 ** -10 + math.expm1(2 * (d + 2.0 ** -13))) + 2 ** -8 * ref.abs() + 1e-38
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+def test_which_form_a_call_takes():
+    """A decode step, drafted tokens and a short chunk on the codes, long chunks by
+    the tensor-memory kernels (measured times in attention_q4_chunk.cu)."""
+    for B, Hq, Hkv, Sq, kv, D, chunk in ((1, 32, 4, 512, 8704, 128, True), (1, 32, 4, 16, 8192, 128, False),
+                                         (64, 32, 4, 4, 8192, 128, False), (1, 8, 2, 512, 32768, 64, True),
+                                         (64, 32, 4, 1, 8192, 128, False), (1, 32, 1, 1, 8192, 128, False)):
+        assert K()._q4_chunk(B, Hq, Hkv, Sq, kv, D) is chunk
+
+
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1e9, 1e-9, 1e15), (1e-12, 1e12, 1e-15), (1e3, 1e3, 1.0)])
+def test_attention_on_the_codes_at_far_sizes_of_values(q_scale, k_scale, v_scale):
+    B, Hq, Hkv, Sq, kv, D, group = 2, 8, 2, 2, 300, 128, 32
+    cache, _, _ = filled_cache(B, Hkv, 304, D, group, 75, 0.5)
+    cache = [cache[0], (cache[1].double() * k_scale).bfloat16(), cache[2], (cache[3].double() * v_scale).bfloat16()]
+    kk, vv = R.values(cache[0], cache[1]), R.values(cache[2], cache[3])
+    q = (rows((B, Hq, Sq, D), 77, 0.5).double() * q_scale).bfloat16()
+    scale = D ** -0.5 / (q_scale * k_scale)
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, scale, True)
+    check_attention(out, q, kk, vv, [kv] * B, scale, True, group)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+@pytest.mark.parametrize("chunk", [False, True])
+def test_scales_that_are_not_positive(monkeypatch, scale, chunk):
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: chunk)
+    B, Hq, Hkv, Sq, kv, D = 1, 8, 2, 3, 200, 64
+    cache, kk, vv = filled_cache(B, Hkv, 208, D, 64, 78)
+    q = rows((B, Hq, Sq, D), 79)
+    check_attention(K().attention_cache_q4(q.to(DEV), *cache, kv, scale, True), q, kk, vv, [kv], scale,
+                    True, 64, chunk=chunk)
 
 
 @pytest.mark.parametrize("Sq", [1, 3, 64])

@@ -89,6 +89,26 @@ def test_attention_refusals(lib, kw, status):
                                a["kv_len"], None, 16, a["D"], 32, 0.1, 0, p(256), None) == status
 
 
+@pytest.mark.parametrize("kw,status", [
+    (dict(Hq=7), 2), (dict(Sq=-1), 2), (dict(kv_len=17), 2), (dict(kv_len=0), 2), (dict(q=None), 1),
+    (dict(q=8), 3), (dict(ws=None), 1), (dict(ws=8), 3), (dict(D=80), 4), (dict(B=40000), 2),
+])
+def test_chunk_attention_refusals(lib, kw, status):
+    a = dict(B=1, Hq=8, Sq=64, kv_len=16, q=256, D=64, ws=256)
+    a.update(kw)
+    p = ctypes.c_void_p
+    assert lib.q35_attn_q4_chunk_fwd(p(a["q"]), p(256), p(256), p(256), p(256), p(256), a["B"], a["Hq"],
+                                     2, a["Sq"], a["kv_len"], 16, a["D"], 32, 0.1, 1, p(a["ws"]), None) == status
+
+
+def test_the_form_for_chunks_is_not_proposed_for_refused_shapes(lib):
+    prefers = lib.q35_attn_q4_prefers_chunk
+    for args in ((0, 32, 4, 4, 8192, 128), (1, 7, 2, 512, 8192, 128), (1, 8, 2, 512, 0, 128),
+                 (40000, 8, 2, 512, 8192, 128)):
+        assert prefers(*args) == 0
+    assert not K._q4_chunk(1, 32, 4, 2, 8192, 128) and not K._q4_chunk(1, 32, 4, 512, 0, 128)
+
+
 def test_workspace_covers_every_shape(lib):
     assert lib.q35_attn_q4_workspace(0, 8, 2, 1, 100, 64) >= 0
     assert lib.q35_attn_q4_workspace(64, 32, 4, 1, 8193, 128) >= 0
