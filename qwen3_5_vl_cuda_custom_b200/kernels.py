@@ -570,15 +570,16 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 def _cache_q4(name: str, k_codes, k_scales, v_codes, v_scales) -> tuple[int, int, int, int, int]:
     """Checks the four tensors of a 4-bit cache; returns (B, Hkv, capacity, D, group)."""
     cs, ss = k_codes.shape, k_scales.shape
-    if (len(cs) == 4 and len(ss) == 5 and cs == v_codes.shape and ss == v_scales.shape
-            and k_codes.dtype == v_codes.dtype == torch.uint8
-            and k_scales.dtype == v_scales.dtype == _BF16
-            and k_codes.is_cuda and k_codes.device == k_scales.device == v_codes.device == v_scales.device
-            and k_codes.is_contiguous() and v_codes.is_contiguous()
+    dev = k_codes.get_device()
+    if (len(cs) == 4 and len(ss) == 5 and cs == v_codes.shape and ss == v_scales.shape and dev >= 0
+            and k_codes.dtype is torch.uint8 and v_codes.dtype is torch.uint8
+            and k_scales.dtype is _BF16 and v_scales.dtype is _BF16
+            and k_scales.get_device() == dev and v_codes.get_device() == dev
+            and v_scales.get_device() == dev and k_codes.is_contiguous() and v_codes.is_contiguous()
             and k_scales.is_contiguous() and v_scales.is_contiguous()):
         B, Hkv, cap, half = cs
         D, groups = 2 * half, ss[3]
-        if D in (32, 64, 128) and groups > 0 and D % groups == 0 and ss == (B, Hkv, cap, groups, 2):
+        if (D == 128 or D == 64 or D == 32) and groups and not D % groups and ss == (B, Hkv, cap, groups, 2):
             return B, Hkv, cap, D, D // groups
     for t, part, dt, dims in ((k_codes, "k_codes", torch.uint8, 4), (k_scales, "k_scales", _BF16, 5),
                               (v_codes, "v_codes", torch.uint8, 4), (v_scales, "v_scales", _BF16, 5)):
