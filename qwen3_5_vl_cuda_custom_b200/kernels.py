@@ -694,8 +694,10 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     of the rows (256 bytes of K and V each per row) and the tensor-memory
     attention kernels."""
     cache = (k_codes, k_scales, v_codes, v_scales)
-    shape = _cache_q4("attention_cache_q4", *cache)
-    B, Hkv, cap, D, group = shape
+    B, Hkv, cap, D, group = _cache_q4("attention_cache_q4", *cache)
+    if torch.cuda.current_device() != k_codes.get_device():  # plans and workspaces are per device
+        with torch.cuda.device(k_codes.device):
+            return attention_cache_q4(q, *cache, kv_len, scale, causal, max_kv_len)
     q = _same_device(_require(q, "attention_cache_q4.q"), "attention_cache_q4.q", k_codes.device)
     if q.data_ptr() % 16:
         q = q.clone()

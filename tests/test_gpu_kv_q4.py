@@ -465,6 +465,61 @@ def test_a_captured_step_follows_the_lengths():
     K().device_error_check()
 
 
+@pytest.mark.parametrize("before", ["copy", "fill", "kernel", "two streams", "nothing"])
+@pytest.mark.parametrize("kv,Sq", [(40, 1), (3000, 1), (900, 200)])
+def test_a_capture_behind_other_work(monkeypatch, before, kv, Sq):
+    """The attention kernels are launched ahead of the work in front of them: what
+    that work writes (a copy, a fill, a kernel, the join of two streams) is what they
+    read, on every replay."""
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: Sq > 100)
+    B, Hq, Hkv, D = 2, 8, 2, 128
+    cache, _, _ = filled_cache(B, Hkv, 3008, D, 32, 121)
+    q, src = (torch.zeros(B, Hq, Sq, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    big = torch.zeros(1 << 24, device=DEV)
+    lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+    n = kv if Sq > 1 else lens
+
+    def work():
+        if before == "copy":
+            big.add_(1)
+            q.copy_(src)
+        elif before == "fill":
+            big.add_(1)
+            q.copy_(src)
+            big[:1024].zero_()
+        elif before == "kernel":
+            big.add_(1)
+            torch.mul(src, 1.0, out=q)
+        elif before == "two streams":
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                big.add_(1)
+                q.copy_(src)
+            lens.fill_(kv)
+            torch.cuda.current_stream().wait_stream(side)
+        if before != "two streams":
+            lens.fill_(kv)
+        if before == "nothing":
+            q.copy_(src)
+        return K().attention_cache_q4(q, *cache, n, 0.09, True)
+
+    warm = torch.cuda.Stream()
+    with torch.cuda.stream(warm):
+        work()
+    torch.cuda.current_stream().wait_stream(warm)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = work()
+    for i in range(3):
+        src.copy_(rows((B, Hq, Sq, D), 500 + i))
+        q.zero_()
+        lens.zero_()
+        g.replay()
+        want = K().attention_cache_q4(src, *cache, kv if Sq > 1 else torch.full_like(lens, kv), 0.09, True)
+        assert torch.equal(out, want), i
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_a_cache_on_another_device():
     cache, kk, vv = filled_cache(1, 2, 64, 64, 32, 111)
