@@ -235,17 +235,6 @@ __device__ __forceinline__ bool nonfinite(uint32_t pair) {
   return (((pair & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
 }
 
-// Programmatic dependent launch: the kernels below are launched before the one in
-// front of them in the stream has finished; nothing is read or written before
-// wait_for_earlier(), and the next launch is let in only behind it (else several
-// kernels in a row pile up and crowd some SMs).
-__device__ __forceinline__ void wait_for_earlier() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void let_next_launch() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 // One CTA = one run of tiles.
 template <int D, int GS, int NT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Params p) {
@@ -364,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
     copies_commit();
   };
   if (!p.kv_lens) wait_for_earlier();
-  let_next_launch();
+  let_next_launch();  // (in front of the wait, several kernels in a row would crowd some SMs)
 #pragma unroll 1
   for (int i = 0; i < L::kStages; ++i) issue();
 
@@ -941,17 +930,7 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
     constexpr int smem = Layout<d(), gs(), nt()>::kSmem;
     const int e = ensure_smem_attr(reinterpret_cast<const void *>(kern), smem);
     if (e) return e;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    cfg.stream = s;
-    cfg.gridDim = dim3(pl.runs);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    Q35_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+    Q35_CHECK_CUDA(launch_early(kern, dim3(pl.runs), dim3(kThreads), smem, s, p));
     Q35_LAUNCH_CHECK("attn_q4 launch");
     if (pl.join) {
       // about runs / groups partials a row: 1 or 2, around a dozen, a hundred
@@ -959,10 +938,8 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
       auto *join = each < 4    ? &attn_q4_join_kernel<d(), 2, 2>
                    : each < 32 ? &attn_q4_join_kernel<d(), 8, 2>
                                : &attn_q4_join_kernel<d(), 16, 8>;
-      cfg.gridDim = dim3(static_cast<unsigned>(rows));
-      cfg.blockDim = dim3(each < 4 ? 64 : each < 32 ? 8 * 32 : 512);
-      cfg.dynamicSmemBytes = 0;
-      Q35_CHECK_CUDA(cudaLaunchKernelEx(&cfg, join, p, 8 * nt()));
+      Q35_CHECK_CUDA(launch_early(join, dim3(static_cast<unsigned>(rows)),
+                                  dim3(each < 4 ? 64 : each < 32 ? 256 : 512), 0, s, p, 8 * nt()));
       Q35_LAUNCH_CHECK("attn_q4 join launch");
     }
     return Q35_OK;

@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_absmax_kernel(Chunk p) {
     m[i] = warp_max(m[i]);
     if ((threadIdx.x & 31) == 0) part[i][threadIdx.x >> 5] = m[i];
   }
+  let_next_launch();
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
@@ -129,6 +130,9 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
       x[i].y = (v ? p.c.v_scales : p.c.k_scales)[at * (p.D / p.group) + 8 * ch / p.group];
     }
   }
+  // (the kernel in front was launched behind all that wrote q and the cache)
+  wait_for_earlier();
+  let_next_launch();
   if (threadIdx.x < 32) {
     float m[3] = {0.f, 0.f, 0.f};
     for (int s = threadIdx.x; s < p.slices; s += 32) {
@@ -175,6 +179,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
 // Joins the splits; a thread owns 4 channels of a query row.
 __global__ void __launch_bounds__(kThreads) attn_q4_splits_kernel(F16Extra x, uint16_t *out, int Hq,
                                                                   int64_t Sq) {
+  wait_for_earlier();
   const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t row = i / (x.D / 4);
   const int ch = static_cast<int>(i - row * (x.D / 4)) * 4;
@@ -316,7 +321,9 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   attn_q4_absmax_kernel<<<dim3(pl.slices, bh), kThreads, 0, s>>>(c);
   Q35_LAUNCH_CHECK("attn_q4 absmax launch");
   const int64_t rows = 2 * int64_t(c.pad) + c.q_rows, step = kRows * kThreads / 16;
-  attn_q4_operands_kernel<<<dim3(static_cast<unsigned>((rows + step - 1) / step), bh), kThreads, 0, s>>>(c);
+  Q35_CHECK_CUDA(launch_early(attn_q4_operands_kernel,
+                              dim3(static_cast<unsigned>((rows + step - 1) / step), bh), dim3(kThreads),
+                              0, s, c));
   Q35_LAUNCH_CHECK("attn_q4 operands launch");
   F16Extra x{};
   x.v_scale = c.v_scale;
@@ -330,8 +337,9 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
                    causal, x, stream);
   if (st) return st;
   if (pl.splits > 1) {
-    attn_q4_splits_kernel<<<static_cast<unsigned>((x.rows * (D / 4) + kThreads - 1) / kThreads), kThreads, 0, s>>>(
-        x, static_cast<uint16_t *>(out), Hq, Sq);
+    Q35_CHECK_CUDA(launch_early(
+        attn_q4_splits_kernel, dim3(static_cast<unsigned>((x.rows * (D / 4) + kThreads - 1) / kThreads)),
+        dim3(kThreads), 0, s, x, static_cast<uint16_t *>(out), Hq, Sq));
     Q35_LAUNCH_CHECK("attn_q4 splits launch");
   }
   return Q35_OK;

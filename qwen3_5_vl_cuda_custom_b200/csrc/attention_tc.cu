@@ -220,6 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  if constexpr (kF16) {
+    wait_for_earlier();
+    let_next_launch();
+  }
 
   if (warp == 0 && lane == 0 && n_tiles > 0) {
     // ------------------------------------------------ TMA producer
@@ -536,6 +540,10 @@ __global__ void __launch_bounds__(kThreads2, 1)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  if constexpr (kF16) {
+    wait_for_earlier();
+    let_next_launch();
+  }
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsCtl2));
@@ -837,7 +845,11 @@ int launch_tc(const void *q, const void *k, const void *v, AttnParams &p, int64_
                       "the register split needs %d", fa.numRegs, kRegsLaunch2);
         regs_ok = true;
       }
-      kern<<<grid2, kThreads2, kSmem2, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tv, p);
+      if constexpr (kF16)
+        Q35_CHECK_CUDA(launch_early(kern, grid2, dim3(kThreads2), kSmem2,
+                                    reinterpret_cast<cudaStream_t>(stream), tq, tk, tv, p));
+      else
+        kern<<<grid2, kThreads2, kSmem2, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tv, p);
       return 0;
     };
     int st3 = go(attn_tc2_kernel<np, kF16>);
@@ -847,7 +859,11 @@ int launch_tc(const void *q, const void *k, const void *v, AttnParams &p, int64_
   }
   { const int _st = ensure_smem_attr(reinterpret_cast<const void *>(attn_tc_kernel<kF16>), kSmem); if (_st) return _st; }
   dim3 grid(p.n_mblocks, static_cast<unsigned>(B * p.Hq), splits);
-  attn_tc_kernel<kF16><<<grid, kThreads, kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tv, p);
+  if constexpr (kF16)
+    Q35_CHECK_CUDA(launch_early(attn_tc_kernel<kF16>, grid, dim3(kThreads), kSmem,
+                                reinterpret_cast<cudaStream_t>(stream), tq, tk, tv, p));
+  else
+    attn_tc_kernel<kF16><<<grid, kThreads, kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(tq, tk, tv, p);
   Q35_LAUNCH_CHECK("attn_prefill_tc launch");
   return Q35_OK;
 }
