@@ -3,11 +3,12 @@
 // With hundreds of rows per key the products belong on the tensor-memory attention
 // kernels, which want dense operands; reading the rows back once costs 5 % of the
 // attention of a 512-token chunk (32 heads, 8704 keys).  But rounding the keys to
-// bf16 on the way shows: a score moves by 2^-9 of its terms, 3 times the error of all
-// other roundings together.  So the operands are fp16, whose 11 bits make it vanish,
-// scaled per sequence and kv head by powers of two, for the range that bf16 has and
-// fp16 has not: v to a largest value in [2^13, 2^14), q and k against one another to
-// largest values of like size, so that the scores stay what they are.
+// bf16 on the way shows: a score moves by up to 2^-8 of its terms and the output by
+// 0.0048 (relative, normal data), against 0.0017 from its own rounding to bf16.  So
+// the operands are fp16, whose 11 bits make it vanish, scaled per sequence and kv head
+// by powers of two, for the range that bf16 has and fp16 has not: v to a largest value
+// in [2^13, 2^14), q and k against one another to largest values of like size, so that
+// the scores stay what they are.
 //
 //   1. attn_q4_absmax_kernel: largest |q|, |k|, |v| of each kv head (k, v from the
 //      scales alone, a fifth of the cache's bytes).
@@ -16,6 +17,9 @@
 //      has SMs (512 tokens x 32 heads: 64 CTAs), so the key tiles are cut into as many
 //      splits as fill it, which leave fp32 partials ...
 //   4. attn_q4_splits_kernel: ... joined here.
+//
+// Measured, that chunk: 97 us (attention 78, the rest mostly operands), 0.43 of the
+// measured matrix peak; relative error 0.0018.
 #include <cuda_fp16.h>
 #include <float.h>
 

@@ -3,8 +3,8 @@
 // For a group of `group` channels with minimum m and maximum M:
 //   s = bf16((M - m) / 15), c = min(15, rint((x - m) / s)), value = m + c s.
 // m is a bf16 input and is stored exactly; s is rounded to nearest once and the
-// codes are taken with the rounded s, so a value is off by s/2 plus at most
-// 15 * 2^-9 s at the top of its group.  s = 0 (all equal, or (M - m) / 15 below
+// codes are taken with the rounded s, so a value is off by at most s/2, and by
+// 15 * 2^-8 s more at the top of its group.  s = 0 (all equal, or (M - m) / 15 below
 // the smallest bf16) stores codes of 0.  A group that holds a NaN or an infinity
 // stores s = m = NaN and reads back as NaN.
 //
@@ -14,6 +14,11 @@
 // HBM feeds about 1.2 words per SM and clock, so about 100 instructions are what a
 // word may cost: hence paired fp32 arithmetic, one shuffle a step for minimum and
 // maximum together, and a multiplication for each division by S or Hkv.
+//
+// Measured (4 kv heads x 128): 8 x 8192 rows appended in 46.5 us, 3.7 TB/s (bound by
+// its 290 instructions per warp and 512 channels: ties and their tests are a fifth),
+// 4096 rows 4.5 us, 64 sequences x 1 row 2.0 us; 16 x 8192 rows read in 58.5 us,
+// 6.0 TB/s.
 #include <type_traits>
 
 #include "kv_q4.cuh"
@@ -24,6 +29,8 @@ namespace {
 using q4::Cache;
 
 constexpr int kThreads = 256;
+// A CTA prefetches its next rows while it quantises: 7 CTAs of 128 threads per SM hold
+// in registers (8 x 8192 rows: 4 CTAs 50.0 us, 7 46.5, 10 with spills 58.8).
 constexpr int kAppendThreads = 128, kAppendCtas = 7;
 
 struct Rows {
