@@ -93,28 +93,23 @@ __device__ __forceinline__ float code_exact(float x, float lo, float s) {
   const double y = (static_cast<double>(x) - static_cast<double>(lo)) / static_cast<double>(s);
   return static_cast<float>(fmin(rint(y), 15.0));
 }
-// The same for a quotient y known to lie next to a half, in fp32: n + 1/2 is the
-// border, (n + 1/2) s has at most 13 significant bits, x - lo = d + err exactly
-// (Knuth's two-sum), and d lies next to the border, so the differences are exact.
-__device__ __forceinline__ float code_at_border(float x, float lo, float s, float y) {
-  const float n = rintf(y - 0.5f), border = (n + 0.5f) * s;
-  const float d = x - lo, z = d - x;
-  const float err = (x - (d - z)) + (-lo - z);
-  const float u = (d - border) + err;
-  const bool odd = static_cast<int>(n) & 1;
-  return (u > 0.f || (u == 0.f && odd)) ? n + 1.f : n;
-}
 
 // 16 channels w (bf16 pairs) of a group -> their code words; `pair` receives the
 // group's (scale, minimum).  The threads of a group are neighbours.
 //
-// With r within 2^-23 of 1/s the fp32 value y = x r + (-m r) is off by less than
-// 15 * 2^-23 (r), 2^-24 |m| r (the rounded -m r) and 2^-20 (the sum): a code can only
-// differ from the 64-bit rule when y lies within 1e-5 + 2^-23 |m| r of a half.  Exact
-// halves are common (x - m and s have few bits: one channel in 500), so those channels
-// are decided on their own in exact fp32 steps, as are scales within 4 fp32 steps of
-// a bf16 border.  Groups outside the range in which 1/s and M - m are normal numbers
-// take 64 bits.
+// The codes are the 64-bit rule's, halves included (x - m and s have few bits: one
+// channel in 500 lies exactly on a half).  With d = x - m, r within 2^-24 of 1/s and
+// y0 = d r, the rest d - y0 s is exact in one fma (it has at most 10 bits), so
+// y = y0 + rest r is d / s rounded to fp32, but for 2^-23 of a step.  If d is exact, it
+// is either (n + 1/2) s, then y = n + 1/2, or off by a step of d at least, which is more
+// than 0.502 steps of y: then y lies on the side of d / s.  d is not exact only where
+//   |m| < 2^-16 d, not 0: then |m / s| < 2^-12;
+//   |x| < 2^-16 |m|, not 0: such an x can only matter where -m / s is within 2^-12 of a
+//   half itself.
+// Groups of the first kind (one in some thousands, if their values have one sign) and
+// the tiny channels of groups of the second are decided in 64 bits one by one, and so
+// are groups outside the range in which 1/s and M - m are normal numbers.  A scale
+// within 4 fp32 steps of a bf16 border is decided in exact fp32 steps.
 template <int GT>  // threads per group: 2, 4 or 8
 __device__ __forceinline__ void quantise16(const uint32_t (&w)[8], uint32_t (&word)[2],
                                            uint32_t &pair) {
@@ -151,32 +146,21 @@ __device__ __forceinline__ void quantise16(const uint32_t (&w)[8], uint32_t (&wo
   if (s == 0.f) return;
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
-  const float c = -lo * r;
+  r = fmaf(r, fmaf(-s, r, 1.f), r);
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
-  const float2 r2 = make_float2(r, r), c2 = make_float2(c, c), up = make_float2(kRound, kRound),
-               down = make_float2(-kRound, -kRound), neg = make_float2(-1.f, -1.f);
+  const float2 r2 = make_float2(r, r), m2 = make_float2(-lo, -lo), s2 = make_float2(-s, -s),
+               up = make_float2(kRound, kRound), down = make_float2(-kRound, -kRound);
   const float2 k16 = make_float2(16.f, 16.f), k23 = make_float2(8388608.f, 8388608.f);
-  const float near = 0.49999f - fabsf(c) * 1.1920929e-7f;
-  uint32_t todo = 0;  // channels to decide on their own
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float2 q[4], e[4];
-    float off = 0.f;
+    float2 q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 v;
       unpack_bf2(w[4 * h + i], v.x, v.y);
-      const float2 y = __ffma2_rn(v, r2, c2);
+      const float2 d = __fadd2_rn(v, m2), y0 = __fmul2_rn(d, r2);
+      const float2 y = __ffma2_rn(__ffma2_rn(y0, s2, d), r2, y0);
       q[i] = __fadd2_rn(__fadd2_rn(y, up), down);
-      e[i] = __ffma2_rn(q[i], neg, y);
-      off = fmaxf(fmaxf(off, fabsf(e[i].x)), fabsf(e[i].y));
-    }
-    if (!(off < near)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!(fabsf(e[i].x) < near)) todo |= 1u << (8 * h + 2 * i);
-        if (!(fabsf(e[i].y) < near)) todo |= 2u << (8 * h + 2 * i);
-      }
     }
     // (even channels, odd channels): sums of 16^i code_i are integers below 2^16, which
     // 2^23 puts into the low bits
@@ -185,7 +169,18 @@ __device__ __forceinline__ void quantise16(const uint32_t (&w)[8], uint32_t (&wo
     f = __fadd2_rn(__ffma2_rn(f, k16, q[0]), k23);
     word[h] = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410);
   }
-  if (!plain) todo = 0xffffu;
+  const float c = -lo * r;
+  uint32_t todo = 0;  // channels to decide in 64 bits
+  if (!plain || (lo != 0.f && fabsf(c) < 0x1p-11f)) {
+    todo = 0xffffu;
+  } else if (c < 16.f && fabsf(c - floorf(c) - 0.5f) < 0x1p-11f) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const uint32_t two = w[k >> 1] & 0x7fff7fffu;
+      const float x = __uint_as_float(k & 1 ? two & 0xffff0000u : two << 16) * r;
+      if (x > 0.f && x < 0x1p-11f) todo |= 1u << k;
+    }
+  }
 #pragma unroll 1
   while (todo) {
     const int k = __ffs(todo) - 1, i = k >> 1;  // channel k of the 16
@@ -194,8 +189,7 @@ __device__ __forceinline__ void quantise16(const uint32_t (&w)[8], uint32_t (&wo
                    a3 = i & 1 ? w[7] : w[6];
     const uint32_t b0 = i & 2 ? a1 : a0, b1 = i & 2 ? a3 : a2, two = i & 4 ? b1 : b0;
     const float x = __uint_as_float(k & 1 ? two & 0xffff0000u : two << 16);
-    const uint32_t code = static_cast<uint32_t>(
-        plain ? code_at_border(x, lo, s, fmaf(x, r, c)) : code_exact(x, lo, s));
+    const uint32_t code = static_cast<uint32_t>(code_exact(x, lo, s));
     const int at = 4 * ((i & 3) + 4 * (k & 1));
     const uint32_t keep = ~(15u << at), put = code << at;
     if (k < 8) word[0] = (word[0] & keep) | put;

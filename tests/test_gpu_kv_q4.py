@@ -118,6 +118,50 @@ def test_append_where_rounding_is_delicate(name):
     check_stored(cache[2], cache[3], x.flip(2), group)
 
 
+@pytest.mark.parametrize("exponent", [-60, 0, 60])
+def test_append_halves_next_to_values_too_small_to_subtract(exponent):
+    """Quotients that are a half but for a value (the channel's or the minimum) whose
+    difference from the other needs more than fp32's 24 bits, and halves of every
+    scale of few bits."""
+    group, rows_ = 32, []
+    for k in range(4, 45):
+        for sign in (-1.0, 1.0):
+            small = sign * 2.0 ** -k
+            row = torch.arange(32) * 0.5 - 1.5             # s = 1, every half
+            row[2], row[3], row[4], row[31] = small, -small, 1.5 * small, 13.5
+            rows_.append(row)
+            row = torch.arange(32) * 0.5                   # minimum next to 0
+            row[0], row[31] = (small, 15.0) if sign < 0 else (1e-3 * small, 15.0)
+            rows_.append(row)
+    for n in range(1, 128):                                # s = n / 8, halves and their neighbours
+        c = torch.arange(32).double() / 2
+        x = ((c - 3) * n / 8).float().bfloat16().float()
+        x[0], x[31] = -3 * n / 8, 12 * n / 8
+        rows_.append(x)
+    x = (torch.stack(rows_) * 2.0 ** exponent).bfloat16()
+    x = x[:x.shape[0] // 4 * 4].view(1, 1, -1, 128).contiguous()
+    S = x.shape[2]
+    cache = empty_cache(1, 1, S + -S % 16, 128, group)
+    K().kv_append_q4(x.to(DEV), (-x).to(DEV), *cache, 0)
+    check_stored(cache[0][:, :, :S], cache[1][:, :, :S], x, group)
+    check_stored(cache[2][:, :, :S], cache[3][:, :, :S], -x, group)
+
+
+@pytest.mark.parametrize("D,group", SHAPES)
+def test_append_of_many_random_groups(D, group):
+    """Every scale, minimum and code of many groups, values of few bits
+    (many quotients on a half) and of many."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    S = 1 << 14
+    x = torch.randn(1, 2, S, D, generator=g, device=DEV)
+    x[:, 1] = (x[:, 1] * torch.exp2(torch.rand(S, 1, generator=g, device=DEV) * 6)).round() * 0.25
+    x = x.bfloat16()
+    cache = empty_cache(1, 2, S, D, group)
+    K().kv_append_q4(x, x.flip(3), *cache, 0)
+    check_stored(cache[0], cache[1], x.cpu(), group)
+    check_stored(cache[2], cache[3], x.flip(3).cpu(), group)
+
+
 def test_append_takes_strided_rows_and_per_sequence_offsets():
     B, Hkv, S, D, cap = 3, 4, 5, 64, 64
     k = rows((B, S, Hkv, D), 5).to(DEV).transpose(1, 2)  # token-major, no copy
