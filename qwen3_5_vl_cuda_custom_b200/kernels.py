@@ -693,38 +693,42 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     with an int ``kv_len`` a chunk of a prompt goes through a temporary fp16 copy
     of the rows (256 bytes of K and V each per row) and the tensor-memory
     attention kernels."""
-    cache = (k_codes, k_scales, v_codes, v_scales)
-    B, Hkv, cap, D, group = _cache_q4("attention_cache_q4", *cache)
-    if torch.cuda.current_device() != k_codes.get_device():  # plans and workspaces are per device
-        with torch.cuda.device(k_codes.device):
-            return attention_cache_q4(q, *cache, kv_len, scale, causal, max_kv_len)
-    q = _same_device(_require(q, "attention_cache_q4.q"), "attention_cache_q4.q", k_codes.device)
-    if q.data_ptr() % 16:
+    B, Hkv, cap, D, group = _cache_q4("attention_cache_q4", k_codes, k_scales, v_codes, v_scales)
+    dev = k_codes.device
+    if torch.cuda.current_device() != dev.index:  # plans and workspaces are per device
+        with torch.cuda.device(dev):
+            return attention_cache_q4(q, k_codes, k_scales, v_codes, v_scales, kv_len, scale, causal,
+                                      max_kv_len)
+    q = _same_device(_require(q, "attention_cache_q4.q"), "attention_cache_q4.q", dev)
+    at = q.data_ptr()
+    if at & 15:
         q = q.clone()
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[1] % Hkv:
-        raise RuntimeError(f"attention_cache_q4: q {tuple(q.shape)} for a cache of {(B, Hkv, cap, D)}")
-    Hq, Sq = q.shape[1], q.shape[2]
+        at = q.data_ptr()
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[1] % Hkv:
+        raise RuntimeError(f"attention_cache_q4: q {tuple(shape)} for a cache of {(B, Hkv, cap, D)}")
+    Hq, Sq = shape[1], shape[2]
     lens = None
     if isinstance(kv_len, torch.Tensor):
-        lens = _per_sequence(kv_len, "attention_cache_q4.kv_len", B, q.device)
+        lens = _per_sequence(kv_len, "attention_cache_q4.kv_len", B, dev)
         n = cap if max_kv_len is None else int(max_kv_len)
     else:
         n = int(kv_len)
     if n < 0 or n > cap:
         raise RuntimeError(f"attention_cache_q4: {n} rows exceed the capacity {cap}")
-    out = torch.empty(B, Sq, Hq * D, device=q.device, dtype=q.dtype)
+    out = torch.empty(B, Sq, Hq * D, device=dev, dtype=_BF16)
     if lens is None and _q4_chunk(B, Hq, Hkv, Sq, n, D):
         w = _lib.query("q35_attn_q4_chunk_workspace", B, Hq, Hkv, Sq, n, D)
-        ws = torch.empty(max(w, 16), device=q.device, dtype=torch.uint8)
-        _call_on(q.device, "q35_attn_q4_chunk_fwd", q.data_ptr(), *[t.data_ptr() for t in cache],
-                 out.data_ptr(), B, Hq, Hkv, Sq, n, cap, D, group, float(scale), 1 if causal else 0,
-                 ws.data_ptr(), _stream(q))
+        ws = torch.empty(max(w, 16), device=dev, dtype=torch.uint8)
+        _lib.call("q35_attn_q4_chunk_fwd", at, k_codes.data_ptr(), k_scales.data_ptr(),
+                  v_codes.data_ptr(), v_scales.data_ptr(), out.data_ptr(), B, Hq, Hkv, Sq, n, cap, D,
+                  group, float(scale), 1 if causal else 0, ws.data_ptr(), _stream(q))
     else:
         w = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, n, D)
-        ws = torch.empty(w, device=q.device, dtype=torch.float32) if w > 0 else None
-        _call_on(q.device, "q35_attn_q4_fwd", q.data_ptr(), *[t.data_ptr() for t in cache],
-                 out.data_ptr(), B, Hq, Hkv, Sq, n, _ptr(lens), cap, D, group, float(scale),
-                 1 if causal else 0, _ptr(ws), _stream(q))
+        ws = torch.empty(w, device=dev, dtype=torch.float32) if w > 0 else None
+        _lib.call("q35_attn_q4_fwd", at, k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                  v_scales.data_ptr(), out.data_ptr(), B, Hq, Hkv, Sq, n, _ptr(lens), cap, D, group,
+                  float(scale), 1 if causal else 0, _ptr(ws), _stream(q))
     return out
 
 
