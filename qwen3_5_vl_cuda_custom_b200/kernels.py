@@ -613,7 +613,9 @@ def _strided_rows(t: torch.Tensor, name: str, device) -> torch.Tensor:
     if (t.dtype != _BF16 or t.device != device or st[3] != 1 or (st[0] | st[1] | st[2]) & 7
             or t.data_ptr() & 15):
         t = _same_device(_require(t, name), name, device)
-        t = t.clone() if t.data_ptr() & 15 else t
+        st = t.stride()
+        if t.data_ptr() & 15 or (st[0] | st[1] | st[2]) & 7:  # (strides of one-element axes)
+            t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 

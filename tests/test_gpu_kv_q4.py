@@ -179,6 +179,18 @@ def test_append_takes_strided_rows_and_per_sequence_offsets():
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+def test_append_takes_any_stride_of_an_axis_of_one_element():
+    base = rows((1, 1, 1, 1200), 7).to(DEV).view(-1)
+    for shape, strides in (((1, 4, 1, 128), (515, 128, 3, 1)), ((2, 1, 1, 128), (512, 5, 7, 1)),
+                           ((1, 1, 4, 128), (1, 9, 136, 1))):
+        k = base.as_strided(shape, strides)
+        B, Hkv, S, D = shape
+        cache = empty_cache(B, Hkv, 16, D, 32)
+        K().kv_append_q4(k, k, *cache, 2)
+        for i in (0, 2):
+            check_stored(cache[i][:, :, 2:2 + S], cache[i + 1][:, :, 2:2 + S], k.cpu(), 32)
+
+
 def test_rows_outside_the_cache_are_left_out_and_reported():
     B, Hkv, S, D, cap = 3, 2, 4, 64, 16
     k = rows((B, Hkv, S, D), 7).to(DEV)
