@@ -501,7 +501,8 @@ Q35_API int q35_kv_read_q4(const void *k_codes, const void *k_scales, const void
  * <= s + len - Sq.  A query that sees no key gives zeros.  A kv_lens entry
  * outside [0, kv_len] is clamped and recorded as a device error (code 2, site
  * 311).  Exact in its scaling for |q| < 2^75 and |v| between 2^-60 and 2^58 (beyond:
- * infinite, or rounded to 0).  workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.      */
+ * infinite, or rounded to 0).  A row that reads back as NaN reaches the queries that
+ * see it only.  workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.     */
 Q35_API int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D);
 Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_scales,
@@ -513,8 +514,9 @@ Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_sc
 /* The same for many query rows per kv head (a chunk of a prompt), all sequences of
  * kv_len >= 1 rows: the rows go through scaled fp16 copies in the workspace
  * (q35_attn_q4_chunk_workspace(...) bytes, 16-byte aligned) and the tensor-memory
- * attention kernels.  B * Hq <= 65535.  A key or value that is not finite may reach
- * all rows that share its 128-key tile, as in q35_attn_prefill_cache_fwd.     */
+ * attention kernels.  B * Hq <= 65535.  Per kv head, the largest |q| times the
+ * largest |k| must stay below 2^30; values, and the keys against the queries, lose
+ * bits once they are 2^-27 of the largest of their head's rows, hidden ones included. */
 Q35_API int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D); /* 1: estimated faster than q35_attn_q4_fwd */
 Q35_API int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64_t Sq,

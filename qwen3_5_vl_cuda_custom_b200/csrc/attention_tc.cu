@@ -118,6 +118,15 @@ __device__ __forceinline__ uint32_t pack_p(float a, float b) {
     return pack_bf2(a, b);
   }
 }
+// A row's maximum is raised (and O rescaled) once it is exceeded by kSlack, in log2.
+// fp16 keeps 11 bits down to 2^-14 only, so its weights are lifted by 2^kLift: they
+// round by 2^-12 down to 2^-25 of the largest, by 2^-36 of it below (131072 such keys:
+// 2^-19 in all).  512 queries behind 8192 keys: 100.7 us; 99.1 with 8 and 7 (2^-15 in
+// all), 102.2 with 1 and 14.
+template <bool kF16>
+constexpr float kSlack = kF16 ? 4.f : 8.f;
+template <bool kF16>
+constexpr float kLift = kF16 ? 11.f : 0.f;
 // The key tiles [j0, j0 + n) of this CTA's split.
 __device__ __forceinline__ int split_tiles(const AttnParams &p, int split, int n_all, int &j0) {
   j0 = split * p.x.tiles_per_split;
@@ -125,15 +134,20 @@ __device__ __forceinline__ int split_tiles(const AttnParams &p, int split, int n
 }
 // kF16 epilogue of one query row: D columns of O (read 32 at a time from TMEM by the
 // whole warp) as bf16, or as an fp32 partial with its (max in log2 units, sum).
+// (Values stored as NaN are zeros among the operands: the blocks of 32 channels in
+// which the row sees one get their NaN here.)
 __device__ __forceinline__ void store_row_f16(const AttnParams &p, uint32_t o_tm, bool some,
                                               bool valid, int b, int h, int64_t qi, int split,
                                               float m_log2, float l, float f) {
   const int64_t rows = p.x.rows;
+  const int64_t last = p.causal ? min(qi + p.Skv - p.Sq, p.Skv - 1) : p.Skv - 1;
+  const int *v_nan = p.x.v_nan + (static_cast<int64_t>(b) * p.Hkv + h / (p.Hq / p.Hkv)) * 4;
   const int64_t row = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq + qi;
   const int64_t slot = row * p.x.splits + split;
-  const float inv = p.x.part ? f : (l > 0.f ? f / l : 0.f);
+  const float all = p.x.part ? f : (l > 0.f ? f / l : 0.f);
 #pragma unroll 1
   for (int c = 0; c < p.x.D / 32; ++c) {
+    const float inv = v_nan[c] <= last ? NAN : all;
     uint32_t r[32];
     if (some) {
       sm100::tmem_ld32(o_tm + c * 32, r);
@@ -343,14 +357,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * p.sl2 > 8.f) {
+      } else if ((m_new - m_used) * p.sl2 > kSlack<kF16>) {
         need = true;
         alpha = exp2f((m_used - m_new) * p.sl2);
         m_used = m_new;
         l *= alpha;
       }
       const float mu = (m_used == -INFINITY) ? 0.f : m_used;
-      const float mus = mu * p.sl2;
+      const float mus = mu * p.sl2 - kLift<kF16>;
       // O may only be touched once PV_{j-1} has finished.
       if (j >= 1 && !sm100::mbar_wait(o_done, (j - 1) & 1)) {
         report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 307, j, row);
@@ -693,13 +707,13 @@ __global__ void __launch_bounds__(kThreads2, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * p.sl2 > 8.f) {
+      } else if ((m_new - m_used) * p.sl2 > kSlack<kF16>) {
         need = true;
         alpha = exp2f((m_used - m_new) * p.sl2);
         m_used = m_new;
         l *= alpha;
       }
-      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * p.sl2;
+      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * p.sl2 - kLift<kF16>;
       // exponentials, bf16 P over the first 64 S columns.  Score pairs are
       // scaled with one f32x2 FMA; pairs alternate between the MUFU unit
       // (ex2.approx) and the paired FMA polynomial; row sums in f32x2.

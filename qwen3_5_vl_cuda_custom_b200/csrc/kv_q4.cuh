@@ -8,11 +8,10 @@
 //
 // Why this order: a matrix instruction wants its operands as pairs of
 // neighbouring values along the summed axis.  With channel 2i in field i and
-// channel 2i + 1 in field i + 4, `(w >> 4i) & 0x000f000f` is the pair
-// (2i, 2i + 1), and OR-ing 0x43004300 makes it the bf16 pair (128 + c, 128 + c')
-// exactly: one shift and one logic operation per two codes.  The words of a
-// thread quarter t are contiguous, so the four threads that share a key read
-// 16 bytes each (D = 128).
+// channel 2i + 1 in field i + 4, `w & 0x000f000f` and `w & 0x00f000f0` (and the same
+// of w >> 8) are such pairs, c * 2^-133 and c * 2^-129 as they stand: bf16's smallest
+// numbers are evenly spaced.  The words of a thread quarter t are contiguous, so the
+// four threads that share a key read 16 bytes each (D = 128).
 #pragma once
 
 #include "common.cuh"

@@ -423,6 +423,53 @@ def test_a_nonfinite_value_reaches_only_the_rows_that_see_it(D, group):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("D,group,Sq,kv,causal", [(128, 32, 40, 300, True), (128, 128, 130, 130, True),
+                                                  (64, 32, 33, 2000, True), (32, 32, 20, 90, False)])
+def test_a_nonfinite_row_in_a_chunk_reaches_only_the_rows_that_see_it(monkeypatch, D, group, Sq, kv, causal):
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: True)
+    B, Hq, Hkv = 2, 4, 2
+    cache, _, vv = filled_cache(B, Hkv, -(-kv // 16) * 16, D, group, 69)
+    q = rows((B, Hq, Sq, D), 70).to(DEV)
+    want = K().attention_cache_q4(q, *cache, kv, 0.125, causal).view(B, Sq, Hkv, 2, D // group, group)
+    v, k = kv - Sq + 7, kv - Sq + 11  # seen from query 7 on, and from 11 on
+    cache[3][1, 0, v, 0] = math.nan
+    cache[3][1, 0, kv - 1, 0] = math.nan
+    cache[1][0, 1, k, D // group - 1] = math.nan
+    got = K().attention_cache_q4(q, *cache, kv, 0.125, causal).view(B, Sq, Hkv, 2, D // group, group)
+    for hit, back in ((got[1, 7 if causal else 0:, 0, :, 0], want[1, 7 if causal else 0:, 0, :, 0]),
+                      (got[0, 11 if causal else 0:, 1], want[0, 11 if causal else 0:, 1])):
+        assert hit.isnan().all()
+        hit.copy_(back)
+    # Without the NaN rows the scales of the operands may be other powers of two.  That
+    # moves only numbers below 2^-14 of them, by 2^-25: values by 2^-38 of the largest,
+    # scores by less than 2^-17; then an output may round to the next bf16 (2^-7).
+    tol = 2 ** -7 * want.double().abs() + 2 ** -16 * float(vv.abs().max())
+    assert ((got.double() - want.double()).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("log2", [-12.0, -20.0, -24.5])
+def test_many_small_weights_beside_a_large_one(monkeypatch, chunk, log2):
+    """60000 keys of weight 2^log2 beside one of weight 1 whose value is 0.  Keys and
+    queries are exact in bf16 and fp16, so scores are off by fp32's sums and the
+    chunk's exponential alone (d = 2^-13); weights and values round to 2^-8 each, in a
+    chunk to 2^-11 (weights 2^-25 of the largest and above)."""
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: chunk)
+    B, Hq, Hkv, Sq, kv, D, group = 1, 2, 1, 2, 60000, 128, 32
+    cache, _, _ = filled_cache(B, Hkv, kv, D, group, 91, 0.5)
+    codes = [t.clone() for t in cache]
+    codes[0].zero_()                      # keys: s = 0, m = -1 everywhere, 0 in row 7
+    codes[1][..., 0], codes[1][..., 1] = 0, -1
+    codes[1][:, :, 7, :, 1] = 0
+    codes[3][:, :, 7] = 0
+    q = torch.full((B, Hq, Sq, D), -log2 * math.log(2) / D).bfloat16()
+    kk, vv = R.values(codes[0], codes[1]), R.values(codes[2], codes[3])
+    out = K().attention_cache_q4(q.to(DEV), *codes, kv, 1.0, False).double().cpu()
+    ref, A = R.attention(q, kk, vv, [kv], 1.0, False)
+    tol = A * (2 ** (-10 if chunk else -7) + math.expm1(2 ** -12)) + 2 ** -8 * ref.abs()
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
 def test_large_scores_and_equal_scores():
     """Scores of thousands (one key takes all) and a row of equal scores."""
     B, Hq, Hkv, D, kv = 1, 4, 1, 128, 300
