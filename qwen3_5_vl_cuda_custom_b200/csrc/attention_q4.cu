@@ -10,10 +10,10 @@
 // HBM delivers about 24 bytes = 48 codes against 128 lanes of issue, 64 of them
 // for logic operations.
 //
-// Codes as bf16.  The bits c << 4 (c = 0..15) read as bf16 are c * 2^-129 and the
-// bits c are c * 2^-133: bf16's subnormals and its first binade are evenly
-// spaced.  The matrix units and fma.bf16x2 take subnormals at full precision, so
-// `w & 0x000f000f` and `w & 0x00f000f0` are pairs of codes as they stand, without
+// Codes as they stand.  The bits c << 4 (c = 0..15) read as bf16 are c * 2^-129 and the
+// bits c are c * 2^-133, as fp16 c * 2^-20 and c * 2^-24: the subnormals and the first
+// binade are evenly spaced.  The matrix units and fma.f16x2 take subnormals at full
+// precision, so `w & 0x000f000f` and `w & 0x00f000f0` are pairs of codes, without
 // a conversion or an offset to take out again; one shift by 8 gives the other
 // four codes of a word.  The powers of two go into the other operand.
 //
@@ -27,10 +27,21 @@
 // Keys are the 16 rows of the instruction and queries its 8 columns (S^T = K Q^T,
 // O^T = V^T P^T): a decode step has G = Hq/Hkv queries per kv head, often 8, and
 // no half of the tile is idle.  P moves from accumulator to operand layout by an
-// 8x8 transpose between the lanes (movmatrix).  P is rounded to bf16 (as in the
-// bf16 attention kernels), V is dequantised to bf16 in registers, one rounding of
-// m + s c: what a read back gives, as (2^-129 c) (2^69 s) + 2^-60 m, or 2^-64 of the
-// value for codes at bit 0 (exact scales: |V| between 2^-60 and 2^58).
+// 8x8 transpose between the lanes (movmatrix).
+//
+// Values.  P and V go into their product as fp16, of 11 bits: rounded to bf16 each
+// would cost as much as the output's own rounding (relative error of normal data
+// 0.0022 to 0.0026; 0.0016 like this, which is the output's rounding alone).  For the
+// range that bf16 has and fp16 has not, every key has a power of two F: V 2^-F enters,
+// dequantised in registers as (2^-24 c) (2^(24-F) s) + 2^-F m (16 times that for the
+// codes at bit 4), and the key's weight is 2^F p, by an F added to its score.  So the
+// running maximum is that of what the keys contribute, a key with a large V and a small
+// weight costs the others nothing, nor does a masked one; the sum of weights takes
+// 2^-F out again.  F is the least one at which 2^(24-F) s < 2^16 and 2^(4-F) |m| < 2^15
+// for all groups of the key, so V is off by at most 2^-11 of itself or 2^-15 of the
+// largest s of its key (a code step is s).  Weights reach 2^15 (kLift), so they have
+// all 11 bits down to 2^-29 of the largest.
+// Visible values: |V| between 2^-60 and 2^100.
 //
 // V's operand wants pairs of neighbouring keys.  A transposing ldmatrix over the
 // codes as 16-bit units (four codes) gives exactly that: a lane receives, for two
@@ -51,14 +62,16 @@
 // are XOR-swizzled by the row, so that both the 16-byte reads of K and the 8-row
 // reads of V touch every bank once.
 //
-// Measured (32/4 heads x 128, groups of 32): 64 sequences x 8193 keys 64 us, 5.3 TB/s
-// (the copies alone 61, the arithmetic alone 57; a plain copy moves 6.5 TB/s); one
-// sequence x 131072 keys 21 us; x 500 keys 6.3 us.  563 warp instructions per 32-key
-// tile, issue slots 60 % busy: what bounds it is the two together, the 16x8 matrix
-// instructions (one per 2 clocks and SM) holding up the logic operations beside them.
-// Tried: e4m3 operands for K (emulated: 48M instructions for 37M, 84 us), shifts as
-// multiplications (72), a tile's scores together with the products of the tile before
-// (75), bulk copies instead of 16-byte ones (82 with an earlier inner loop).
+// Measured (32/4 heads x 128, groups of 32): 64 sequences x 8193 keys 68.7 us, 4.9 TB/s
+// (the copies alone 61; a plain copy moves 6.5 TB/s); one sequence x 131072 keys 22.5 us;
+// x 500 keys 6.6 us.  610 warp instructions per 32-key tile, issue slots 60 % busy: what
+// bounds it is copies and arithmetic together, the 16x8 matrix instructions (one per 2
+// clocks and SM) holding up the logic operations beside them.
+// Tried: P and V in bf16 (64.0 us, the errors above), P as two bf16 parts (70.8, 0.0021
+// to 0.0023); e4m3 operands for K (emulated: 48M instructions for 37M), shifts as
+// multiplications (12 % slower), a tile's scores together with the products of the tile
+// before (17 %), bulk copies instead of 16-byte ones.
+#include <cuda_fp16.h>
 #include <float.h>
 
 #include <type_traits>
@@ -77,6 +90,8 @@ constexpr int kTile = 32;  // keys per tile
 // allow 3 CTAs; 4 of 128 registers (spills) measured 70.5 us against 68.0 at 64 x
 // 8193 keys, 3 tiles in flight 68.6.
 constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr float kLift = 15.f;   // weights reach 2^kLift
+constexpr int kMinF = -60;      // smallest F of a key
 constexpr int stages(int d, int nt) { return d == 128 && nt == 1 ? 2 : 4; }
 
 struct Params {
@@ -104,7 +119,8 @@ struct Layout {
   static constexpr int kStage = 2 * (kCodes + kScales);
   static constexpr int kRing = kStages * kStage;
   static constexpr int kRegs = NT * (D / 4 + 4);  // a lane's O, m, l
-  static constexpr int kSmem = kWarps * kRing + (kWarps - 1) * kRegs * 128;
+  static constexpr int kKeys = kTile * 8;         // (F, 2^-F) of a tile's keys
+  static constexpr int kSmem = kWarps * (kRing + kKeys) + (kWarps - 1) * kRegs * 128;
 };
 
 // Workspace: [2 runs][8 NT rows][D] floats and [2 runs][8 NT rows] (m, l) of partials
@@ -180,7 +196,7 @@ template <int N>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// D = A(16x16 bf16) * B(16x8 bf16) + C, fp32.
+// D = A(16x16) * B(16x8) + C, fp32: bf16 operands, and fp16.
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                     uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1,
                                     float c2, float c3) {
@@ -188,6 +204,13 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -199,8 +222,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The codes of fields 0..3 and 4..7 of a word as bf16 pairs (field i, field i + 4):
-// c * 2^-133 for i = 0, 2 and c * 2^-129 for i = 1, 3.
+// The codes of fields 0..3 and 4..7 of a word as 16-bit pairs (field i, field i + 4):
+// as bf16 c * 2^-133 for i = 0, 2 and c * 2^-129 for i = 1, 3, as fp16 c * 2^-24 and
+// c * 2^-20.
 __device__ __forceinline__ void codes4(uint32_t w, uint32_t (&c)[4]) {
   const uint32_t h = w >> 8;
   c[0] = w & 0x000f000fu;
@@ -208,18 +232,27 @@ __device__ __forceinline__ void codes4(uint32_t w, uint32_t (&c)[4]) {
   c[2] = h & 0x000f000fu;
   c[3] = h & 0x00f000f0u;
 }
+// fp16 pairs; subnormals count.
 __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// Powers of two as bf16 bits.
-constexpr uint32_t pow2_bf16(int e) { return static_cast<uint32_t>(127 + e) << 7; }
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Larger magnitudes of bf16 pairs (the signs are of no use; a NaN gives way).
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
@@ -230,6 +263,16 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
   else
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+}
+template <int N>
+__device__ __forceinline__ void sts_words(uint32_t addr, const uint32_t (&w)[N]) {
+  if constexpr (N == 4)
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};"
+                 ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(w[0]), "r"(w[1]) : "memory");
+  else
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(w[0]) : "memory");
 }
 __device__ __forceinline__ uint32_t lds1(uint32_t addr) {
   uint32_t w[1];
@@ -297,7 +340,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   };
 
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * L::kRing;
-  float *merge = reinterpret_cast<float *>(smem + kWarps * L::kRing);
+  const uint32_t keys = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
+                        kWarps * L::kRing + warp * L::kKeys;
+  float *merge = reinterpret_cast<float *>(smem + kWarps * (L::kRing + L::kKeys));
 
   // ---- copies: this warp's tiles (tile 4 r + warp of round r of a group), ahead of
   // their use.  Lane i copies chunks i, i + 32, ... of the tile's codes (chunk c of row
@@ -372,8 +417,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
   const int vch = D == 32 ? 0 : lane >> 4;
   const int gv = (D == 128 ? g >> 1 : D == 64 ? (g >> 1) & 1 : 0) / BPG;  // the lane's V scale group
   const uint32_t vsoff = (2 * t * NS + gv) * 4;
-  constexpr uint32_t kUpS = pow2_bf16(69) * 0x10001u, kDownM0 = pow2_bf16(-64) * 0x10001u,
-                     kDownM1 = pow2_bf16(-60) * 0x10001u;
   const float scale_up = p.scale_log2 * 0x1p81f;
   uint32_t stage = 0;
 
@@ -456,8 +499,44 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
       const uint32_t sk = ring + stage;
       const uint32_t sks = sk + L::kCodes, sv = sks + L::kScales, svs = sv + L::kCodes;
 
-      // ---- S^T = K Q^T (two blocks of 16 keys), in units of log2
-      float s[2][NT][4];
+      const bool partial = key0 + kTile > lim_all;
+      if (partial) {
+        // A weight of 0 does not silence a NaN or an infinity in V: rows behind the
+        // length are cleared, and a non-finite group that some query must not see is
+        // cleared too and put into the outputs of the queries that do see it.
+        const bool behind = key0 + lane >= len;
+        uint32_t clear = behind ? (1u << NS) - 1u : 0u;  // groups of key row `lane`
+        if (!behind) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+            if (nonfinite(lds1(svs + (lane * NS + i) * 4))) clear |= 1u << i;
+        }
+        uint32_t todo = __ballot_sync(0xffffffffu, clear != 0 && !behind);
+        while (todo) {
+          const int kk = __ffs(todo) - 1;
+          todo &= todo - 1;
+          if (nonfinite(lds1(svs + (kk * NS + gv) * 4))) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (key0 + kk < lim[nt][e & 1]) o[i][nt][e] = NAN;
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          if (clear >> i & 1u)
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(svs + (lane * NS + i) * 4), "r"(0u) : "memory");
+        __syncwarp();
+      }
+      uint32_t vw[NS];  // V's scales and minima of key `lane`
+      lds_words<NS>(vw, svs + lane * (NS * 4));
+
+      // ---- S^T = K Q^T (two blocks of 16 keys) + F, in units of log2
+      float s[2][NT][4], unf[2][2];  // unf: 2^-F
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         uint32_t wl[J], wh[J], pl[NS], ph[NS];
@@ -500,13 +579,41 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
             }
           }
         }
+        if (mt == 0) {
+          // V's scales and minima as fp16, by a power of two 2^-F per key, and F for the
+          // key's weights
+          uint32_t top = vw[0];
+#pragma unroll
+          for (int i = 1; i < NS; ++i) top = max_abs2(top, vw[i]);
+          const int f = max(kMinF + 127, max(static_cast<int>(top >> 7 & 0xffu) + 9,
+                                             static_cast<int>(top >> 23 & 0xffu) - 10));
+          const float fs = __uint_as_float((278 - f) << 23), fm = fs * 0x1p-20f;  // 2^(24-F), 2^(4-F)
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+            vw[i] = pack_h2(__uint_as_float(vw[i] << 16) * fs,
+                            __uint_as_float(vw[i] & 0xffff0000u) * fm);
+          sts_words<NS>(svs + lane * (NS * 4), vw);
+          const uint32_t k2[2] = {
+              __float_as_uint(__uint_as_float(0x4b000000u | f) - (8388608.f + 127.f)),
+              __float_as_uint(fs * 0x1p-24f)};
+          sts_words<2>(keys + lane * 8, k2);
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t f0[2], f1[2];
+        lds_words<2>(f0, keys + (16 * mt + g) * 8);
+        lds_words<2>(f1, keys + (16 * mt + g + 8) * 8);
+        unf[mt][0] = __uint_as_float(f0[1]);
+        unf[mt][1] = __uint_as_float(f1[1]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][nt][e] *= scale_up;
+          for (int e = 0; e < 4; ++e)
+            s[mt][nt][e] = fmaf(s[mt][nt][e], scale_up, __uint_as_float(e < 2 ? f0[0] : f1[0]));
       }
-
-      if (key0 + kTile > lim_all) {
+      if (partial) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -514,36 +621,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (key0 + 16 * mt + g + 8 * (e >> 1) >= lim[nt][e & 1]) s[mt][nt][e] = -INFINITY;
-        // A weight of 0 does not silence a NaN or an infinity in V: rows behind the
-        // length are cleared, and a non-finite group that some query must not see is
-        // cleared too and put into the outputs of the queries that do see it.
-        const bool behind = key0 + lane >= len;
-        uint32_t clear = behind ? (1u << NS) - 1u : 0u;  // groups of key row `lane`
-        if (!behind) {
-#pragma unroll
-          for (int i = 0; i < NS; ++i)
-            if (nonfinite(lds1(svs + (lane * NS + i) * 4))) clear |= 1u << i;
-        }
-        uint32_t todo = __ballot_sync(0xffffffffu, clear != 0 && !behind);
-        while (todo) {
-          const int kk = __ffs(todo) - 1;
-          todo &= todo - 1;
-          if (nonfinite(lds1(svs + (kk * NS + gv) * 4))) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (key0 + kk < lim[nt][e & 1]) o[i][nt][e] = NAN;
-          }
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-          if (clear >> i & 1u)
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(svs + (lane * NS + i) * 4), "r"(0u) : "memory");
-        __syncwarp();
       }
 
       // ---- softmax: the maximum is raised (and O rescaled) only when some key exceeds it
@@ -573,15 +650,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
             o[i][nt][3] *= a1;
           }
         }
-        const float mu0 = row_m[nt][0], mu1 = row_m[nt][1];
+        const float mu0 = row_m[nt][0] - kLift, mu1 = row_m[nt][1] - kLift;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           const float p0 = exp2_fast(s[mt][nt][0] - mu0), p1 = exp2_fast(s[mt][nt][1] - mu1);
           const float p2 = exp2_fast(s[mt][nt][2] - mu0), p3 = exp2_fast(s[mt][nt][3] - mu1);
-          row_l[nt][0] += p0 + p2;
-          row_l[nt][1] += p1 + p3;
-          pb[mt][nt][0] = transpose8x8(pack_bf2(p0, p1));
-          pb[mt][nt][1] = transpose8x8(pack_bf2(p2, p3));
+          row_l[nt][0] = fmaf(p2, unf[mt][1], fmaf(p0, unf[mt][0], row_l[nt][0]));
+          row_l[nt][1] = fmaf(p3, unf[mt][1], fmaf(p1, unf[mt][0], row_l[nt][1]));
+          pb[mt][nt][0] = transpose8x8(pack_h2(p0, p1));
+          pb[mt][nt][1] = transpose8x8(pack_h2(p2, p3));
         }
       }
 
@@ -590,16 +667,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
       if constexpr (D == 32) ldsm4_t(u, sv + vrow * RB);  // keys 0-7, 8-15, 16-23, 24-31
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        // scale pairs of keys (2t, 2t + 1) and (2t + 8, 2t + 9), with their powers of two
+        // scale pairs of keys (2t, 2t + 1) and (2t + 8, 2t + 9); minima for even and odd fields
         uint32_t s2[2], m2[2][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t at0 = svs + vsoff + (16 * mt + 8 * h) * (NS * 4);
           const uint32_t pa = lds1(at0), pc = lds1(at0 + NS * 4);
-          s2[h] = mul2(__byte_perm(pa, pc, 0x5410), kUpS);
-          const uint32_t mm = __byte_perm(pa, pc, 0x7632);
-          m2[h][0] = mul2(mm, kDownM0);
-          m2[h][1] = mul2(mm, kDownM1);
+          s2[h] = __byte_perm(pa, pc, 0x5410);
+          m2[h][1] = __byte_perm(pa, pc, 0x7632);
+          m2[h][0] = mul2(m2[h][1], 0x2c002c00u);  // 2^-4
         }
         auto product = [&](int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int i) {
           a0 = fma2(a0, s2[0], m2[0][i]);
@@ -609,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float(&acc)[4] = o[tile][nt];
-            mma(acc, a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1], acc[0], acc[1], acc[2], acc[3]);
+            mma_f16(acc, a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
           }
         };
         if constexpr (D == 32) {
@@ -647,7 +723,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Para
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][nt][e] *= i % 2 == 0 ? 0x1p64f : 0x1p60f;
+        for (int e = 0; e < 4; ++e) o[i][nt][e] *= i % 2 == 0 ? 0x1p-15f : 0x1p-19f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      row_l[nt][0] *= 0x1p-15f;
+      row_l[nt][1] *= 0x1p-15f;
+    }
     __syncthreads();
     if (warp > 0) {
       float *dst = merge + (warp - 1) * (L::kRegs * 32) + lane;

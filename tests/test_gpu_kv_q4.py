@@ -277,6 +277,49 @@ def test_attention_on_the_codes(D, group, Hq, Hkv, Sq, kv, causal):
     check_attention(out, q, kk, vv, [kv] * B, D ** -0.5, causal, group)
 
 
+@pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("Hq,Hkv,Sq,kv,causal", [(1, 1, 1, 7, False), (8, 1, 1, 300, False),
+                                                 (14, 2, 3, 1000, True), (4, 4, 1, 4000, False)])
+def test_attention_on_the_codes_keeps_11_bits(D, group, Hq, Hkv, Sq, kv, causal):
+    """With A = sum p |v|: weights and values each rounded by 2^-11, values at most by
+    2^-15 of the largest scale; scores off by d (check_attention), exp2 by 2^-21; the
+    output rounded to bf16."""
+    B = 2
+    cache, kk, vv = filled_cache(B, Hkv, -(-kv // 16) * 16, D, group, 83, 0.5)
+    q = rows((B, Hq, Sq, D), 84, 0.5)
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, causal).double().cpu()
+    ref, A = R.attention(q, kk, vv, [kv] * B, D ** -0.5, causal)
+    qa, ka = q.double().abs().amax(dim=(0, 1, 2)), kk.abs().amax(dim=(0, 1, 2))
+    groups = ka.view(-1, group).amax(-1).repeat_interleave(group)
+    d = 2.0 ** -19 * D ** -0.5 * float((qa * groups).sum()) * (128 * 2 / 15 + 1)
+    tol = (A * (2 ** -10 + math.expm1(2 * d + 2.0 ** -20)) + 2 ** -8 * ref.abs()
+           + 2 ** -15 * float(cache[3][..., 0].max()))
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+@pytest.mark.parametrize("D,group", SHAPES)
+def test_far_larger_values_cost_the_others_nothing(D, group):
+    """Rows a query does not see, whatever finite values they hold, change nothing; a
+    visible row of huge values and no weight adds what it weighs and nothing else."""
+    B, Hq, Hkv, kv, Sq = 1, 4, 2, 150, 4
+    cache, kk, vv = filled_cache(B, Hkv, 160, D, group, 85)
+    q = rows((B, Hq, Sq, D), 86, 0.3)
+    want = K().attention_cache_q4(q.to(DEV), *cache, kv, 0.125, True)
+    other = [t.clone() for t in cache]
+    for s, m in ((0.0, 3e38), (2e37, -3e38), (4e37, -3e38), (1e-38, 1e-38)):
+        other[1][:, :, kv - 3:kv, :, 0], other[1][:, :, kv - 3:kv, :, 1] = s, m
+        other[3][:, :, kv - 3:kv, :, 0], other[3][:, :, kv - 3:kv, :, 1] = s, m
+        got = K().attention_cache_q4(q.to(DEV), *other, kv, 0.125, True)
+        assert torch.equal(got[:, :1], want[:, :1])
+    q[:, :, :, 0] = 40.0  # row 9: a score of -40 * 64 * 0.125 below the rest, values of 1e5
+    cache[1][:, :, 9], cache[0][:, :, 9] = 0, 0
+    cache[1][:, :, 9, 0, 1] = -64
+    cache[3][:, :, 9, :, 0], cache[3][:, :, 9, :, 1] = 1e4, -1e5
+    kk, vv = R.values(cache[0], cache[1]), R.values(cache[2], cache[3])
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, 0.125, True)
+    check_attention(out, q, kk, vv, [kv], 0.125, True, group)
+
+
 @pytest.mark.parametrize("D,group", [(128, 32), (64, 64)])
 def test_attention_long_and_split(D, group):
     B, Hq, Hkv, kv = 1, 8, 2, 9001
