@@ -908,15 +908,19 @@ struct Plan {
   int nt, n_rg, runs, per;
   bool scan, join;
 };
-// When to cut groups: a round at D = 128 takes about 0.72 us while every CTA has an SM
-// to itself and 1.4 once some SMs hold two or three; the second kernel adds 3.8 us and
-// 0.011 us per query row, 1.7 more when lengths on the device cut the runs.  In tenths
-// of a lone round (8 sequences x 4 kv heads: 512 keys whole 6.3, cut 6.5 us; 1024 keys
-// 9.2 and 7.9; 256 sequences: 1024 keys 43 and 47, 4096 keys 139 and 122).
+// When to cut groups: a round at D = 128 takes about 0.8 us while every CTA has an SM
+// to itself and 1.6 once some SMs hold two or three; the second kernel adds 2.2 us and
+// 0.025 us per query row, 1.3 more when lengths on the device cut the runs.  That, in
+// tenths of a lone round, fits both forms' times at 96 shapes (head_dim 64 and 128, 1 to
+// 256 sequences, 128 to 4096 keys; 0.5 % above the better one on average).  Another 1.8
+// us is counted because the second launch and its workspace cost the host 4 us, which a
+// short call waits for outside a graph (on the device it costs 1 % on average).
+// 8 sequences x 4 kv heads: 512 keys whole 6.7, cut 7.1 us; 1024 keys 10.0 and 8.4; 256
+// sequences: 1024 keys 46 and 49, 4096 keys 151 and 131.
 int round_cost(int64_t ctas, int D) {
-  return (ctas <= num_sms() ? 10 : 20) * (D + 128) / 256;
+  return (ctas <= num_sms() ? 10 : 20) * (D + 192) / 320;
 }
-int64_t join_cost(int64_t rows, bool lens) { return 53 + rows / 64 + (lens ? 24 : 0); }
+int64_t join_cost(int64_t rows, bool lens) { return 50 + rows / 32 + (lens ? 16 : 0); }
 int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, int D, bool lens) {
   pl.nt = R > 8 ? 2 : 1;
   const int64_t n_rg = (R + 8 * pl.nt - 1) / (8 * pl.nt);

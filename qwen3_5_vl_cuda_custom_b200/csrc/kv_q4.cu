@@ -15,10 +15,10 @@
 // word may cost: hence paired fp32 arithmetic, one shuffle a step for minimum and
 // maximum together, and a multiplication for each division by S or Hkv.
 //
-// Measured (4 kv heads x 128): 8 x 8192 rows appended in 46.5 us, 3.7 TB/s (bound by
-// its 290 instructions per warp and 512 channels: ties and their tests are a fifth),
-// 4096 rows 4.5 us, 64 sequences x 1 row 2.0 us; 16 x 8192 rows read in 58.5 us,
-// 6.0 TB/s.
+// Measured (4 kv heads x 128): 8 x 8192 rows appended in 44.0 us, 3.9 TB/s (240
+// instructions per warp and 512 channels, a quarter of them paired fp32 at half rate;
+// issue slots 65 % busy), 4096 rows 4.1 us, 64 sequences x 1 row 1.9 us; 16 x 8192 rows
+// read in 58.7 us, 6.0 TB/s.
 #include <type_traits>
 
 #include "kv_q4.cuh"
@@ -30,7 +30,7 @@ using q4::Cache;
 
 constexpr int kThreads = 256;
 // A CTA prefetches its next rows while it quantises: 7 CTAs of 128 threads per SM hold
-// in registers (8 x 8192 rows: 4 CTAs 50.0 us, 7 46.5, 10 with spills 58.8).
+// in registers (8 x 8192 rows: 4 CTAs 46.7 us, 6 44.5, 7 43.9, 8 45.7, 10 49.0).
 constexpr int kAppendThreads = 128, kAppendCtas = 7;
 
 struct Rows {
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) kv_append_q4_kern
 
 // Rows [start, start + n) as bf16 [B, Hkv, out_cap, D]; rows n .. out_cap are zeros.
 // kWords code words per thread: 4 when that still gives every SM eight CTAs (16 x 8192
-// rows: 58.3 us, 92 % of the copy rate; 63.7 with 2), else 2 (4096 rows: 3.4, not 3.7).
+// rows: 58.7 us, 92 % of the copy rate; 63.7 with 2), else 2 (4096 rows: 3.4, not 3.7).
 template <int D, int GROUP, int kWords>
 __global__ void __launch_bounds__(kThreads) kv_read_q4_kernel(
     Cache c, uint16_t *__restrict__ k, uint16_t *__restrict__ v, uint32_t rows, Divisor by_out,

@@ -604,19 +604,21 @@ def _same_device(t: torch.Tensor, name: str, device) -> torch.Tensor:
     return t
 
 
-def _strided_rows(t: torch.Tensor, name: str, device) -> torch.Tensor:
-    """t [B, Hkv, S, D] as the append kernel can address it: contiguous channels,
-    16-byte aligned rows (a transposed view of a token-major tensor needs no copy)."""
+def _strided_rows(t: torch.Tensor, name: str, device) -> tuple[torch.Tensor, tuple]:
+    """t [B, Hkv, S, D] as the append kernel can address it, and its strides: contiguous
+    channels, 16-byte aligned rows (a transposed view of a token-major tensor needs no
+    copy)."""
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
         raise TypeError(f"{name}: expected a 4-D tensor")
     st = t.stride()
-    if (t.dtype != _BF16 or t.device != device or st[3] != 1 or (st[0] | st[1] | st[2]) & 7
+    if (t.dtype is not _BF16 or t.device != device or st[3] != 1 or (st[0] | st[1] | st[2]) & 7
             or t.data_ptr() & 15):
         t = _same_device(_require(t, name), name, device)
         st = t.stride()
         if t.data_ptr() & 15 or (st[0] | st[1] | st[2]) & 7:  # (strides of one-element axes)
             t = t.clone(memory_format=torch.contiguous_format)
-    return t
+            st = t.stride()
+    return t, st
 
 
 def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
@@ -633,7 +635,8 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
     out and recorded as a device error.  k and v may be strided views."""
     B, Hkv, cap, D, group = _cache_q4("kv_append_q4", k_codes, k_scales, v_codes, v_scales)
     dev = k_codes.device
-    k, v = _strided_rows(k, "kv_append_q4.k", dev), _strided_rows(v, "kv_append_q4.v", dev)
+    k, ks = _strided_rows(k, "kv_append_q4.k", dev)
+    v, vs = _strided_rows(v, "kv_append_q4.v", dev)
     shape = k.shape
     S = shape[2]
     if shape != v.shape or shape != (B, Hkv, S, D):
@@ -643,22 +646,11 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
         rows, first = _per_sequence(offset, "kv_append_q4.offset", B, dev).data_ptr(), 0
     else:
         rows, first = None, int(offset)
-    ks, vs = k.stride(), v.stride()
     k_strides = _lib.strides_arg(ks)
     _call_on(dev, "q35_kv_append_q4", k.data_ptr(), v.data_ptr(), k_strides,
              k_strides if ks == vs else _lib.strides_arg(vs), k_codes.data_ptr(), k_scales.data_ptr(),
              v_codes.data_ptr(), v_scales.data_ptr(), B, Hkv, S, D, group, cap, first, rows,
              _stream(k_codes))
-
-
-def _read_q4(cache, shape, start: int, starts, n: int, out_cap: int):
-    B, Hkv, cap, D, group = shape
-    dev = cache[0].device
-    k = torch.empty(B, Hkv, out_cap, D, device=dev, dtype=_BF16)
-    v = torch.empty_like(k)
-    _call_on(dev, "q35_kv_read_q4", *[t.data_ptr() for t in cache], k.data_ptr(), v.data_ptr(), B, Hkv,
-             n, out_cap, D, group, cap, start, _ptr(starts), _stream(cache[0]))
-    return k, v
 
 
 def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
@@ -667,11 +659,18 @@ def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Ten
     (B,Hkv,length,D), each value rounded once.  ``start`` is an int or an int32
     (B,) device tensor; a row outside the cache reads as zero and is recorded as
     a device error."""
-    cache = (k_codes, k_scales, v_codes, v_scales)
-    shape = _cache_q4("kv_read_q4", *cache)
-    starts = (_per_sequence(start, "kv_read_q4.start", shape[0], k_codes.device)
-              if isinstance(start, torch.Tensor) else None)
-    return _read_q4(cache, shape, 0 if starts is not None else int(start), starts, int(length), int(length))
+    B, Hkv, cap, D, group = _cache_q4("kv_read_q4", k_codes, k_scales, v_codes, v_scales)
+    dev, n = k_codes.device, int(length)
+    if isinstance(start, torch.Tensor):
+        starts, first = _per_sequence(start, "kv_read_q4.start", B, dev).data_ptr(), 0
+    else:
+        starts, first = None, int(start)
+    k = torch.empty(B, Hkv, n, D, device=dev, dtype=_BF16)
+    v = torch.empty_like(k)
+    _call_on(dev, "q35_kv_read_q4", k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+             v_scales.data_ptr(), k.data_ptr(), v.data_ptr(), B, Hkv, n, n, D, group, cap, first, starts,
+             _stream(k_codes))
+    return k, v
 
 
 def _q4_chunk(B: int, Hq: int, Hkv: int, Sq: int, kv_len: int, D: int) -> bool:
