@@ -86,10 +86,11 @@ using q4::Cache;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;  // keys per tile
-// CTAs per SM, and tiles in flight per warp.  At D = 128, NT = 1 the registers
-// allow 3 CTAs; 4 of 128 registers (spills) measured 70.5 us against 68.0 at 64 x
-// 8193 keys, 3 tiles in flight 68.6.
-constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+// CTAs per SM, and tiles in flight per warp.  At D = 128 the registers allow 3 CTAs with
+// 8 query rows and 2 with 16 (64 sequences x 8193 keys: 4 CTAs of 128 registers 73.7 us,
+// 3 68.7; 16 rows, 2 kv heads: 3 with spills 94, 2 71); at D = 64 and 32 3 with either
+// (16 rows, 2 kv heads: 2 CTAs 54.6 and 45.0 us, 3 38.9 and 29.1).
+constexpr int ctas_per_sm(int d, int nt) { return d == 128 && nt == 2 ? 2 : 3; }
 constexpr float kLift = 15.f;   // weights reach 2^kLift
 constexpr int kMinF = -60;      // smallest F of a key
 constexpr int stages(int d, int nt) { return d == 128 && nt == 1 ? 2 : 4; }
@@ -289,7 +290,7 @@ __device__ __forceinline__ bool nonfinite(uint32_t pair) {
 
 // One CTA = one run of tiles.
 template <int D, int GS, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_q4_kernel(Params p) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(Params p) {
   using L = Layout<D, GS, NT>;
   constexpr int J = L::J, NS = L::NS, BPG = GS / 32;
   constexpr int RB = D / 2;                     // bytes of a row of codes
@@ -921,17 +922,30 @@ int round_cost(int64_t ctas, int D) {
   return (ctas <= num_sms() ? 10 : 20) * (D + 192) / 320;
 }
 int64_t join_cost(int64_t rows, bool lens) { return 50 + rows / 32 + (lens ? 16 : 0); }
+// Query rows of a group, in eights.  16 rows unpack a key once for two instructions, but
+// a round takes longer and there are fewer: by the rounds of a run, from both forms'
+// times at 12 to 64 rows (D = 128, 64, 32; one sequence x 32768 to 64 x 8192 keys).
+// 2 kv heads x 64 sequences x 8192 keys, 16 / 32 rows: D = 128 eights 67 / 122 us,
+// sixteens 71 / 97; D = 64 47 / 84 and 39 / 65; one sequence, 4 heads x 32768, D = 64:
+// 12.3 / 16.9 and 13.7 / 16.5.
+int rows_per_group(int64_t heads, int64_t R, int64_t rounds, int D) {
+  auto run = [&](int nt) {
+    const int64_t slots = int64_t(num_sms()) * ctas_per_sm(D, nt);
+    return (heads * ((R + 8 * nt - 1) / (8 * nt)) * rounds + slots - 1) / slots;
+  };
+  return 20 * run(1) <= (D == 128 ? 26 : D == 64 ? 33 : 29) * run(2) + 10 ? 1 : 2;
+}
 int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, int D, bool lens) {
-  pl.nt = R > 8 ? 2 : 1;
-  const int64_t n_rg = (R + 8 * pl.nt - 1) / (8 * pl.nt);
   const int rounds = rounds_of(static_cast<int>(kv_len));
   const int64_t lim = int64_t(1) << 30;  // rounds and rows of the list are counted in 32 bits
-  if (B >= lim || R >= lim || Hkv * n_rg >= lim || B * Hkv >= lim / R ||
-      rounds * B >= lim / (Hkv * n_rg))
-    return fail(Q35_ERR_SHAPE, "attn_q4: too many query rows or key tiles");
+  if (B >= lim || R >= lim || B * Hkv >= lim / R)
+    return fail(Q35_ERR_SHAPE, "attn_q4: too many query rows");
+  pl.nt = R > 8 ? rows_per_group(B * Hkv, R, rounds, D) : 1;
+  const int64_t n_rg = (R + 8 * pl.nt - 1) / (8 * pl.nt);
+  if (rounds * B >= lim / (Hkv * n_rg)) return fail(Q35_ERR_SHAPE, "attn_q4: too many key tiles");
   pl.n_rg = static_cast<int>(n_rg);
   const int groups = static_cast<int>(B * Hkv * n_rg), total = groups * rounds;
-  const int slots = num_sms() * ctas_per_sm(pl.nt);
+  const int slots = num_sms() * ctas_per_sm(D, pl.nt);
   const int cut = total < slots ? total : slots, cut_per = (total + cut - 1) / cut;
   const int each = (groups + slots - 1) / slots, whole = each * rounds;
   pl.join = int64_t(cut_per) * round_cost(cut, D) + join_cost(B * Hkv * R, lens) <
@@ -949,7 +963,7 @@ using namespace q35;
 
 extern "C" int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                          int D) {
-  if (B <= 0 || Hkv <= 0 || Hq <= 0 || Sq <= 0 || D <= 0) return 0;
+  if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || Sq <= 0 || D <= 0) return 0;
   if (kv_len < 0 || kv_len >= (int64_t(1) << 31) - 256) return 0;
   int64_t most = 0;  // of the calls with and without kv_lens
   for (int lens = 0; lens < 2; ++lens) {

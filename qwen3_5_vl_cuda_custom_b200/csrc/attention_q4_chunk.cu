@@ -268,13 +268,13 @@ extern "C" int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64
   return plan(B, Hq, Hkv, Sq, kv_len, D).bytes;
 }
 
-// Fitted to 542 shapes (head_dim 64 and 128, 8 to 32 heads on 1 to 8, 1 to 16
-// sequences, 4 to 512 queries, 512 to 32768 keys); its choice costs 0.8 % on average
-// over the better of the two measured times, a fixed limit of 256 rows 14 %.  In
+// Fitted to 972 shapes (head_dim 32, 64 and 128, 8 to 32 heads on 1 to 8, 1 to 16
+// sequences, 4 to 512 queries, 512 to 32768 keys); its choice costs 0.6 % on average
+// over the better of the two measured times, a fixed limit of 256 rows 7 %.  In
 // microseconds: on the codes 16 query rows pass over all keys at a time; in chunks
 // a 128-key tile takes 2 in each of the CTAs the GPU holds, and the operands move at
-// 3.7 TB/s.  (512 queries x 32 heads, 8704 keys: 354 on the codes, 102 in chunks;
-// 16 queries x 32 heads, 8192 keys: 21 and 46.)
+// 5 TB/s.  (32 heads on 4, 8192 keys: 512 queries 355 on the codes, 100 in chunks; 64
+// queries 68 and 46; 16 queries 25 and 44.)
 extern "C" int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                          int D) {
   if (!plannable(B, Hq, Hkv, Sq, kv_len) || Hq % Hkv != 0 || B * Hq > 65535) return 0;
@@ -282,10 +282,11 @@ extern "C" int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq,
   int64_t tile;
   const double ctas = static_cast<double>(attn_tc_ctas(B, Hq, Hkv, Sq, &tile)) * pl.splits;
   const double waves = static_cast<double>((static_cast<int64_t>(ctas) + num_sms() - 1) / num_sms());
-  const double rows = static_cast<double>(Hq / Hkv * Sq), keys = static_cast<double>(B) * Hkv * kv_len;
+  const double passes = static_cast<double>((Hq / Hkv * Sq + 15) / 16);
+  const double keys = static_cast<double>(B) * Hkv * kv_len;
   const double bytes = keys * (1.25 * D + 1024) + static_cast<double>(B) * Hq * Sq * 768;
-  const double chunk = 14 + 2 * waves * pl.tiles_per_split + bytes * 0.27e-6;
-  const double codes = 9.4 + keys * ((rows + 15) / 16) * (D + 64) * 0.227e-6;
+  const double chunk = 14 + 2 * waves * pl.tiles_per_split + bytes * 0.2e-6;
+  const double codes = 12 + keys * passes * (D + 96) * 0.16e-6;
   return chunk < codes ? 1 : 0;
 }
 

@@ -579,7 +579,7 @@ def _cache_q4(name: str, k_codes, k_scales, v_codes, v_scales) -> tuple[int, int
             and k_scales.is_contiguous() and v_scales.is_contiguous()):
         B, Hkv, cap, half = cs
         D, groups = 2 * half, ss[3]
-        if (D == 128 or D == 64 or D == 32) and groups and not D % groups and ss == (B, Hkv, cap, groups, 2):
+        if (D == 128 or D == 64 or D == 32) and Hkv and groups and not D % groups and ss == (B, Hkv, cap, groups, 2):
             return B, Hkv, cap, D, D // groups
     for t, part, dt, dims in ((k_codes, "k_codes", torch.uint8, 4), (k_scales, "k_scales", _BF16, 5),
                               (v_codes, "v_codes", torch.uint8, 4), (v_scales, "v_scales", _BF16, 5)):

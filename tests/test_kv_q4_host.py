@@ -114,6 +114,20 @@ def test_workspace_covers_every_shape(lib):
     assert lib.q35_attn_q4_workspace(64, 32, 4, 1, 8193, 128) >= 0
 
 
+def test_workspace_of_refused_shapes_is_empty(lib):
+    for Hq, Hkv in ((1, 4), (7, 2), (0, 4), (4, 0), (-4, 2)):
+        assert lib.q35_attn_q4_workspace(2, Hq, Hkv, 1, 100, 64) == 0
+        assert lib.q35_attn_q4_chunk_workspace(2, Hq, Hkv, 1, 100, 64) == 0
+    assert lib.q35_attn_q4_workspace(2, 4, 2, 0, 100, 64) == 0
+    assert lib.q35_attn_q4_workspace(2, 4, 2, 1, 1 << 40, 64) == 0
+
+
+def test_a_cache_without_heads_is_refused():
+    empty = [torch.zeros(2, 0, 16, 32, dtype=torch.uint8), torch.zeros(2, 0, 16, 2, 2, dtype=torch.bfloat16)] * 2
+    with pytest.raises(RuntimeError):
+        K.attention_cache_q4(torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16), *empty, 4, 1.0, False)
+
+
 def test_operators_refuse_cpu_tensors():
     c = Q4LayerKVCache(1, 2, 16, 64, "cpu")
     x = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16)
