@@ -120,7 +120,8 @@ struct Layout {
   static constexpr int kStage = 2 * (kCodes + kScales);
   static constexpr int kRing = kStages * kStage;
   static constexpr int kRegs = NT * (D / 4 + 4);  // a lane's O, m, l
-  static constexpr int kKeys = kTile * 8;         // (F, 2^-F) of a tile's keys
+  // (F, 2^-F) of a tile's keys, V's scales and minima as fp16
+  static constexpr int kKeys = kTile * (8 + 16 + 16);
   static constexpr int kSmem = kWarps * (kRing + kKeys) + (kWarps - 1) * kRegs * 128;
 };
 
@@ -343,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * L::kRing;
   const uint32_t keys = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
                         kWarps * L::kRing + warp * L::kKeys;
+  const uint32_t vscale = keys + kTile * 8 + lane * 16;
   float *merge = reinterpret_cast<float *>(smem + kWarps * (L::kRing + L::kKeys));
 
   // ---- copies: this warp's tiles (tile 4 r + warp of round r of a group), ahead of
@@ -417,7 +419,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
   const int vsw = D == 128 ? (vrow >> 1) & 3 : D == 64 ? (vrow >> 2) & 1 : 0;
   const int vch = D == 32 ? 0 : lane >> 4;
   const int gv = (D == 128 ? g >> 1 : D == 64 ? (g >> 1) & 1 : 0) / BPG;  // the lane's V scale group
-  const uint32_t vsoff = (2 * t * NS + gv) * 4;
   const float scale_up = p.scale_log2 * 0x1p81f;
   uint32_t stage = 0;
 
@@ -589,11 +590,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
           const int f = max(kMinF + 127, max(static_cast<int>(top >> 7 & 0xffu) + 9,
                                              static_cast<int>(top >> 23 & 0xffu) - 10));
           const float fs = __uint_as_float((278 - f) << 23), fm = fs * 0x1p-20f;  // 2^(24-F), 2^(4-F)
+          // for a transposing ldmatrix: word j of the key's row serves lanes g = 2j, 2j + 1
+          uint32_t vs[4], vm[4];
 #pragma unroll
-          for (int i = 0; i < NS; ++i)
-            vw[i] = pack_h2(__uint_as_float(vw[i] << 16) * fs,
-                            __uint_as_float(vw[i] & 0xffff0000u) * fm);
-          sts_words<NS>(svs + lane * (NS * 4), vw);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t w = vw[(D == 128 ? j : D == 64 ? j & 1 : 0) / BPG];
+            const float sc = __uint_as_float(w << 16) * fs, mi = __uint_as_float(w & 0xffff0000u) * fm;
+            vs[j] = pack_h2(sc, sc);
+            vm[j] = pack_h2(mi, mi);
+          }
+          sts_words<4>(vscale, vs);
+          sts_words<4>(vscale + kTile * 16, vm);
           const uint32_t k2[2] = {
               __float_as_uint(__uint_as_float(0x4b000000u | f) - (8388608.f + 127.f)),
               __float_as_uint(fs * 0x1p-24f)};
@@ -664,18 +671,18 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
       }
 
       // ---- O^T += V^T P^T
-      uint32_t u[4];
+      uint32_t u[4], vs[4], vm[4];
+      ldsm4_t(vs, vscale);
+      ldsm4_t(vm, vscale + kTile * 16);
       if constexpr (D == 32) ldsm4_t(u, sv + vrow * RB);  // keys 0-7, 8-15, 16-23, 24-31
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         // scale pairs of keys (2t, 2t + 1) and (2t + 8, 2t + 9); minima for even and odd fields
-        uint32_t s2[2], m2[2][2];
+        const uint32_t s2[2] = {vs[2 * mt], vs[2 * mt + 1]};
+        uint32_t m2[2][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t at0 = svs + vsoff + (16 * mt + 8 * h) * (NS * 4);
-          const uint32_t pa = lds1(at0), pc = lds1(at0 + NS * 4);
-          s2[h] = __byte_perm(pa, pc, 0x5410);
-          m2[h][1] = __byte_perm(pa, pc, 0x7632);
+          m2[h][1] = vm[2 * mt + h];
           m2[h][0] = mul2(m2[h][1], 0x2c002c00u);  // 2^-4
         }
         auto product = [&](int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int i) {
