@@ -62,12 +62,12 @@
 // are XOR-swizzled by the row, so that both the 16-byte reads of K and the 8-row
 // reads of V touch every bank once.
 //
-// Measured (32/4 heads x 128, groups of 32): 64 sequences x 8193 keys 68.7 us, 4.9 TB/s
-// (the copies alone 61; a plain copy moves 6.5 TB/s); one sequence x 131072 keys 22.5 us;
-// x 500 keys 6.6 us.  610 warp instructions per 32-key tile, issue slots 60 % busy: what
+// Measured (32/4 heads x 128, groups of 32): 64 sequences x 8193 keys 67.8 us, 5.0 TB/s
+// (the copies alone 61; a plain copy moves 6.5 TB/s); one sequence x 131072 keys 21.7 us;
+// x 500 keys 6.6 us.  595 warp instructions per 32-key tile, issue slots 60 % busy: what
 // bounds it is copies and arithmetic together, the 16x8 matrix instructions (one per 2
 // clocks and SM) holding up the logic operations beside them.
-// Tried: P and V in bf16 (64.0 us, the errors above), P as two bf16 parts (70.8, 0.0021
+// Tried: P and V in bf16 (64.0 us at the time of 68.7, the errors above), P as two bf16 parts (70.8, 0.0021
 // to 0.0023); e4m3 operands for K (emulated: 48M instructions for 37M), shifts as
 // multiplications (12 % slower), a tile's scores together with the products of the tile
 // before (17 %), bulk copies instead of 16-byte ones.
@@ -358,25 +358,33 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
   const uint32_t cdst = crow * RB + ((cch ^ csw) << 4);
   const int srow = lane * 4 / NS;           // first row of the lane's chunk of scales
   Group ahead = gr;
-  int64_t arow = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
-  int next = lo;
+  int next = lo, ahead_end = gr.begin + gr.rounds;
+  // first row of this warp's tile of round `next` in its group (negative: the mark)
+  int r0 = ((lo - gr.begin - 1) * kWarps + warp) * kTile;
+  const uint8_t *kc_at, *vc_at, *ks_at, *vs_at;  // the group's row 0 (this lane's chunks)
+  auto ahead_at = [&]() {
+    const int64_t row = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
+    kc_at = reinterpret_cast<const uint8_t *>(p.c.k_codes) + row * RB + lane * 16;
+    vc_at = reinterpret_cast<const uint8_t *>(p.c.v_codes) + row * RB + lane * 16;
+    ks_at = reinterpret_cast<const uint8_t *>(p.c.k_scales) + row * (NS * 4) + lane * 16;
+    vs_at = reinterpret_cast<const uint8_t *>(p.c.v_scales) + row * (NS * 4) + lane * 16;
+  };
+  ahead_at();
   uint32_t next_stage = 0;  // byte offset in the ring
   auto issue = [&]() {
-    int r0 = 0;
-    for (; next < hi; ++next) {  // to the next round with a tile for this warp
-      if (next >= ahead.begin + ahead.rounds) {
+    for (; next < hi; ++next, r0 += kWarps * kTile) {  // to the next round with a tile for this warp
+      if (next >= ahead_end) {
         next_group(ahead);
-        arow = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
+        ahead_end = ahead.begin + ahead.rounds;
+        r0 = (warp - kWarps) * kTile;
+        ahead_at();
       }
-      r0 = ((next - ahead.begin - 1) * kWarps + warp) * kTile;
-      if (next > ahead.begin && r0 < ahead.len) break;
+      if (static_cast<uint32_t>(r0) < static_cast<uint32_t>(ahead.len)) break;
     }
     if (next < hi) {
       const int left = ahead.len - r0;
-      const int64_t row = arow + r0;
       const uint32_t dst = ring + next_stage;
-      const uint8_t *kc = reinterpret_cast<const uint8_t *>(p.c.k_codes) + row * RB + lane * 16;
-      const uint8_t *vc = reinterpret_cast<const uint8_t *>(p.c.v_codes) + row * RB + lane * 16;
+      const uint8_t *kc = kc_at + int64_t(r0) * RB, *vc = vc_at + int64_t(r0) * RB;
       if (left >= kTile) {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
@@ -392,14 +400,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
         }
       }
       if (lane < L::kScales / 16) {
-        const int64_t off = (row * NS + lane * 4) * 4;
+        const int64_t off = int64_t(r0) * (NS * 4);
         const bool live = srow < left;
-        copy16(dst + L::kCodes + lane * 16,
-               reinterpret_cast<const uint8_t *>(p.c.k_scales) + (live ? off : 0), live);
-        copy16(dst + 2 * L::kCodes + L::kScales + lane * 16,
-               reinterpret_cast<const uint8_t *>(p.c.v_scales) + (live ? off : 0), live);
+        copy16(dst + L::kCodes + lane * 16, ks_at + (live ? off : 0), live);
+        copy16(dst + 2 * L::kCodes + L::kScales + lane * 16, vs_at + (live ? off : 0), live);
       }
       ++next;
+      r0 += kWarps * kTile;
       next_stage = next_stage + L::kStage == L::kRing ? 0 : next_stage + L::kStage;
     }
     copies_commit();
