@@ -32,15 +32,6 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """_lib.call with ``device`` current (no context switch when it is already)."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args)
-    else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args)
-
-
 def _require(t: torch.Tensor, name: str, dtype: torch.dtype | tuple = _BF16) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
@@ -635,6 +626,9 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
     out and recorded as a device error.  k and v may be strided views."""
     B, Hkv, cap, D, group = _cache_q4("kv_append_q4", k_codes, k_scales, v_codes, v_scales)
     dev = k_codes.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return kv_append_q4(k, v, k_codes, k_scales, v_codes, v_scales, offset)
     k, ks = _strided_rows(k, "kv_append_q4.k", dev)
     v, vs = _strided_rows(v, "kv_append_q4.v", dev)
     shape = k.shape
@@ -647,10 +641,10 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
     else:
         rows, first = None, int(offset)
     k_strides = _lib.strides_arg(ks)
-    _call_on(dev, "q35_kv_append_q4", k.data_ptr(), v.data_ptr(), k_strides,
-             k_strides if ks == vs else _lib.strides_arg(vs), k_codes.data_ptr(), k_scales.data_ptr(),
-             v_codes.data_ptr(), v_scales.data_ptr(), B, Hkv, S, D, group, cap, first, rows,
-             _stream(k_codes))
+    _lib.call("q35_kv_append_q4", k.data_ptr(), v.data_ptr(), k_strides,
+              k_strides if ks == vs else _lib.strides_arg(vs), k_codes.data_ptr(), k_scales.data_ptr(),
+              v_codes.data_ptr(), v_scales.data_ptr(), B, Hkv, S, D, group, cap, first, rows,
+              _stream(k_codes))
 
 
 def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
@@ -661,15 +655,18 @@ def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Ten
     a device error."""
     B, Hkv, cap, D, group = _cache_q4("kv_read_q4", k_codes, k_scales, v_codes, v_scales)
     dev, n = k_codes.device, int(length)
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return kv_read_q4(k_codes, k_scales, v_codes, v_scales, start, length)
     if isinstance(start, torch.Tensor):
         starts, first = _per_sequence(start, "kv_read_q4.start", B, dev).data_ptr(), 0
     else:
         starts, first = None, int(start)
     k = torch.empty(B, Hkv, n, D, device=dev, dtype=_BF16)
     v = torch.empty_like(k)
-    _call_on(dev, "q35_kv_read_q4", k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-             v_scales.data_ptr(), k.data_ptr(), v.data_ptr(), B, Hkv, n, n, D, group, cap, first, starts,
-             _stream(k_codes))
+    _lib.call("q35_kv_read_q4", k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+              v_scales.data_ptr(), k.data_ptr(), v.data_ptr(), B, Hkv, n, n, D, group, cap, first, starts,
+              _stream(k_codes))
     return k, v
 
 

@@ -241,9 +241,8 @@ def check_attention(out, q, kv, vv, lens, scale, causal, group, chunk=False):
       * weights and values each rounded to bf16 (half a step, 2^-8):  2 * 2^-8 * A
       * scores off by at most d each: weights off by a factor e^(2d), so (e^(2d) - 1) * A.
         On the codes d is fp32 accumulation over T = scale sum_d |q_d| (128 s + |m|)
-        (the codes enter as 128 + c): 2^-19 T.  A chunk also rounds the keys to
-        bf16, 2^-8 scale sum_d |q_d k_d|, and its kernel's exp2 is off by up to
-        7.5e-5 < 2^-13.
+        (codes of up to 128 s): 2^-19 T.  A chunk also rounds the keys, 2^-8 scale
+        sum_d |q_d k_d|, and its kernel's exp2 is off by up to 7.5e-5 < 2^-13.
       * the output's own rounding: 2^-8 |ref|."""
     ref, A = R.attention(q, kv, vv, lens, scale, causal)
     qa = q.double().cpu().abs().amax(dim=(0, 1, 2))
