@@ -15,10 +15,10 @@
 // word may cost: hence paired fp32 arithmetic, one shuffle a step for minimum and
 // maximum together, and a multiplication for each division by S or Hkv.
 //
-// Measured (4 kv heads x 128): 8 x 8192 rows appended in 44.0 us, 3.9 TB/s (240
-// instructions per warp and 512 channels, a quarter of them paired fp32 at half rate;
-// issue slots 65 % busy), 4096 rows 4.1 us, 64 sequences x 1 row 1.9 us; 16 x 8192 rows
-// read in 58.7 us, 6.0 TB/s.
+// Measured (4 kv heads x 128): 8 x 8192 rows appended in 42.3 us, 4.0 TB/s (234
+// instructions per warp and 512 channels, 40 of them paired fp32 at half rate; issue
+// slots 66 % busy), 4096 rows 4.1 us, 64 sequences x 1 row 1.9 us; 16 x 8192 rows read in
+// 58.7 us, 6.0 TB/s.
 #include <type_traits>
 
 #include "kv_q4.cuh"
@@ -30,7 +30,7 @@ using q4::Cache;
 
 constexpr int kThreads = 256;
 // A CTA prefetches its next rows while it quantises: 7 CTAs of 128 threads per SM hold
-// in registers (8 x 8192 rows: 4 CTAs 46.7 us, 6 44.5, 7 43.9, 8 45.7, 10 49.0).
+// in registers (8 x 8192 rows, at 43.9 us: 4 CTAs 46.7, 6 44.5, 8 45.7, 10 49.0).
 constexpr int kAppendThreads = 128, kAppendCtas = 7;
 
 struct Rows {
@@ -149,25 +149,21 @@ __device__ __forceinline__ void quantise16(const uint32_t (&w)[8], uint32_t (&wo
   r = fmaf(r, fmaf(-s, r, 1.f), r);
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
   const float2 r2 = make_float2(r, r), m2 = make_float2(-lo, -lo), s2 = make_float2(-s, -s),
-               up = make_float2(kRound, kRound), down = make_float2(-kRound, -kRound);
-  const float2 k16 = make_float2(16.f, 16.f), k23 = make_float2(8388608.f, 8388608.f);
+               up = make_float2(kRound, kRound);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float2 q[4];
+    uint32_t q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 v;
       unpack_bf2(w[4 * h + i], v.x, v.y);
       const float2 d = __fadd2_rn(v, m2), y0 = __fmul2_rn(d, r2);
       const float2 y = __ffma2_rn(__ffma2_rn(y0, s2, d), r2, y0);
-      q[i] = __fadd2_rn(__fadd2_rn(y, up), down);
+      // the codes in the low 16 bits of two sums: (even channel, odd channel)
+      const float2 z = __fadd2_rn(y, up);
+      q[i] = __byte_perm(__float_as_uint(z.x), __float_as_uint(z.y), 0x5410);
     }
-    // (even channels, odd channels): sums of 16^i code_i are integers below 2^16, which
-    // 2^23 puts into the low bits
-    float2 f = __ffma2_rn(q[3], k16, q[2]);
-    f = __ffma2_rn(f, k16, q[1]);
-    f = __fadd2_rn(__ffma2_rn(f, k16, q[0]), k23);
-    word[h] = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410);
+    word[h] = (q[3] * 16u + q[2]) * 256u + (q[1] * 16u + q[0]);
   }
   const float c = -lo * r;
   uint32_t todo = 0;  // channels to decide in 64 bits
