@@ -31,7 +31,8 @@ using q4::Cache;
 
 constexpr int kThreads = 256;
 // A CTA prefetches its next rows while it quantises: 7 CTAs of 128 threads per SM hold
-// in registers (8 x 8192 rows, at 43.9 us: 4 CTAs 46.7, 6 44.5, 8 45.7, 10 49.0).
+// in registers (6, 7 and 8 CTAs: 8 x 8192 rows 39.8, 39.1 and 38.6 us, 4096 rows 4.0,
+// 4.1 and 4.4).
 constexpr int kAppendThreads = 128, kAppendCtas = 7;
 
 struct Rows {
