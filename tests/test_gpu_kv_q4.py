@@ -610,6 +610,46 @@ def test_a_captured_step_follows_the_lengths():
     K().device_error_check()
 
 
+@pytest.mark.parametrize("S,kv0", [(1, 0), (1, 700), (40, 300)])
+def test_a_captured_chain_equals_its_calls_one_by_one(S, kv0):
+    """Each call is launched ahead of the one in front of it and needs its results:
+    rows stored, read back and attended over, the next rows made from both."""
+    B, Hq, Hkv, D, steps = 2, 8, 2, 64, 8
+    x0 = rows((B, Hkv, S, D), 95).to(DEV)
+    cache0 = filled_cache(B, Hkv, 1024, D, 32, 96)[0]
+
+    def chain(x, cache, pause):
+        outs = []
+        for i in range(steps):
+            K().kv_append_q4(x, x * 0.5, *cache, kv0 + i * S)
+            pause()
+            k, v = K().kv_read_q4(*cache, max(0, kv0 + i * S - 3), 3 + S if kv0 else S)
+            pause()
+            q = (k[:, :, -S:].repeat_interleave(Hq // Hkv, dim=1) - 0.25).contiguous()
+            out = K().attention_cache_q4(q, *cache, kv0 + (i + 1) * S, 0.125, True)
+            pause()
+            x = (out.view(B, S, Hkv, Hq // Hkv, D).sum(3).transpose(1, 2) + v[:, :, -S:]).contiguous()
+            outs += [out, x]
+        return outs
+
+    want = chain(x0, [t.clone() for t in cache0], torch.cuda.synchronize)
+    cache, x = [t.clone() for t in cache0], x0.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain(x, cache, lambda: None)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(x, cache, lambda: None)
+    for _ in range(3):
+        for t, old in zip(cache, cache0):
+            t.copy_(old)
+        graph.replay()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("before", ["copy", "fill", "kernel", "two streams", "nothing"])
 @pytest.mark.parametrize("kv,Sq", [(40, 1), (3000, 1), (900, 200)])
 def test_a_capture_behind_other_work(monkeypatch, before, kv, Sq):
