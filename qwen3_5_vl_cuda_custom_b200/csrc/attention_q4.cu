@@ -55,7 +55,9 @@
 // several whole and begin another.  Nothing depends on the lengths being alike,
 // and the rings below do not drain between groups.  A group that one run holds
 // whole is written at once, the others leave (max, sum, O) partials that a second
-// kernel joins; a run leaves at most two.
+// kernel joins; a run leaves at most two.  When there are many short groups, runs are of
+// whole groups, and of single warps: a warp takes all tiles of a group one after the
+// other, and nothing is joined.
 //
 // Each warp keeps its tiles coming through a private ring of asynchronous 16-byte
 // copies, so warps meet only at the end of a group.  The 16-byte chunks of a row
@@ -134,10 +136,11 @@ __device__ __forceinline__ int clamp_len(const Params &p, int b) {
   if (!p.kv_lens) return p.kv_len;
   return max(0, min(p.kv_lens[b], p.kv_len));
 }
-// Rounds of a group in the list: its tiles by fours (a sequence without rows counts
-// one, so that some CTA writes its zeros) behind one for its start and end.
-__host__ __device__ __forceinline__ int rounds_of(int len) {
-  return 1 + (len > 0 ? (len + kWarps * kTile - 1) / (kWarps * kTile) : 1);
+// Rounds of a group in the list: its tiles by `share`, the warps that take part in it
+// (a sequence without rows counts one, so that someone writes its zeros), behind one for
+// its start and end.
+__host__ __device__ __forceinline__ int rounds_of(int len, int share = kWarps) {
+  return 1 + (len > 0 ? (len + share * kTile - 1) / (share * kTile) : 1);
 }
 
 // A group of the list: its sequence, its (kv head, row group) index, its first
@@ -289,8 +292,8 @@ __device__ __forceinline__ bool nonfinite(uint32_t pair) {
   return (((pair & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
 }
 
-// One CTA = one run of tiles.
-template <int D, int GS, int NT>
+// One CTA = one run of tiles (SHARE = 4), or each of its warps has one of its own (1).
+template <int D, int GS, int NT, int SHARE>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(Params p) {
   using L = Layout<D, GS, NT>;
   constexpr int J = L::J, NS = L::NS, BPG = GS / 32;
@@ -301,12 +304,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_seq = p.Hkv * p.n_rg;
+  constexpr bool kAlone = SHARE == 1;
+  const int part = kAlone ? 0 : warp;        // the warp's tile of a round
+  constexpr int kRound = SHARE * kTile;      // keys of a round
 
   if (p.kv_lens) wait_for_earlier();
   // ---- the run [lo, hi) of rounds and the group it begins in
   Group gr;
   int lo, hi;
-  if (p.scan) {
+  if (!kAlone && p.scan) {
     int per = 0;
     int *table = reinterpret_cast<int *>(p.ws + partial_rows(p.runs, NT) * (D + 2));
     const int total = scan_rounds(p, [&](int n) {
@@ -316,8 +322,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
     lo = static_cast<int>(min(int64_t(blockIdx.x) * per, int64_t(total)));
     hi = min(lo + per, total);
   } else {
-    const int all = rounds_of(p.kv_len) * per_seq;
-    lo = blockIdx.x * p.per;
+    const int all = rounds_of(p.kv_len, SHARE) * per_seq;
+    lo = (kAlone ? blockIdx.x * kWarps + warp : blockIdx.x) * p.per;
     hi = min(lo + p.per, all * p.B);
     gr.b = lo / all;
     gr.begin = gr.b * all;
@@ -327,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
       if (p.kv_lens[b] < 0 || p.kv_lens[b] > p.kv_len)
         report_error(p.err, DEV_ERR_INDEX, 311, b, p.kv_lens[b]);
   if (lo >= hi) return;
-  auto seq_rounds = [&](int len) { return rounds_of(p.scan ? len : p.kv_len); };
+  auto seq_rounds = [&](int len) { return rounds_of(!kAlone && p.scan ? len : p.kv_len, SHARE); };
   gr.len = clamp_len(p, gr.b);
   gr.rounds = seq_rounds(gr.len);
   gr.hg = (lo - gr.begin) / gr.rounds;
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
   const uint32_t vscale = keys + kTile * 8 + lane * 16;
   float *merge = reinterpret_cast<float *>(smem + kWarps * (L::kRing + L::kKeys));
 
-  // ---- copies: this warp's tiles (tile 4 r + warp of round r of a group), ahead of
+  // ---- copies: this warp's tiles (tile SHARE r + part of round r of a group), ahead of
   // their use.  Lane i copies chunks i, i + 32, ... of the tile's codes (chunk c of row
   // r goes to chunk c ^ swizzle(r)) and chunk i of its scales.  Rows behind the length
   // are not read (a chunk of narrow scales may hold up to 3 of them: the capacity is a
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
   Group ahead = gr;
   int next = lo, ahead_end = gr.begin + gr.rounds;
   // first row of this warp's tile of round `next` in its group (negative: the mark)
-  int r0 = ((lo - gr.begin - 1) * kWarps + warp) * kTile;
+  int r0 = (lo - gr.begin - 1) * kRound + part * kTile;
   const uint8_t *kc_at, *vc_at, *ks_at, *vs_at;  // the group's row 0 (this lane's chunks)
   auto ahead_at = [&]() {
     const int64_t row = (int64_t(ahead.b) * p.Hkv + ahead.hg / p.n_rg) * p.cap;
@@ -372,11 +378,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
   ahead_at();
   uint32_t next_stage = 0;  // byte offset in the ring
   auto issue = [&]() {
-    for (; next < hi; ++next, r0 += kWarps * kTile) {  // to the next round with a tile for this warp
+    for (; next < hi; ++next, r0 += kRound) {  // to the next round with a tile for this warp
       if (next >= ahead_end) {
         next_group(ahead);
         ahead_end = ahead.begin + ahead.rounds;
-        r0 = (warp - kWarps) * kTile;
+        r0 = part * kTile - kRound;
         ahead_at();
       }
       if (static_cast<uint32_t>(r0) < static_cast<uint32_t>(ahead.len)) break;
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
         copy16(dst + 2 * L::kCodes + L::kScales + lane * 16, vs_at + (live ? off : 0), live);
       }
       ++next;
-      r0 += kWarps * kTile;
+      r0 += kRound;
       next_stage = next_stage + L::kStage == L::kRing ? 0 : next_stage + L::kStage;
     }
     copies_commit();
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
     }
 
     for (int round = max(at, gr.begin + 1); round < end; ++round) {
-      const int key0 = ((round - gr.begin - 1) * kWarps + warp) * kTile;
+      const int key0 = (round - gr.begin - 1) * kRound + part * kTile;
       if (key0 >= len) break;
       copies_wait<L::kStages - 1>();
       __syncwarp();
@@ -744,8 +750,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
       row_l[nt][0] *= 0x1p-15f;
       row_l[nt][1] *= 0x1p-15f;
     }
-    __syncthreads();
-    if (warp > 0) {
+    if constexpr (!kAlone) __syncthreads();
+    if (part > 0) {
       float *dst = merge + (warp - 1) * (L::kRegs * 32) + lane;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -760,25 +766,25 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
           for (int e = 0; e < 4; ++e) dst[((D / 4 + 4) * nt + 4 + 4 * i + e) * 32] = o[i][nt][e];
       }
     }
-    __syncthreads();
-    if (warp == 0) {
+    if constexpr (!kAlone) __syncthreads();
+    if (part == 0) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float *src = merge + (D / 4 + 4) * nt * 32 + lane;
-        float f[kWarps][2], l[2], m[2];
+        float f[SHARE][2], l[2], m[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float mw[kWarps - 1];
           m[c] = row_m[nt][c];
 #pragma unroll
-          for (int w = 0; w < kWarps - 1; ++w) {
+          for (int w = 0; w < SHARE - 1; ++w) {
             mw[w] = src[(w * L::kRegs + c) * 32];
             m[c] = fmaxf(m[c], mw[w]);
           }
-          f[0][c] = exp2_fast(row_m[nt][c] - m[c]);
+          f[0][c] = kAlone ? 1.f : exp2_fast(row_m[nt][c] - m[c]);
           l[c] = row_l[nt][c] * f[0][c];
 #pragma unroll
-          for (int w = 0; w < kWarps - 1; ++w) {
+          for (int w = 0; w < SHARE - 1; ++w) {
             f[w + 1][c] = exp2_fast(mw[w] - m[c]);
             l[c] = fmaf(src[(w * L::kRegs + 2 + c) * 32], f[w + 1][c], l[c]);
           }
@@ -791,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
           for (int e = 0; e < 4; ++e) {
             float v = o[i][nt][e] * f[0][e & 1];
 #pragma unroll
-            for (int w = 0; w < kWarps - 1; ++w)
+            for (int w = 0; w < SHARE - 1; ++w)
               v = fmaf(src[(w * L::kRegs + 4 + 4 * i + e) * 32], f[w + 1][e & 1], v);
             o[i][nt][e] = v;
           }
@@ -921,7 +927,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_q4_join_kernel(Params p, int 
 // Query rows per CTA, and the runs the rounds are cut into.
 struct Plan {
   int nt, n_rg, runs, per;
-  bool scan, join;
+  bool scan, join, alone;  // alone: a warp per group
 };
 // When to cut groups: a round at D = 128 takes about 0.8 us while every CTA has an SM
 // to itself and 1.6 once some SMs hold two or three; the second kernel adds 2.2 us and
@@ -962,11 +968,27 @@ int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, int D, bool le
   const int slots = num_sms() * ctas_per_sm(D, pl.nt);
   const int cut = total < slots ? total : slots, cut_per = (total + cut - 1) / cut;
   const int each = (groups + slots - 1) / slots, whole = each * rounds;
-  pl.join = int64_t(cut_per) * round_cost(cut, D) + join_cost(B * Hkv * R, lens) <
-            int64_t(whole) * round_cost((groups + each - 1) / each, D);
+  const int64_t cost = int64_t(whole) * round_cost((groups + each - 1) / each, D);
+  const int64_t cut_cost = int64_t(cut_per) * round_cost(cut, D) + join_cost(B * Hkv * R, lens);
+  // A warp per group: its tiles one after the other, but four groups begin and end at a
+  // time and no warp is without a tile.  A round of it costs 0.85 of one that four warps
+  // share and join (396 shapes, 1 to 1000 keys: the choice is 0.7 % above the best of the
+  // three on average; 59 sequences x 8 heads x 272 rows, 44 keys, D = 64: whole 84 us,
+  // alone 31; 64 x 8 heads x 8 rows, 64 keys, D = 128: 8.0 and 4.3; 64 x 4 x 8, 128 keys:
+  // 5.5 and 6.1).
+  const int64_t tiles = rounds_of(static_cast<int>(kv_len), 1);
+  const int64_t warp_each = (groups + kWarps * int64_t(slots) - 1) / (kWarps * int64_t(slots));
+  const int64_t alone_runs = (groups + kWarps * warp_each - 1) / (kWarps * warp_each);
+  pl.alone = tiles * groups < lim &&
+             17 * tiles * warp_each * round_cost(alone_runs, D) < 20 * (cost < cut_cost ? cost : cut_cost);
+  pl.join = !pl.alone && cut_cost < cost;
   pl.scan = pl.join && lens;
   pl.per = pl.join ? cut_per : whole;
   pl.runs = pl.scan ? cut : (total + pl.per - 1) / pl.per;
+  if (pl.alone) {
+    pl.per = static_cast<int>(warp_each * tiles);
+    pl.runs = static_cast<int>(alone_runs);
+  }
   return Q35_OK;
 }
 
@@ -1043,7 +1065,7 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
   const int64_t rows = B * Hkv * R;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto d, auto gs, auto nt) -> int {
-    auto *kern = &attn_q4_kernel<d(), gs(), nt()>;
+    auto *kern = pl.alone ? &attn_q4_kernel<d(), gs(), nt(), 1> : &attn_q4_kernel<d(), gs(), nt(), kWarps>;
     constexpr int smem = Layout<d(), gs(), nt()>::kSmem;
     const int e = ensure_smem_attr(reinterpret_cast<const void *>(kern), smem);
     if (e) return e;

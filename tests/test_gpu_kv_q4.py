@@ -277,6 +277,25 @@ def test_attention_on_the_codes(D, group, Hq, Hkv, Sq, kv, causal):
 
 
 @pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,kv,causal", [
+    (70, 8, 8, 1, 20, False), (60, 8, 8, 3, 33, True), (130, 4, 4, 2, 1, True),
+    (30, 8, 4, 10, 70, True),                      # several groups of rows per kv head
+])
+def test_attention_of_many_short_caches(D, group, B, Hq, Hkv, Sq, kv, causal):
+    """More groups than the GPU holds at a time, of a tile or a few: with one length and
+    with a length per sequence (0 among them)."""
+    cap = -(-kv // 16) * 16
+    cache, kk, vv = filled_cache(B, Hkv, cap, D, group, 87, 0.5)
+    q = rows((B, Hq, Sq, D), 88, 0.5)
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, causal)
+    check_attention(out, q, kk, vv, [kv] * B, D ** -0.5, causal, group)
+    lens = [(7 * b) % (kv + 1) for b in range(B)]
+    got = K().attention_cache_q4(q.to(DEV), *cache, torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                 D ** -0.5, causal, kv)
+    check_attention(got, q, kk, vv, lens, D ** -0.5, causal, group)
+
+
+@pytest.mark.parametrize("D,group", SHAPES)
 @pytest.mark.parametrize("Hq,Hkv,Sq,kv,causal", [(1, 1, 1, 7, False), (8, 1, 1, 300, False),
                                                  (14, 2, 3, 1000, True), (4, 4, 1, 4000, False)])
 def test_attention_on_the_codes_keeps_11_bits(D, group, Hq, Hkv, Sq, kv, causal):
