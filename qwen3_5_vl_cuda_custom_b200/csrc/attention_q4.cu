@@ -69,10 +69,10 @@
 // x 500 keys 6.6 us.  595 warp instructions per 32-key tile, issue slots 60 % busy: what
 // bounds it is copies and arithmetic together, the 16x8 matrix instructions (one per 2
 // clocks and SM) holding up the logic operations beside them.
-// Tried: P and V in bf16 (64.0 us at the time of 68.7, the errors above), P as two bf16 parts (70.8, 0.0021
-// to 0.0023); e4m3 operands for K (emulated: 48M instructions for 37M), shifts as
-// multiplications (12 % slower), a tile's scores together with the products of the tile
-// before (17 %), bulk copies instead of 16-byte ones.
+// Tried: P and V in bf16 (64.0 us when this form took 68.7, the errors above), P as two
+// bf16 parts (70.8, 0.0021 to 0.0023); e4m3 operands for K (emulated: 48M instructions
+// for 37M), shifts as multiplications (12 % slower), a tile's scores together with the
+// products of the tile before (17 %), bulk copies instead of 16-byte ones.
 #include <cuda_fp16.h>
 #include <float.h>
 
