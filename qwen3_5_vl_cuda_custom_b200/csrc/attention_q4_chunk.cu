@@ -13,8 +13,10 @@
 //   1. attn_q4_absmax_kernel: largest |q|, |k|, |v| of each kv head (k, v from the
 //      scales alone, a fifth of the cache's bytes).
 //   2. attn_q4_operands_kernel: q, k, v as scaled fp16 [.., 128].  A NaN among the
-//      values would reach rows that do not see it (0 * NaN); it becomes 0 and 3. puts it
-//      into the rows that do, from the first such key of every 32 channels.
+//      values would reach rows that do not see it (0 * NaN), and one among the keys is
+//      lost in 3., whose polynomial exponential clamps its argument; both become 0 and 3.
+//      puts the NaN into the rows that see it, from the first such key of every 32
+//      channels (of all channels for a key).
 //   3. attn_tc_f16: the attention.  A short chunk has fewer query blocks than the GPU
 //      has SMs (512 tokens x 32 heads: 64 CTAs), so the key tiles are cut into as many
 //      splits as fill it, which leave fp32 partials ...
@@ -44,7 +46,7 @@ struct Chunk {
   Cache c;
   float4 *maxima;  // [slices][B * Hkv] (|q|, |k|, |v|)
   float *v_scale;  // [B * Hkv]
-  int *v_nan;      // [B * Hkv][4] first key whose value is NaN in 32 channels each
+  int *nan;        // [B * Hkv][4] first key that makes 32 output channels NaN
   __half *qo, *ko, *vo;
   int D, group, q_rows;  // q_rows = Hq / Hkv * Sq
   int64_t cap;
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_absmax_kernel(Chunk p) {
   }
   let_next_launch();
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x < 4) p.v_nan[bh * 4 + threadIdx.x] = INT_MAX;
+  if (blockIdx.x == 0 && threadIdx.x < 4) p.nan[bh * 4 + threadIdx.x] = INT_MAX;
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 0; i < 3; ++i)
@@ -174,8 +176,10 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
         o[k] = pack_h2(a * f, b * f);
       }
     } else {
-      if (which[i] == 2 && ((x[i].y & 0x7fffffffu) > 0x7f800000u)) {  // (a minimum of NaN)
-        atomicMin(&p.v_nan[bh * 4 + ch / 4], static_cast<int>(row[i]));
+      if ((x[i].y & 0x7fffffffu) > 0x7f800000u) {  // (a minimum of NaN)
+        // a value's group covers its own channels; a key's score is NaN, and so are all
+        for (int c = which[i] == 2 ? ch / 4 : 0; c < (which[i] == 2 ? ch / 4 + 1 : 4); ++c)
+          atomicMin(&p.nan[bh * 4 + c], static_cast<int>(row[i]));
         x[i].x = x[i].y = 0u;
       }
 #pragma unroll
@@ -222,7 +226,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_splits_kernel(F16Extra x, ui
 // Splits of the key tiles and the workspace's parts, in bytes.
 struct Plan {
   int splits, tiles_per_split, pad, slices;
-  int64_t v_scale, v_nan, ko, vo, qo, part, bytes;
+  int64_t v_scale, nan, ko, vo, qo, part, bytes;
 };
 Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   Plan pl{};
@@ -242,8 +246,8 @@ Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   const int64_t slices = 4 * int64_t(num_sms()) / bh;
   pl.slices = static_cast<int>(slices < 2 ? 2 : slices > kMaxSlices ? kMaxSlices : slices);
   pl.v_scale = pl.slices * bh * int64_t(sizeof(float4));
-  pl.v_nan = pl.v_scale + (bh * int64_t(sizeof(float)) + 15) / 16 * 16;
-  pl.ko = pl.v_nan + bh * int64_t(sizeof(int4));
+  pl.nan = pl.v_scale + (bh * int64_t(sizeof(float)) + 15) / 16 * 16;
+  pl.ko = pl.nan + bh * int64_t(sizeof(int4));
   pl.vo = pl.ko + bh * pl.pad * kPad * 2;
   pl.qo = pl.vo + bh * pl.pad * kPad * 2;
   pl.part = pl.qo + rows * kPad * 2;
@@ -320,7 +324,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
               static_cast<uint32_t *>(const_cast<void *>(v_scales))};
   c.maxima = reinterpret_cast<float4 *>(ws);
   c.v_scale = reinterpret_cast<float *>(ws + pl.v_scale);
-  c.v_nan = reinterpret_cast<int *>(ws + pl.v_nan);
+  c.nan = reinterpret_cast<int *>(ws + pl.nan);
   c.ko = reinterpret_cast<__half *>(ws + pl.ko);
   c.vo = reinterpret_cast<__half *>(ws + pl.vo);
   c.qo = reinterpret_cast<__half *>(ws + pl.qo);
@@ -343,7 +347,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   Q35_LAUNCH_CHECK("attn_q4 operands launch");
   F16Extra x{};
   x.v_scale = c.v_scale;
-  x.v_nan = c.v_nan;
+  x.nan = c.nan;
   x.rows = B * Hq * Sq;
   x.splits = pl.splits;
   x.tiles_per_split = pl.tiles_per_split;

@@ -134,20 +134,20 @@ __device__ __forceinline__ int split_tiles(const AttnParams &p, int split, int n
 }
 // kF16 epilogue of one query row: D columns of O (read 32 at a time from TMEM by the
 // whole warp) as bf16, or as an fp32 partial with its (max in log2 units, sum).
-// (Values stored as NaN are zeros among the operands: the blocks of 32 channels in
-// which the row sees one get their NaN here.)
+// (Keys and values stored as NaN are zeros among the operands: the blocks of 32 channels
+// of a row that sees one get their NaN here.)
 __device__ __forceinline__ void store_row_f16(const AttnParams &p, uint32_t o_tm, bool some,
                                               bool valid, int b, int h, int64_t qi, int split,
                                               float m_log2, float l, float f) {
   const int64_t rows = p.x.rows;
   const int64_t last = p.causal ? min(qi + p.Skv - p.Sq, p.Skv - 1) : p.Skv - 1;
-  const int *v_nan = p.x.v_nan + (static_cast<int64_t>(b) * p.Hkv + h / (p.Hq / p.Hkv)) * 4;
+  const int *nan = p.x.nan + (static_cast<int64_t>(b) * p.Hkv + h / (p.Hq / p.Hkv)) * 4;
   const int64_t row = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq + qi;
   const int64_t slot = row * p.x.splits + split;
   const float all = p.x.part ? f : (l > 0.f ? f / l : 0.f);
 #pragma unroll 1
   for (int c = 0; c < p.x.D / 32; ++c) {
-    const float inv = v_nan[c] <= last ? NAN : all;
+    const float inv = nan[c] <= last ? NAN : all;
     uint32_t r[32];
     if (some) {
       sm100::tmem_ld32(o_tm + c * 32, r);

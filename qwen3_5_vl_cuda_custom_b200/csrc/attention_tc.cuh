@@ -8,7 +8,7 @@ namespace q35 {
 
 struct F16Extra {
   const float *v_scale; // [B * Hkv]: what the output is multiplied by
-  const int *v_nan;     // [B * Hkv][4]: first key whose value is NaN in 32 channels each
+  const int *nan;       // [B * Hkv][4]: first key that makes 32 output channels NaN each
   float *part;          // fp32 partials [rows, splits, D], then (m, l) [rows, splits]; or null
   int64_t rows;         // B * Hq * Sq
   int splits, tiles_per_split, D;
