@@ -55,9 +55,17 @@ struct Chunk {
   float q_sign;          // of the scale: the attention kernels want it positive
 };
 
+__device__ __forceinline__ bool nonfinite(uint32_t pair) {
+  return (((pair & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
+}
 __device__ __forceinline__ float largest(float a, float x) {
   x = fabsf(x);
   return x < INFINITY ? fmaxf(a, x) : a;
+}
+// The largest magnitude that a (scale, minimum) pair's codes can stand for.
+__device__ __forceinline__ float largest_of(float a, uint32_t pair) {
+  if (nonfinite(pair)) return a;  // its values count as NaN
+  return fminf(fmaxf(a, fmaxf(fabsf(q4::value(0.f, pair)), fabsf(q4::value(15.f, pair)))), FLT_MAX);
 }
 
 __global__ void __launch_bounds__(kThreads) attn_q4_absmax_kernel(Chunk p) {
@@ -82,8 +90,8 @@ __global__ void __launch_bounds__(kThreads) attn_q4_absmax_kernel(Chunk p) {
 #pragma unroll 4
   for (int64_t i = tid; i < n; i += step) {
     const uint32_t k = p.c.k_scales[base + i], v = p.c.v_scales[base + i];
-    m[1] = largest(largest(m[1], q4::value(0.f, k)), q4::value(15.f, k));
-    m[2] = largest(largest(m[2], q4::value(0.f, v)), q4::value(15.f, v));
+    m[1] = largest_of(m[1], k);
+    m[2] = largest_of(m[2], v);
   }
   __shared__ float part[3][kThreads / 32];
 #pragma unroll
@@ -113,6 +121,10 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
+
+// fp16's finite range: a value that fp32 cannot hold (finite scale and minimum, infinite
+// together) must not become 0 * infinity in a row that does not see it.
+__device__ __forceinline__ float saturate(float x) { return fminf(fmaxf(x, -65504.f), 65504.f); }
 
 // A thread writes 8 of the 128 channels of kRows operand rows; rows: keys, values,
 // queries.  What it reads is on its way before the scales are known.
@@ -154,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) e[i] = exponent(warp_max(m[i]));
     if (threadIdx.x == 0) {
-      const int a = max(-100, min((e[0] - e[1]) / 2, 100)), v = max(-100, min(e[2] - 14, 100));
+      const int a = max(-100, min((e[0] - e[1]) / 2, 100)), v = max(-100, e[2] - 14);  // (at most 114)
       scale[0] = pow2(-a) * p.q_sign;
       scale[1] = pow2(a);
       scale[2] = pow2(-v);
@@ -176,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
         o[k] = pack_h2(a * f, b * f);
       }
     } else {
-      if ((x[i].y & 0x7fffffffu) > 0x7f800000u) {  // (a minimum of NaN)
+      if (nonfinite(x[i].y)) {
         // a value's group covers its own channels; a key's score is NaN, and so are all
         for (int c = which[i] == 2 ? ch / 4 : 0; c < (which[i] == 2 ? ch / 4 + 1 : 4); ++c)
           atomicMin(&p.nan[bh * 4 + c], static_cast<int>(row[i]));
@@ -184,8 +196,8 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        o[k] = pack_h2(q4::value(q4::code_of(x[i].x, 2 * k), x[i].y) * f,
-                       q4::value(q4::code_of(x[i].x, 2 * k + 1), x[i].y) * f);
+        o[k] = pack_h2(saturate(q4::value(q4::code_of(x[i].x, 2 * k), x[i].y) * f),
+                       saturate(q4::value(q4::code_of(x[i].x, 2 * k + 1), x[i].y) * f));
     }
     __half *dst = which[i] == 0 ? p.qo + (bh * p.q_rows + row[i]) * kPad
                                 : (which[i] == 2 ? p.vo : p.ko) + (bh * p.pad + row[i]) * kPad;

@@ -46,3 +46,46 @@ def test_a_nan_key_at_any_place_of_a_tile(monkeypatch, chunk, Hq, Hkv):
             assert torch.isfinite(want).all()
             assert torch.equal(got[:first], want[:first]), (key, causal)
             assert torch.equal(got[:, :Hkv - 1], want[:, :Hkv - 1]), (key, causal)
+
+
+# ------------------------------------------------------------------ values of every size
+@pytest.mark.parametrize("D,group", [(128, 32), (64, 64), (32, 32)])
+@pytest.mark.parametrize("hidden", [(0.0, 3e38), (2e37, -3e38), (3e37, 0.0), (0.0, 2.0 ** 20), (0.0, 2.0 ** 116),
+                                    (math.inf, 1.0), (1.0, -math.inf)])
+def test_rows_a_chunk_does_not_see_hold_anything(monkeypatch, D, group, hidden):
+    """Finite or not, a value reaches the queries that see it only.  A head's values share
+    one power of two in this form: with e the exponent of the largest they round to
+    2^(e - 39) at least, 2^-38 of the largest (at most fp32's largest).
+    Other bounds as for any chunk: weights and values 2^-11 each, the keys' rounding and
+    the exponential's 2^-13 in d, the output's 2^-8."""
+    force(monkeypatch, True)
+    B, Hq, Hkv, Sq, kv = 1, 4, 2, 40, 150
+    cache, kk, vv = filled_cache(B, Hkv, 160, D, group, 133, 0.5)
+    q = rows((B, Hq, Sq, D), 134, 0.5)
+    seen = kv - 3  # keys 147 .. 149: the last three queries'
+    cache[3][:, :, seen:kv, :, 0], cache[3][:, :, seen:kv, :, 1] = hidden
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, True).double().cpu()[:, :Sq - 3]
+    ref, A = R.attention(q[:, :, :Sq - 3], kk, vv, [seen], D ** -0.5, True)
+    big = R.values(cache[2], cache[3])[:, :, :kv].abs()
+    big = float(torch.where(torch.isfinite(big), big.clamp(max=2.0 ** 128), torch.zeros_like(big)).max())
+    d = 2.0 ** -11 * D ** -0.5 * float((q.double().abs().amax((0, 1, 2)) * kk.abs().amax((0, 1, 2))).sum())
+    tol = A * (2 ** -10 + math.expm1(2 * (d + 2.0 ** -13))) + 2 ** -8 * ref.abs() + 2.0 ** -38 * big
+    assert torch.isfinite(out).all()
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+@pytest.mark.parametrize("chunk", [True, False])
+def test_the_largest_values_come_through(monkeypatch, chunk):
+    """Values up to 2^126 (2^98 on the codes): both forms return their weighted mean."""
+    force(monkeypatch, chunk)
+    top = 2.0 ** (127 if chunk else 99)
+    B, Hq, Hkv, Sq, kv, D, group = 1, 4, 2, 20, 150, 64, 32
+    cache, kk, _ = filled_cache(B, Hkv, 160, D, group, 135, 0.5)
+    q = rows((B, Hq, Sq, D), 136, 0.5)
+    cache[3][..., 0], cache[3][..., 1] = top / 32, -top / 2
+    vv = R.values(cache[2], cache[3])
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, False).double().cpu()
+    ref, A = R.attention(q, kk, vv, [kv], D ** -0.5, False)
+    d = 2.0 ** -11 * D ** -0.5 * float((q.double().abs().amax((0, 1, 2)) * kk.abs().amax((0, 1, 2))).sum())
+    tol = A * (2 ** -10 + math.expm1(2 * (d + 2.0 ** -13))) + 2 ** -8 * ref.abs()
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
