@@ -515,9 +515,9 @@ Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_sc
 /* The same for many query rows per kv head (a chunk of a prompt), all sequences of
  * kv_len >= 1 rows: the rows go through scaled fp16 copies in the workspace
  * (q35_attn_q4_chunk_workspace(...) bytes, 16-byte aligned) and the tensor-memory
- * attention kernels.  B * Hq <= 65535.  Per kv head, the largest |q| times the
- * largest |k| must stay below 2^30; values, and the keys against the queries, lose
- * bits once they are 2^-27 of the largest of their head's rows, hidden ones included. */
+ * attention kernels.  B * Hq <= 65535.  Per kv head, queries and keys lose bits once
+ * they are 2^-27 of the largest of their head's rows, values 2^-38 of it, rows that a
+ * query does not see included.                                              */
 Q35_API int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D); /* 1: estimated faster than q35_attn_q4_fwd */
 Q35_API int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64_t Sq,

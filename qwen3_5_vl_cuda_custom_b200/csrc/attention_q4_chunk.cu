@@ -6,9 +6,9 @@
 // bf16 on the way shows: a score moves by up to 2^-8 of its terms and the output by
 // 0.0048 (relative, normal data), against 0.0017 from its own rounding to bf16.  So
 // the operands are fp16, whose 11 bits make it vanish, scaled per sequence and kv head
-// by powers of two, for the range that bf16 has and fp16 has not: v to a largest value
-// in [2^13, 2^14), q and k against one another to largest values of like size, so that
-// the scores stay what they are.
+// by powers of two, for the range that bf16 has and fp16 has not: q, k and v to largest
+// values in [2^13, 2^14) each.  The attention kernels multiply the scores by what q and
+// k were divided by, and the output by v's.
 //
 //   1. attn_q4_absmax_kernel: largest |q|, |k|, |v| of each kv head (k, v from the
 //      scales alone, a fifth of the cache's bytes).
@@ -45,14 +45,14 @@ struct Chunk {
   const uint16_t *q;
   Cache c;
   float4 *maxima;  // [slices][B * Hkv] (|q|, |k|, |v|)
-  float *v_scale;  // [B * Hkv]
+  float2 *scales;  // [B * Hkv] factors of the scores and of the output
   int *nan;        // [B * Hkv][4] first key that makes 32 output channels NaN
   __half *qo, *ko, *vo;
   int D, group, q_rows;  // q_rows = Hq / Hkv * Sq
   int64_t cap;
   int len, pad;          // keys, and their rows in ko / vo
   int slices;
-  float q_sign;          // of the scale: the attention kernels want it positive
+  float scale;
 };
 
 __device__ __forceinline__ bool nonfinite(uint32_t pair) {
@@ -166,11 +166,17 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) e[i] = exponent(warp_max(m[i]));
     if (threadIdx.x == 0) {
-      const int a = max(-100, min((e[0] - e[1]) / 2, 100)), v = max(-100, e[2] - 14);  // (at most 114)
-      scale[0] = pow2(-a) * p.q_sign;
-      scale[1] = pow2(a);
-      scale[2] = pow2(-v);
-      if (blockIdx.x == 0) p.v_scale[bh] = pow2(v);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) e[i] = max(-100, e[i] - 14);  // (at most 114)
+      scale[0] = p.scale < 0.f ? -pow2(-e[0]) : pow2(-e[0]);  // (the scores' factor is positive)
+      scale[1] = pow2(-e[1]);
+      scale[2] = pow2(-e[2]);
+      if (blockIdx.x == 0) {
+        // In log2 units.  Not 0, which would turn masked scores into 0 * inf, and finite:
+        // scores reach 2^35.
+        const float s = scalbnf(fabsf(p.scale) * 1.4426950408889634f, e[0] + e[1]);
+        p.scales[bh] = make_float2(fminf(fmaxf(s, 0x1p-120f), 0x1p90f), pow2(e[2]));
+      }
     }
   }
   __syncthreads();
@@ -185,7 +191,8 @@ __global__ void __launch_bounds__(kThreads) attn_q4_operands_kernel(Chunk p) {
       for (int k = 0; k < 4; ++k) {
         float a, b;
         unpack_bf2(w[k], a, b);
-        o[k] = pack_h2(a * f, b * f);
+        // (an infinity makes NaN of a row's scores sooner or later)
+        o[k] = nonfinite(w[k]) ? 0x7fff7fffu : pack_h2(a * f, b * f);
       }
     } else {
       if (nonfinite(x[i].y)) {
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_splits_kernel(F16Extra x, ui
 // Splits of the key tiles and the workspace's parts, in bytes.
 struct Plan {
   int splits, tiles_per_split, pad, slices;
-  int64_t v_scale, nan, ko, vo, qo, part, bytes;
+  int64_t scales, nan, ko, vo, qo, part, bytes;
 };
 Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   Plan pl{};
@@ -257,8 +264,8 @@ Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   // about four CTAs per SM read for the largest values
   const int64_t slices = 4 * int64_t(num_sms()) / bh;
   pl.slices = static_cast<int>(slices < 2 ? 2 : slices > kMaxSlices ? kMaxSlices : slices);
-  pl.v_scale = pl.slices * bh * int64_t(sizeof(float4));
-  pl.nan = pl.v_scale + (bh * int64_t(sizeof(float)) + 15) / 16 * 16;
+  pl.scales = pl.slices * bh * int64_t(sizeof(float4));
+  pl.nan = pl.scales + (bh * int64_t(sizeof(float2)) + 15) / 16 * 16;
   pl.ko = pl.nan + bh * int64_t(sizeof(int4));
   pl.vo = pl.ko + bh * pl.pad * kPad * 2;
   pl.qo = pl.vo + bh * pl.pad * kPad * 2;
@@ -335,7 +342,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
               static_cast<uint32_t *>(const_cast<void *>(v_codes)),
               static_cast<uint32_t *>(const_cast<void *>(v_scales))};
   c.maxima = reinterpret_cast<float4 *>(ws);
-  c.v_scale = reinterpret_cast<float *>(ws + pl.v_scale);
+  c.scales = reinterpret_cast<float2 *>(ws + pl.scales);
   c.nan = reinterpret_cast<int *>(ws + pl.nan);
   c.ko = reinterpret_cast<__half *>(ws + pl.ko);
   c.vo = reinterpret_cast<__half *>(ws + pl.vo);
@@ -347,7 +354,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   c.len = static_cast<int>(kv_len);
   c.pad = pl.pad;
   c.slices = pl.slices;
-  c.q_sign = scale < 0.f ? -1.f : 1.f;
+  c.scale = scale;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const unsigned bh = static_cast<unsigned>(B * Hkv);
   attn_q4_absmax_kernel<<<dim3(pl.slices, bh), kThreads, 0, s>>>(c);
@@ -358,16 +365,14 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
                               0, s, c));
   Q35_LAUNCH_CHECK("attn_q4 operands launch");
   F16Extra x{};
-  x.v_scale = c.v_scale;
+  x.scales = c.scales;
   x.nan = c.nan;
   x.rows = B * Hq * Sq;
   x.splits = pl.splits;
   x.tiles_per_split = pl.tiles_per_split;
   x.D = D;
   x.part = pl.splits > 1 ? reinterpret_cast<float *>(ws + pl.part) : nullptr;
-  // (a scale of 0 would turn masked scores into 0 * inf)
-  st = attn_tc_f16(c.qo, c.ko, c.vo, out, B, Hq, Hkv, Sq, kv_len, c.pad, fmaxf(fabsf(scale), 1e-30f),
-                   causal, x, stream);
+  st = attn_tc_f16(c.qo, c.ko, c.vo, out, B, Hq, Hkv, Sq, kv_len, c.pad, causal, x, stream);
   if (st) return st;
   if (pl.splits > 1) {
     Q35_CHECK_CUDA(launch_early(

@@ -26,8 +26,8 @@
 //
 // Both kernels also come with fp16 operands (kF16), for rows read back from a 4-bit
 // cache (attention_q4_chunk.cu): same tiles, P in fp16, the key tiles optionally cut
-// into splits that leave fp32 partials, a power of two per kv head on the scores and
-// on the output, head_dim 32 and 64 zero-padded to 128.
+// into splits that leave fp32 partials, a factor per kv head on the scores and on
+// the output, head_dim 32 and 64 zero-padded to 128.
 #include <cuda_fp16.h>
 #include <float.h>
 
@@ -127,6 +127,12 @@ template <bool kF16>
 constexpr float kSlack = kF16 ? 4.f : 8.f;
 template <bool kF16>
 constexpr float kLift = kF16 ? 11.f : 0.f;
+// What turns the products of q and k into scores in log2 units.
+template <bool kF16>
+__device__ __forceinline__ float score_scale(const AttnParams &p, int b, int hk) {
+  if constexpr (kF16) return p.x.scales[static_cast<int64_t>(b) * p.Hkv + hk].x;
+  else return p.sl2;
+}
 // The key tiles [j0, j0 + n) of this CTA's split.
 __device__ __forceinline__ int split_tiles(const AttnParams &p, int split, int n_all, int &j0) {
   j0 = split * p.x.tiles_per_split;
@@ -323,6 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
+    const float sl2 = score_scale<kF16>(p, b, hk);
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j & 1;
       if (!sm100::mbar_wait(&s_full[st], (j >> 1) & 1)) {
@@ -357,14 +364,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * p.sl2 > kSlack<kF16>) {
+      } else if ((m_new - m_used) * sl2 > kSlack<kF16>) {
         need = true;
-        alpha = exp2f((m_used - m_new) * p.sl2);
+        alpha = exp2f((m_used - m_new) * sl2);
         m_used = m_new;
         l *= alpha;
       }
       const float mu = (m_used == -INFINITY) ? 0.f : m_used;
-      const float mus = mu * p.sl2 - kLift<kF16>;
+      const float mus = mu * sl2 - kLift<kF16>;
       // O may only be touched once PV_{j-1} has finished.
       if (j >= 1 && !sm100::mbar_wait(o_done, (j - 1) & 1)) {
         report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 307, j, row);
@@ -389,8 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float a = exp2_mufu(fmaf(s[half * 64 + 2 * i], p.sl2, -mus));
-          const float b2 = exp2_fma(fmaf(s[half * 64 + 2 * i + 1], p.sl2, -mus));
+          const float a = exp2_mufu(fmaf(s[half * 64 + 2 * i], sl2, -mus));
+          const float b2 = exp2_fma(fmaf(s[half * 64 + 2 * i + 1], sl2, -mus));
           l += a + b2;
           pk[i] = pack_p<kF16>(a, b2);
         }
@@ -412,8 +419,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::tc_fence_after();
       const bool seen = done && m_used != -INFINITY;
       store_row_f16(p, tmem + lane_base, done, valid, b, h, qi, blockIdx.z,
-                    seen ? m_used * p.sl2 : -FLT_MAX, seen ? l : 0.f,
-                    seen ? p.x.v_scale[static_cast<int64_t>(b) * p.Hkv + hk] : 0.f);
+                    seen ? m_used * sl2 : -FLT_MAX, seen ? l : 0.f,
+                    seen ? p.x.scales[static_cast<int64_t>(b) * p.Hkv + hk].y : 0.f);
     } else {
     uint16_t *orow = p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * 128;
     if (n_tiles > 0 && ok) {
@@ -674,6 +681,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
                           static_cast<int64_t>(j0) * kTile;  // of the split's own keys
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
+    const float sl2 = score_scale<kF16>(p, b, hk);
     for (int j = 0; j < n_tiles; ++j) {
       if (!sm100::mbar_wait(&s_full[hh], j & 1)) {
         report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 326, j, row);
@@ -707,17 +715,17 @@ __global__ void __launch_bounds__(kThreads2, 1)
       float alpha = 1.f;
       if (j == 0 || m_used == -INFINITY) {
         m_used = m_new;
-      } else if ((m_new - m_used) * p.sl2 > kSlack<kF16>) {
+      } else if ((m_new - m_used) * sl2 > kSlack<kF16>) {
         need = true;
-        alpha = exp2f((m_used - m_new) * p.sl2);
+        alpha = exp2f((m_used - m_new) * sl2);
         m_used = m_new;
         l *= alpha;
       }
-      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * p.sl2 - kLift<kF16>;
+      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * sl2 - kLift<kF16>;
       // exponentials, bf16 P over the first 64 S columns.  Score pairs are
       // scaled with one f32x2 FMA; pairs alternate between the MUFU unit
       // (ex2.approx) and the paired FMA polynomial; row sums in f32x2.
-      const float2 sl2v = make_float2(p.sl2, p.sl2), nmus = make_float2(-mus, -mus);
+      const float2 sl2v = make_float2(sl2, sl2), nmus = make_float2(-mus, -mus);
       float2 lsum0 = make_float2(0.f, 0.f), lsum1 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int qtr = 0; qtr < 4; ++qtr) {
@@ -769,8 +777,8 @@ __global__ void __launch_bounds__(kThreads2, 1)
       done = __all_sync(0xffffffffu, done);
       sm100::tc_fence_after();
       const bool seen = done && m_used != -INFINITY;
-      store_row_f16(p, o_tm, done, valid, b, h, qi, blockIdx.y, seen ? m_used * p.sl2 : -FLT_MAX,
-                    seen ? l : 0.f, seen ? p.x.v_scale[static_cast<int64_t>(b) * p.Hkv + hk] : 0.f);
+      store_row_f16(p, o_tm, done, valid, b, h, qi, blockIdx.y, seen ? m_used * sl2 : -FLT_MAX,
+                    seen ? l : 0.f, seen ? p.x.scales[static_cast<int64_t>(b) * p.Hkv + hk].y : 0.f);
     } else {
     uint16_t *orow = p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * 128;
     if (n_tiles > 0 && ok) {
@@ -911,15 +919,14 @@ int attn_tc_ctas(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t *tile_rows) {
 }
 
 int attn_tc_f16(const void *q, const void *k, const void *v, void *out, int64_t B, int Hq, int Hkv,
-                int64_t Sq, int64_t Skv, int64_t kv_cap, float scale, int causal,
-                const F16Extra &x, q35_stream_t stream) {
+                int64_t Sq, int64_t Skv, int64_t kv_cap, int causal, const F16Extra &x,
+                q35_stream_t stream) {
   AttnParams p{};
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.Sq = Sq;
   p.Skv = Skv;
   p.kv_cap = kv_cap;
-  p.scale = scale;
   p.causal = causal ? 1 : 0;
   p.out = static_cast<uint16_t *>(out);
   p.x = x;

@@ -7,7 +7,7 @@
 namespace q35 {
 
 struct F16Extra {
-  const float *v_scale; // [B * Hkv]: what the output is multiplied by
+  const float2 *scales; // [B * Hkv]: the scale in log2 units, what the output is multiplied by
   const int *nan;       // [B * Hkv][4]: first key that makes 32 output channels NaN each
   float *part;          // fp32 partials [rows, splits, D], then (m, l) [rows, splits]; or null
   int64_t rows;         // B * Hq * Sq
@@ -20,7 +20,7 @@ int attn_tc_ctas(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t *tile_rows);
 // q [B,Hq,Sq,128], k / v [B,Hkv,kv_cap,128] fp16 (channels behind D zero, rows behind
 // Skv finite), out token-major bf16 [B,Sq,Hq*D] unless x.part takes partials.
 int attn_tc_f16(const void *q, const void *k, const void *v, void *out, int64_t B, int Hq, int Hkv,
-                int64_t Sq, int64_t Skv, int64_t kv_cap, float scale, int causal,
-                const F16Extra &x, q35_stream_t stream);
+                int64_t Sq, int64_t Skv, int64_t kv_cap, int causal, const F16Extra &x,
+                q35_stream_t stream);
 
 }  // namespace q35

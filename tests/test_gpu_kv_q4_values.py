@@ -89,3 +89,44 @@ def test_the_largest_values_come_through(monkeypatch, chunk):
     d = 2.0 ** -11 * D ** -0.5 * float((q.double().abs().amax((0, 1, 2)) * kk.abs().amax((0, 1, 2))).sum())
     tol = A * (2 ** -10 + math.expm1(2 * (d + 2.0 ** -13))) + 2 ** -8 * ref.abs()
     assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+@pytest.mark.parametrize("chunk", [True])
+@pytest.mark.parametrize("q_log2,k_log2", [(20, 20), (70, 40), (-60, 90), (-60, -30), (40, -90), (0, 110)])
+def test_queries_and_keys_of_every_size(monkeypatch, chunk, q_log2, k_log2):
+    """Powers of two on the queries and the keys that the scale takes back change nothing:
+    the same call without them has the same products.  (In a chunk bit for bit; on the
+    codes a product may meet fp32's smallest numbers.)"""
+    force(monkeypatch, chunk)
+    B, Hq, Hkv, Sq, kv, D, group = 1, 4, 2, 24, 300, 64, 32
+    cache, kk, vv = filled_cache(B, Hkv, 304, D, group, 137, 0.5)
+    q = rows((B, Hq, Sq, D), 138, 0.5)
+    scale = 2.0 ** -3
+    want = K().attention_cache_q4(q.to(DEV), *cache, kv, scale, True)
+    q2 = (q.double() * 2.0 ** q_log2).bfloat16().to(DEV)
+    ks = (cache[1].double() * 2.0 ** k_log2).bfloat16()
+    got = K().attention_cache_q4(q2, cache[0], ks, *cache[2:], kv, scale * 2.0 ** -(q_log2 + k_log2), True)
+    if chunk:
+        assert torch.equal(got, want)
+        return
+    got, (ref, A) = got.double().cpu(), R.attention(q, kk, vv, [kv], scale, True)
+    d = 2.0 ** -19 * scale * float((q.double().abs().amax((0, 1, 2)) * kk.abs().amax((0, 1, 2))).sum()) * 20
+    tol = A * (2 ** -10 + math.expm1(2 * d + 2.0 ** -20)) + 2 ** -8 * ref.abs() + 2 ** -14 * float(vv.abs().max())
+    assert ((got - ref).abs() <= tol).all(), float(((got - ref).abs() / tol).max())
+
+
+@pytest.mark.parametrize("chunk", [True, False])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_nonfinite_query_spoils_its_own_row_only(monkeypatch, chunk, bad):
+    force(monkeypatch, chunk)
+    for Hq, Hkv in ((4, 2), (3, 3)):
+        B, Sq, kv, D, group = 1, 9, 140, 64, 32
+        cache, _, _ = filled_cache(B, Hkv, 144, D, group, 139, 0.5)
+        q = rows((B, Hq, Sq, D), 140, 0.5).to(DEV)
+        q[0, 1, 3, 37] = 0
+        want = K().attention_cache_q4(q, *cache, kv, 0.125, True).view(Sq, Hq, D)
+        q[0, 1, 3, 37] = bad
+        got = K().attention_cache_q4(q, *cache, kv, 0.125, True).view(Sq, Hq, D)
+        assert got[3, 1].isnan().all()
+        got[3, 1] = want[3, 1]
+        assert torch.equal(got, want)
