@@ -500,10 +500,11 @@ Q35_API int q35_kv_read_q4(const void *k_codes, const void *k_scales, const void
  * kv head (a decode step, drafted tokens).  causal != 0: query s sees keys
  * <= s + len - Sq.  A query that sees no key gives zeros.  A kv_lens entry
  * outside [0, kv_len] is clamped and recorded as a device error (code 2, site
- * 311).  Scores need |q| < 2^75.  Weights and values are rounded to 11 bits, values at
- * most to 2^-15 of the largest scale of their row; rows a query sees need |v| between
- * 2^-60 and 2^100 (beyond: rounded to 0, or infinite).  A NaN reaches the queries that
- * see its row only.  workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.  */
+ * 311).  Scores need |q| < 2^100, and lose bits of queries 2^-100 of the largest among
+ * their kv head's.  Weights and values are rounded to 11 bits, values at most to 2^-15 of
+ * the largest scale of their row; rows a query sees need |v| between 2^-60 and 2^100
+ * (beyond: rounded to 0, or infinite).  A NaN reaches the queries that see its row only.
+ * workspace: fp32 scratch of q35_attn_q4_workspace(...) floats.             */
 Q35_API int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D);
 Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_scales,
@@ -515,9 +516,9 @@ Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_sc
 /* The same for many query rows per kv head (a chunk of a prompt), all sequences of
  * kv_len >= 1 rows: the rows go through scaled fp16 copies in the workspace
  * (q35_attn_q4_chunk_workspace(...) bytes, 16-byte aligned) and the tensor-memory
- * attention kernels.  B * Hq <= 65535.  Per kv head, queries and keys lose bits once
- * they are 2^-27 of the largest of their head's rows, values 2^-38 of it, rows that a
- * query does not see included.                                              */
+ * attention kernels.  B * Hq <= 65535.  Per kv head, queries, keys and values lose
+ * bits once they are 2^-27 of the largest of their head's rows and are 0 at 2^-39 of
+ * it, rows that a query does not see included.                              */
 Q35_API int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D); /* 1: estimated faster than q35_attn_q4_fwd */
 Q35_API int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64_t Sq,

@@ -18,11 +18,12 @@
 // four codes of a word.  The powers of two go into the other operand.
 //
 // Scores.  With K = m + s c per group j, q . K = sum_j s_j (Q_j . c_j) + m_j sum(Q_j).
-// Q is scaled by 2^52 (codes at bit 0) or 2^48 (at bit 4), so a product is
-// 2^-81 Q . c; the minima go through one more matrix instruction whose other
-// operand is 2^-81 sum(Q_j) split into three bf16 parts (24 bits).  So K is never
-// rounded, and the scale costs one fp32 operation per key, query and group.
-// |Q| must stay below 2^75.
+// Q is scaled by 2^X, which brings the largest of a group's queries into [2^60, 2^61)
+// (X at most 75, so queries below 2^-15 are left smaller), and by 2^52 (codes at bit 0)
+// or 2^48 (at bit 4), so a product is 2^(X-81) Q . c; the minima go through one more
+// matrix instruction whose other operand is 2^(X-81) sum(Q_j) split into three bf16 parts
+// (24 bits).  So K is never rounded, and the scale costs one fp32 operation per key,
+// query and group.  Queries 2^-100 of their group's largest lose bits; |Q| < 2^100.
 //
 // Keys are the 16 rows of the instruction and queries its 8 columns (S^T = K Q^T,
 // O^T = V^T P^T): a decode step has G = Hq/Hkv queries per kv head, often 8, and
@@ -432,7 +433,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
   const int vsw = D == 128 ? (vrow >> 1) & 3 : D == 64 ? (vrow >> 2) & 1 : 0;
   const int vch = D == 32 ? 0 : lane >> 4;
   const int gv = (D == 128 ? g >> 1 : D == 64 ? (g >> 1) & 1 : 0) / BPG;  // the lane's V scale group
-  const float scale_up = p.scale_log2 * 0x1p81f;
   uint32_t stage = 0;
 
   for (int at = lo; at < hi;) {
@@ -450,8 +450,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
     // Query rows: row r -> head hk G + r / Sq, position r % Sq.  Column g of an
     // operand tile holds 8 channels of every 32; accumulator columns are 2t, 2t + 1.
     uint32_t qf[NT][J][4];
-    uint32_t qm[NT][2];  // 2^-81 sum(Q_t) of group t in three bf16 parts
+    uint32_t qm[NT][2];  // 2^(X-81) sum(Q_t) of group t in three bf16 parts
     int lim[NT][2];      // keys the column's query sees
+    uint32_t top = 0u;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = (rg * NT + nt) * 8 + g;
@@ -460,21 +461,36 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
         const int h = r / p.Sq, s = r - h * p.Sq;
         src = p.q + ((int64_t(b) * p.Hq + hk * p.G + h) * p.Sq + s) * D;
       }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const uint4 x = src ? *reinterpret_cast<const uint4 *>(src + 32 * j + 8 * t)
+                            : make_uint4(0u, 0u, 0u, 0u);
+        qf[nt][j][0] = x.x, qf[nt][j][1] = x.y, qf[nt][j][2] = x.z, qf[nt][j][3] = x.w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max_abs2(top, qf[nt][j][i]);
+      }
+    }
+    // (an infinite query spoils its own row; the others' power of two goes by the rest)
+    const uint32_t e0 = top >> 7 & 0xffu, e1 = top >> 23 & 0xffu;
+    const int e = __reduce_max_sync(0xffffffffu, max(e0 == 255u ? 0u : e0, e1 == 255u ? 0u : e1));
+    const int up_by = max(-60, min(187 - e, 75));  // X
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 52 + up_by) << 23);
+    const float scale_up = p.scale_log2 * 0x1p20f *
+                           __uint_as_float(static_cast<uint32_t>(127 + 61 - up_by) << 23);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       float sum[NS];
 #pragma unroll
       for (int j = 0; j < NS; ++j) sum[j] = 0.f;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const uint4 x = src ? *reinterpret_cast<const uint4 *>(src + 32 * j + 8 * t)
-                            : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float lo, hi;
-          unpack_bf2(xs[i], lo, hi);
+          unpack_bf2(qf[nt][j][i], lo, hi);
           sum[j / BPG] += lo + hi;
-          const float up = i % 2 == 0 ? 0x1p52f : 0x1p48f;
-          qf[nt][j][i] = pack_bf2(lo * up, hi * up);
+          const float f = i % 2 == 0 ? up : up * 0x1p-4f;
+          qf[nt][j][i] = pack_bf2(lo * f, hi * f);
         }
       }
       float mine = 0.f;
@@ -483,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
         float v = sum[j];
         v += __shfl_xor_sync(0xffffffffu, v, 1);
         v += __shfl_xor_sync(0xffffffffu, v, 2);
-        if (j == t) mine = v * 0x1p-81f;
+        if (j == t) mine = v * (up * 0x1p-133f);
       }
       const float h0 = bf2f(f2bf(mine)), h1 = bf2f(f2bf(mine - h0));
       qm[nt][0] = pack_bf2(h0, h1);

@@ -91,7 +91,7 @@ def test_the_largest_values_come_through(monkeypatch, chunk):
     assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
 
 
-@pytest.mark.parametrize("chunk", [True])
+@pytest.mark.parametrize("chunk", [True, False])
 @pytest.mark.parametrize("q_log2,k_log2", [(20, 20), (70, 40), (-60, 90), (-60, -30), (40, -90), (0, 110)])
 def test_queries_and_keys_of_every_size(monkeypatch, chunk, q_log2, k_log2):
     """Powers of two on the queries and the keys that the scale takes back change nothing:
