@@ -687,7 +687,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
             o[i][nt][3] *= a1;
           }
         }
-        const float mu0 = row_m[nt][0] - kLift, mu1 = row_m[nt][1] - kLift;
+        // rounded up: scores whose fp32 step is above 1 must not lift a weight past fp16
+        const float mu0 = __fadd_ru(row_m[nt][0], -kLift), mu1 = __fadd_ru(row_m[nt][1], -kLift);
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           const float p0 = exp2_fast(s[mt][nt][0] - mu0), p1 = exp2_fast(s[mt][nt][1] - mu1);

@@ -130,3 +130,25 @@ def test_a_nonfinite_query_spoils_its_own_row_only(monkeypatch, chunk, bad):
         assert got[3, 1].isnan().all()
         got[3, 1] = want[3, 1]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("chunk,log2", [(c, x) for c in (True, False) for x in (20, 23, 24, 25, 26)]
+                         + [(False, x) for x in (28, 33, 60)])
+@pytest.mark.parametrize("part", [0.5, 0.625, 0.75, 0.9375])
+def test_scores_of_many_millions(monkeypatch, chunk, log2, part):
+    """Keys 3 and 77 have the same score, part * 2^log2, all others its negative: the
+    output is the mean of their values (all operands and sums are exact)."""
+    force(monkeypatch, chunk)
+    B, Hq, Hkv, Sq, kv, D, group = 1, 4, 2, 3, 140, 64, 32
+    cache, _, vv = filled_cache(B, Hkv, 144, D, group, 141, 0.5)
+    cache[3][:, :, 77] = cache[3][:, :, 3]  # (values of one size)
+    vv = R.values(cache[2], cache[3])
+    cache[1][..., 0], cache[1][..., 1] = 0, -1
+    cache[1][:, :, 3, :, 1] = cache[1][:, :, 77, :, 1] = 1
+    q = torch.full((B, Hq, Sq, D), part * 2.0 ** (log2 - 6), dtype=torch.bfloat16, device=DEV)
+    out = K().attention_cache_q4(q, *cache, kv, 1.0, False).double().cpu().view(Sq, Hkv, 2, D)
+    pair = vv[0][:, [3, 77]]
+    ref, A = pair.mean(1)[None, :, None], pair.abs().mean(1)[None, :, None]
+    # weights and values 2^-11 each, values at most 2^-15 of the largest scale; the output
+    tol = A * 2 ** -10 + 2 ** -15 * float(cache[3][:, :, 3, :, 0].max()) + 2 ** -8 * ref.abs()
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
