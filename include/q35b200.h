@@ -518,7 +518,7 @@ Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_sc
  * (q35_attn_q4_chunk_workspace(...) bytes, 16-byte aligned) and the tensor-memory
  * attention kernels.  B * Hq <= 65535.  Per kv head, queries, keys and values lose
  * bits once they are 2^-27 of the largest of their head's rows and are 0 at 2^-39 of
- * it, rows that a query does not see included.                              */
+ * it, rows that a query does not see included.  Scores: |scale q.k| < 2^27. */
 Q35_API int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D); /* 1: estimated faster than q35_attn_q4_fwd */
 Q35_API int64_t q35_attn_q4_chunk_workspace(int64_t B, int Hq, int Hkv, int64_t Sq,

@@ -127,6 +127,13 @@ template <bool kF16>
 constexpr float kSlack = kF16 ? 4.f : 8.f;
 template <bool kF16>
 constexpr float kLift = kF16 ? 11.f : 0.f;
+// What is taken from a row's scores (log2 units) in front of the exponential.  fp16:
+// rounded up, or scores whose fp32 step is above 1 (2^24 and more) would lift a weight
+// past 65504; up to 2^28 a step is at most 16 and the largest weight at least 2^-5.
+template <bool kF16>
+__device__ __forceinline__ float weight_base(float m, float sl2) {
+  return kF16 ? __fmaf_ru(m, sl2, -kLift<kF16>) : m * sl2;
+}
 // What turns the products of q and k into scores in log2 units.
 template <bool kF16>
 __device__ __forceinline__ float score_scale(const AttnParams &p, int b, int hk) {
@@ -371,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= alpha;
       }
       const float mu = (m_used == -INFINITY) ? 0.f : m_used;
-      const float mus = mu * sl2 - kLift<kF16>;
+      const float mus = weight_base<kF16>(mu, sl2);
       // O may only be touched once PV_{j-1} has finished.
       if (j >= 1 && !sm100::mbar_wait(o_done, (j - 1) & 1)) {
         report_error(p.err, DEV_ERR_WAIT_TIMEOUT, 307, j, row);
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
         m_used = m_new;
         l *= alpha;
       }
-      const float mus = ((m_used == -INFINITY) ? 0.f : m_used) * sl2 - kLift<kF16>;
+      const float mus = weight_base<kF16>((m_used == -INFINITY) ? 0.f : m_used, sl2);
       // exponentials, bf16 P over the first 64 S columns.  Score pairs are
       // scaled with one f32x2 FMA; pairs alternate between the MUFU unit
       // (ex2.approx) and the paired FMA polynomial; row sums in f32x2.

@@ -152,3 +152,27 @@ def test_scores_of_many_millions(monkeypatch, chunk, log2, part):
     # weights and values 2^-11 each, values at most 2^-15 of the largest scale; the output
     tol = A * 2 ** -10 + 2 ** -15 * float(cache[3][:, :, 3, :, 0].max()) + 2 ** -8 * ref.abs()
     assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+def test_a_chunk_at_scores_whose_steps_exceed_the_slack(monkeypatch):
+    """Key 140, in the second key tile, scores 4 * 0.9 above key 3 in log2 units at about
+    2^25: its weight is not rescaled for and must still fit fp16, whatever the rounding
+    of the running maximum.  Operands and products are exact."""
+    force(monkeypatch, True)
+    B, Hq, Hkv, Sq, kv, D, group = 1, 2, 1, 103, 150, 64, 32
+    cache, _, vv = filled_cache(B, Hkv, 160, D, group, 143, 0.5)
+    cache[1][..., 0], cache[1][..., 1] = 0, -1
+    cache[1][:, :, 3, :, 1] = cache[1][:, :, 140, :, 1] = 1
+    cache[0][:, :, 140] = 0
+    cache[0][:, :, 140, 0] = 1          # channel 0: code 1 of scale 1
+    cache[1][:, :, 140, 0, 0] = 1
+    kk = R.values(cache[0], cache[1])
+    assert kk[0, 0, 140, 0] == 2 and (kk[0, 0, 140, 1:] == 1).all() and (kk[0, 0, 3] == 1).all()
+    q = (2.0 ** 19 * (1 + torch.arange(18, 121) / 128)).bfloat16()[None, None, :, None].repeat(B, Hq, 1, D)
+    q[..., 0] = 4
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, 0.9 * math.log(2), False).double().cpu().view(Sq, Hq, D)
+    w = 2.0 ** 3.6
+    ref = (w * vv[0, 0, 140] + vv[0, 0, 3]) / (w + 1)
+    A = (w * vv[0, 0, 140].abs() + vv[0, 0, 3].abs()) / (w + 1)
+    tol = A * (2 ** -10 + math.expm1(2 ** -12)) + 2 ** -8 * ref.abs()
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
