@@ -636,14 +636,15 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
     if shape != v.shape or shape != (B, Hkv, S, D):
         raise RuntimeError(f"kv_append_q4: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of "
                            f"{(B, Hkv, cap, D)}")
+    rows, first = None, 0
     if isinstance(offset, torch.Tensor):
-        rows, first = _per_sequence(offset, "kv_append_q4.offset", B, dev).data_ptr(), 0
+        rows = _per_sequence(offset, "kv_append_q4.offset", B, dev)
     else:
-        rows, first = None, int(offset)
+        first = int(offset)
     k_strides = _lib.strides_arg(ks)
     _lib.call("q35_kv_append_q4", k.data_ptr(), v.data_ptr(), k_strides,
               k_strides if ks == vs else _lib.strides_arg(vs), k_codes.data_ptr(), k_scales.data_ptr(),
-              v_codes.data_ptr(), v_scales.data_ptr(), B, Hkv, S, D, group, cap, first, rows,
+              v_codes.data_ptr(), v_scales.data_ptr(), B, Hkv, S, D, group, cap, first, _ptr(rows),
               _stream(k_codes))
 
 
@@ -658,15 +659,16 @@ def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Ten
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return kv_read_q4(k_codes, k_scales, v_codes, v_scales, start, length)
+    starts, first = None, 0  # (a copy of strided starts lives as long as the launch needs it)
     if isinstance(start, torch.Tensor):
-        starts, first = _per_sequence(start, "kv_read_q4.start", B, dev).data_ptr(), 0
+        starts = _per_sequence(start, "kv_read_q4.start", B, dev)
     else:
-        starts, first = None, int(start)
+        first = int(start)
     k = torch.empty(B, Hkv, n, D, device=dev, dtype=_BF16)
     v = torch.empty_like(k)
     _lib.call("q35_kv_read_q4", k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-              v_scales.data_ptr(), k.data_ptr(), v.data_ptr(), B, Hkv, n, n, D, group, cap, first, starts,
-              _stream(k_codes))
+              v_scales.data_ptr(), k.data_ptr(), v.data_ptr(), B, Hkv, n, n, D, group, cap, first,
+              _ptr(starts), _stream(k_codes))
     return k, v
 
 
