@@ -941,7 +941,9 @@ __global__ void __launch_bounds__(WARPS * 32) attn_q4_join_kernel(Params p, int 
   }
 }
 
-// Query rows per CTA, and the runs the rounds are cut into.
+// Query rows per CTA, and the runs the rounds are cut into.  All plans go by the
+// device's SMs, not by a thread's limit: what the workspace was asked for is what any
+// launch of the same sizes takes.
 struct Plan {
   int nt, n_rg, runs, per;
   bool scan, join, alone;  // alone: a warp per group
@@ -956,7 +958,7 @@ struct Plan {
 // 8 sequences x 4 kv heads: 512 keys whole 6.7, cut 7.1 us; 1024 keys 10.0 and 8.4; 256
 // sequences: 1024 keys 46 and 49, 4096 keys 151 and 131.
 int round_cost(int64_t ctas, int D) {
-  return (ctas <= num_sms() ? 10 : 20) * (D + 192) / 320;
+  return (ctas <= device_sms() ? 10 : 20) * (D + 192) / 320;
 }
 int64_t join_cost(int64_t rows, bool lens) { return 50 + rows / 32 + (lens ? 16 : 0); }
 // Query rows of a group, in eights.  16 rows unpack a key once for two instructions, but
@@ -967,7 +969,7 @@ int64_t join_cost(int64_t rows, bool lens) { return 50 + rows / 32 + (lens ? 16 
 // 12.3 / 16.9 and 13.7 / 16.5.
 int rows_per_group(int64_t heads, int64_t R, int64_t rounds, int D) {
   auto run = [&](int nt) {
-    const int64_t slots = int64_t(num_sms()) * ctas_per_sm(D, nt);
+    const int64_t slots = int64_t(device_sms()) * ctas_per_sm(D, nt);
     return (heads * ((R + 8 * nt - 1) / (8 * nt)) * rounds + slots - 1) / slots;
   };
   return 20 * run(1) <= (D == 128 ? 26 : D == 64 ? 33 : 29) * run(2) + 10 ? 1 : 2;
@@ -982,7 +984,7 @@ int plan(Plan &pl, int64_t B, int Hkv, int64_t R, int64_t kv_len, int D, bool le
   if (rounds * B >= lim / (Hkv * n_rg)) return fail(Q35_ERR_SHAPE, "attn_q4: too many key tiles");
   pl.n_rg = static_cast<int>(n_rg);
   const int groups = static_cast<int>(B * Hkv * n_rg), total = groups * rounds;
-  const int slots = num_sms() * ctas_per_sm(D, pl.nt);
+  const int slots = device_sms() * ctas_per_sm(D, pl.nt);
   const int cut = total < slots ? total : slots, cut_per = (total + cut - 1) / cut;
   const int each = (groups + slots - 1) / slots, whole = each * rounds;
   const int64_t cost = int64_t(whole) * round_cost((groups + each - 1) / each, D);

@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(kThreads) attn_q4_splits_kernel(F16Extra x, ui
       make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
 }
 
-// Splits of the key tiles and the workspace's parts, in bytes.
+// Splits of the key tiles and the workspace's parts, in bytes (by the device's SMs, not
+// by a thread's limit: the launch takes what was asked for).
 struct Plan {
   int splits, tiles_per_split, pad, slices;
   int64_t scales, nan, ko, vo, qo, part, bytes;
@@ -254,7 +255,7 @@ Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   const int tiles = static_cast<int>((kv_len + tile - 1) / tile);
   // Splits that fill the SMs once; a split of fewer than 4 tiles costs more to begin
   // and join than it saves.
-  int n = ctas > 0 ? num_sms() / ctas : 1;
+  int n = ctas > 0 ? device_sms() / ctas : 1;
   if (n > tiles / 4) n = tiles / 4;
   if (n < 1) n = 1;
   pl.tiles_per_split = (tiles + n - 1) / n;
@@ -262,7 +263,7 @@ Plan plan(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len, int D) {
   pl.pad = static_cast<int>(tiles * tile);
   const int64_t bh = B * Hkv, rows = B * Hq * Sq;
   // about four CTAs per SM read for the largest values
-  const int64_t slices = 4 * int64_t(num_sms()) / bh;
+  const int64_t slices = 4 * int64_t(device_sms()) / bh;
   pl.slices = static_cast<int>(slices < 2 ? 2 : slices > kMaxSlices ? kMaxSlices : slices);
   pl.scales = pl.slices * bh * int64_t(sizeof(float4));
   pl.nan = pl.scales + (bh * int64_t(sizeof(float2)) + 15) / 16 * 16;
@@ -304,7 +305,7 @@ extern "C" int q35_attn_q4_prefers_chunk(int64_t B, int Hq, int Hkv, int64_t Sq,
   const Plan pl = plan(B, Hq, Hkv, Sq, kv_len, D);
   int64_t tile;
   const double ctas = static_cast<double>(attn_tc_ctas(B, Hq, Hkv, Sq, &tile)) * pl.splits;
-  const double waves = static_cast<double>((static_cast<int64_t>(ctas) + num_sms() - 1) / num_sms());
+  const double waves = static_cast<double>((static_cast<int64_t>(ctas) + device_sms() - 1) / device_sms());
   const double passes = static_cast<double>((Hq / Hkv * Sq + 15) / 16);
   const double keys = static_cast<double>(B) * Hkv * kv_len;
   const double bytes = keys * (1.25 * D + 1024) + static_cast<double>(B) * Hq * Sq * 768;

@@ -57,7 +57,7 @@ int *device_error_word() {
 
 thread_local int g_sm_limit = 0;  // 0: all SMs
 
-int num_sms() {
+int device_sms() {
   int dev = 0;
   if (current_device(&dev) != Q35_OK) return 1;
   if (g_num_sms[dev] == 0) {
@@ -65,7 +65,11 @@ int num_sms() {
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     g_num_sms[dev] = n > 0 ? n : 1;
   }
-  const int hw = g_num_sms[dev];
+  return g_num_sms[dev];
+}
+
+int num_sms() {
+  const int hw = device_sms();
   return (g_sm_limit > 0 && g_sm_limit < hw) ? g_sm_limit : hw;
 }
 

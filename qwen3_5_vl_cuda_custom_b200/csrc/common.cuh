@@ -19,7 +19,9 @@ int cuda_fail(cudaError_t e, const char *what);
 // Device error word of the current device (4 ints: code, site, a, b); lazily
 // allocated once per device, zero-initialised.
 int *device_error_word();
-// Number of SMs of the current device (cached).
+// Number of SMs of the current device (cached): all of them, and within the calling
+// thread's q35_set_sm_limit().
+int device_sms();
 int num_sms();
 // Raises a kernel's dynamic shared-memory limit to `bytes` on the current
 // device, once (cached per device and kernel) so launches inside CUDA-graph

@@ -38,3 +38,53 @@ def test_strided_positions():
     assert torch.equal(out, K().attention_cache_q4(q, *other, table[:, 1].contiguous(), 0.2, False))
     for a, b in zip(cache, other):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+class Scratch:
+    """`n` bytes of scratch with a margin behind them that must stay as it is."""
+
+    def __init__(self, n, margin=1 << 24):
+        self.n = n
+        self.t = torch.full((n + margin,), 0xA5, dtype=torch.uint8, device=DEV)
+
+    def whole(self):
+        return bool((self.t[self.n:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("asked,launched", [(100, 0), (16, 0), (0, 100), (2, 130), (147, 148)])
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,kv,D,group", [
+    (64, 32, 4, 1, 2049, 128, 32), (1, 32, 4, 1, 9000, 128, 64), (3, 16, 2, 2, 5000, 64, 32),
+    (2, 8, 2, 4, 777, 32, 32), (1, 8, 2, 40, 3000, 64, 64),
+])
+def test_scratch_suffices_whatever_the_sm_limits(monkeypatch, asked, launched, B, Hq, Hkv, Sq, kv, D, group):
+    """Through the C interface: scratch sized under one limit, used under another (a
+    margin behind it is larger than any plan's difference)."""
+    from qwen3_5_vl_cuda_custom_b200 import _lib
+    cap = -(-kv // 16) * 16
+    cache = [torch.randint(0, 256, (B, Hkv, cap, D // 2), dtype=torch.uint8, device=DEV) if i % 2 == 0 else
+             torch.rand(B, Hkv, cap, D // group, 2, device=DEV).bfloat16() for i in range(4)]
+    q = rows((B, Hq, Sq, D), 155).to(DEV)
+    lens = torch.full((B,), kv, dtype=torch.int32, device=DEV)
+    outs = [torch.full((B, Sq, Hq * D), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(3)]
+    stream = torch.cuda.current_stream().cuda_stream
+    ptrs = [q.data_ptr()] + [t.data_ptr() for t in cache]
+    try:
+        _lib.call("q35_set_sm_limit", asked)
+        size = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, kv, D)
+        chunk_size = _lib.query("q35_attn_q4_chunk_workspace", B, Hq, Hkv, Sq, kv, D)
+        _lib.call("q35_set_sm_limit", launched)
+        assert size == _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, kv, D)
+        assert chunk_size == _lib.query("q35_attn_q4_chunk_workspace", B, Hq, Hkv, Sq, kv, D)
+        scratch = [Scratch(4 * size), Scratch(4 * size), Scratch(chunk_size)]
+        for i, p in enumerate((None, lens.data_ptr())):
+            _lib.call("q35_attn_q4_fwd", *ptrs, outs[i].data_ptr(), B, Hq, Hkv, Sq, kv, p, cap, D, group, 0.1,
+                      1, scratch[i].t.data_ptr(), stream)
+        _lib.call("q35_attn_q4_chunk_fwd", *ptrs, outs[2].data_ptr(), B, Hq, Hkv, Sq, kv, cap, D, group, 0.1, 1,
+                  scratch[2].t.data_ptr(), stream)
+    finally:
+        _lib.call("q35_set_sm_limit", 0)
+    assert all(s.whole() for s in scratch)
+    for out, chunk, n in ((outs[0], False, kv), (outs[1], False, lens), (outs[2], True, kv)):
+        monkeypatch.setattr(K(), "_q4_chunk", lambda *a: chunk)
+        assert torch.isfinite(out).all()
+        assert torch.equal(out, K().attention_cache_q4(q, *cache, n, 0.1, True, kv))
