@@ -689,10 +689,11 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     length per sequence, at most ``max_kv_len`` (the capacity if not given); it
     is read on the device, so such a call can be captured once and replayed as
     the lengths grow.  Causal masking is aligned to each sequence's last row; a
-    query that sees no row gives zeros.  Decode-shaped calls run on the codes;
-    with an int ``kv_len`` a chunk of a prompt goes through a temporary fp16 copy
-    of the rows (256 bytes of K and V each per row) and the tensor-memory
-    attention kernels."""
+    query that sees no row gives zeros.  Decode-shaped calls run on the codes; with
+    an int ``kv_len`` a chunk of a prompt goes through a temporary fp16 copy of the
+    rows (512 bytes of K and V per row and kv head, against 160 stored at head_dim 128)
+    and the tensor-memory attention kernels, unless there is no memory for the copy;
+    with a length per sequence chunks run on the codes too."""
     B, Hkv, cap, D, group = _cache_q4("attention_cache_q4", k_codes, k_scales, v_codes, v_scales)
     dev = k_codes.device
     if torch.cuda.current_device() != dev.index:  # plans and workspaces are per device
@@ -719,16 +720,20 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     out = torch.empty(B, Sq, Hq * D, device=dev, dtype=_BF16)
     if lens is None and _q4_chunk(B, Hq, Hkv, Sq, n, D):
         w = _lib.query("q35_attn_q4_chunk_workspace", B, Hq, Hkv, Sq, n, D)
-        ws = torch.empty(max(w, 16), device=dev, dtype=torch.uint8)
-        _lib.call("q35_attn_q4_chunk_fwd", at, k_codes.data_ptr(), k_scales.data_ptr(),
-                  v_codes.data_ptr(), v_scales.data_ptr(), out.data_ptr(), B, Hq, Hkv, Sq, n, cap, D,
-                  group, float(scale), 1 if causal else 0, ws.data_ptr(), _stream(q))
-    else:
-        w = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, n, D)
-        ws = torch.empty(w, device=dev, dtype=torch.float32) if w > 0 else None
-        _lib.call("q35_attn_q4_fwd", at, k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-                  v_scales.data_ptr(), out.data_ptr(), B, Hq, Hkv, Sq, n, _ptr(lens), cap, D, group,
-                  float(scale), 1 if causal else 0, _ptr(ws), _stream(q))
+        try:
+            ws = torch.empty(max(w, 16), device=dev, dtype=torch.uint8)
+        except torch.OutOfMemoryError:
+            ws = None  # 512 bytes a row and kv head: the form on the codes needs next to none
+        if ws is not None:
+            _lib.call("q35_attn_q4_chunk_fwd", at, k_codes.data_ptr(), k_scales.data_ptr(),
+                      v_codes.data_ptr(), v_scales.data_ptr(), out.data_ptr(), B, Hq, Hkv, Sq, n, cap,
+                      D, group, float(scale), 1 if causal else 0, ws.data_ptr(), _stream(q))
+            return out
+    w = _lib.query("q35_attn_q4_workspace", B, Hq, Hkv, Sq, n, D)
+    ws = torch.empty(w, device=dev, dtype=torch.float32) if w > 0 else None
+    _lib.call("q35_attn_q4_fwd", at, k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+              v_scales.data_ptr(), out.data_ptr(), B, Hq, Hkv, Sq, n, _ptr(lens), cap, D, group,
+              float(scale), 1 if causal else 0, _ptr(ws), _stream(q))
     return out
 
 

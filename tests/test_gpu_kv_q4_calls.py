@@ -88,3 +88,24 @@ def test_scratch_suffices_whatever_the_sm_limits(monkeypatch, asked, launched, B
         monkeypatch.setattr(K(), "_q4_chunk", lambda *a: chunk)
         assert torch.isfinite(out).all()
         assert torch.equal(out, K().attention_cache_q4(q, *cache, n, 0.1, True, kv))
+
+
+def test_a_chunk_without_memory_for_its_copy_runs_on_the_codes(monkeypatch):
+    B, Hq, Hkv, Sq, kv, D, group = 1, 16, 8, 40, 65536, 64, 64
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: True)
+    cache, _, _ = filled_cache(B, Hkv, 1024, D, group, 157)
+    cache = [t.repeat(1, 1, kv // 1024, *[1] * (t.dim() - 3)) for t in cache]
+    q = rows((B, Hq, Sq, D), 158).to(DEV)
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: False)
+    want = K().attention_cache_q4(q, *cache, kv, 0.125, True)
+    monkeypatch.setattr(K(), "_q4_chunk", lambda *a: True)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    try:  # room for 64 MB more than what is held; the copy takes 268 MB
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / total)
+        got = K().attention_cache_q4(q, *cache, kv, 0.125, True)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert torch.equal(got, want)
+    assert not torch.equal(K().attention_cache_q4(q, *cache, kv, 0.125, True), want)  # the other form
