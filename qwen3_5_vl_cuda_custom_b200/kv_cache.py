@@ -57,6 +57,11 @@ class LayerKVCache:
         self.length = Sk
         return out
 
+    @property
+    def empty(self) -> bool:
+        """Whether no sequence holds a row (known on the host)."""
+        return self.length == 0
+
     def _room(self, S: int) -> int:
         if self.length + S > self.capacity:
             raise RuntimeError(f"KV cache full: {self.length} + {S} > {self.capacity}")
@@ -116,6 +121,7 @@ class Q4LayerKVCache(LayerKVCache):
         self.v_scales = torch.zeros_like(self.k_scales)
         self._length = 0
         self._lengths: torch.Tensor | None = None
+        self._empty = True  # of the sequences behind _lengths
 
     @property
     def capacity(self) -> int:
@@ -131,6 +137,10 @@ class Q4LayerKVCache(LayerKVCache):
         if self.lengths is not None:
             raise RuntimeError("this cache keeps a length per sequence: use set_lengths")
         self._length = n
+
+    @property
+    def empty(self) -> bool:
+        return self._length == 0 if self.lengths is None else self._empty
 
     @property
     def buffers(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -149,6 +159,7 @@ class Q4LayerKVCache(LayerKVCache):
             self._lengths = torch.empty(B, device=self.k_codes.device, dtype=torch.int32)
         # always the same tensor: captured graphs read and advance it
         self._lengths.copy_(lengths)
+        self._empty = hi == 0
         self.lengths = self._lengths
 
     def read(self, start: int, length: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -169,6 +180,7 @@ class Q4LayerKVCache(LayerKVCache):
         if self.lengths is not None:
             K.kv_append_q4(k, v, *self.buffers, self.lengths)
             self.lengths.add_(S)
+            self._empty = self._empty and S == 0
             return K.attention_cache_q4(q, *self.buffers, self.lengths, scale, causal)
         past, Sk = self._length, self._room(S)
         K.kv_append_q4(k, v, *self.buffers, past)
@@ -180,13 +192,14 @@ class Q4LayerKVCache(LayerKVCache):
         return out
 
     def save_length(self):
-        return self._length if self.lengths is None else self.lengths.clone()
+        return self._length if self.lengths is None else (self.lengths.clone(), self._empty)
 
     def restore_length(self, saved) -> None:
         if self.lengths is None:
             self._length = saved
         else:
-            self.lengths.copy_(saved)
+            self.lengths.copy_(saved[0])
+            self._empty = saved[1]
 
     def reset(self) -> None:
         self.lengths = None

@@ -261,10 +261,7 @@ class CudaFullAttention(nn.Module):
         if isinstance(past_kv, LayerKVCache):
             # preallocated cache: append in place, attend over the buffers
             cache = past_kv
-            if self.reference_chunk_mask:
-                causal = cache.lengths is None and cache.length == 0
-            else:
-                causal = S > 1
+            causal = cache.empty if self.reference_chunk_mask else S > 1
             out = cache.append_attend(q, k, v, self.scale, causal)
             return self.o_proj(out, residual=residual, out_dtype=out_dtype), cache
         if past_kv is not None:

@@ -42,3 +42,44 @@ def test_a_copy_of_the_positions_lives_until_the_launch(monkeypatch, name):
     else:
         K.attention_cache_q4(x, *cache, at, 1.0, False)
     assert seen == [[True]]
+
+
+def test_the_reference_mask_over_caches_with_lengths(monkeypatch):
+    """reference_chunk_mask: causal on an empty cache, no mask behind rows; also when the
+    lengths are on the device, and in the warm-up and the capture of one step."""
+    from qwen3_5_vl_cuda_custom_b200.kv_cache import LayerKVCache, Q4LayerKVCache
+    from qwen3_5_vl_cuda_custom_b200.modules import CudaFullAttention
+
+    class Seen(Exception):
+        pass
+
+    attn = CudaFullAttention(64, 2, 1, 32)
+    attn.reference_chunk_mask = True
+    x = torch.zeros(2, 3, 64)
+    monkeypatch.setattr(attn, "_project", lambda x, m: (x, x, x))
+
+    def mask(cache):
+        def append_attend(q, k, v, scale, causal):
+            raise Seen(causal)
+        with monkeypatch.context() as m, pytest.raises(Seen) as e:
+            m.setattr(cache, "append_attend", append_attend)
+            attn(x, None, past_kv=cache)
+        return e.value.args[0]
+
+    for cache in (LayerKVCache(2, 1, 16, 32, "cpu"), Q4LayerKVCache(2, 1, 16, 32, "cpu")):
+        assert mask(cache) is True
+        cache.length = 3
+        assert mask(cache) is False
+    cache.set_lengths(torch.tensor([0, 4]))
+    assert mask(cache) is False
+    cache.set_lengths(torch.tensor([0, 0]))
+    assert mask(cache) is True
+    saved = cache.save_length()
+    monkeypatch.setattr(K, "kv_append_q4", lambda *a: None)
+    monkeypatch.setattr(K, "attention_cache_q4", lambda *a, **k: None)
+    cache.append_attend(x[:, None, :, :32], x[:, None, :, :32], x[:, None, :, :32], 1.0, True)
+    assert cache.lengths.tolist() == [3, 3] and mask(cache) is False
+    cache.restore_length(saved)
+    assert cache.lengths.tolist() == [0, 0] and mask(cache) is True
+    cache.reset()
+    assert mask(cache) is True
