@@ -92,15 +92,17 @@ class Q4LayerKVCache(LayerKVCache):
     ``group_size`` channels (32, 64 or 128; smaller groups are more exact:
     0.31 / 0.28 / 0.27 of the bf16 bytes at head_dim 128).
 
-    The first chunk of an empty cache attends over its own exact k/v; later
-    calls attend over the stored rows, their own included.
+    A first chunk of two tokens or more attends over its own exact k/v (not when a
+    length per sequence was set before it); later calls, and a first chunk of one
+    token, attend over the stored rows, their own included.
 
     ``set_lengths(lengths)`` switches to a length per sequence, held on the
     device in ``lengths``: appends go behind each sequence's own rows and
     attention stops at them.  The usual way is a right-padded prompt batch,
     then ``set_lengths`` with the prompts' true lengths.  Nothing checks the
-    capacity on the host then; rows that do not fit are left out and recorded
-    as a device error (``kernels.device_error_check``)."""
+    capacity on the host then; a step that passes it attends over the rows within
+    it and is recorded as a device error (``kernels.device_error_check``), while
+    ``lengths`` goes on counting until ``set_lengths`` or ``reset``."""
 
     def __init__(self, batch: int, num_kv_heads: int, capacity: int, head_dim: int, device,
                  group_size: int = 32):
@@ -181,7 +183,8 @@ class Q4LayerKVCache(LayerKVCache):
             K.kv_append_q4(k, v, *self.buffers, self.lengths)
             self.lengths.add_(S)
             self._empty = self._empty and S == 0
-            return K.attention_cache_q4(q, *self.buffers, self.lengths, scale, causal)
+            return K.attention_cache_q4(q, *self.buffers, self.lengths, scale, causal,
+                                        max_kv_len=self.capacity)
         past, Sk = self._length, self._room(S)
         K.kv_append_q4(k, v, *self.buffers, past)
         if past == 0 and S > 1:

@@ -109,3 +109,31 @@ def test_a_chunk_without_memory_for_its_copy_runs_on_the_codes(monkeypatch):
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert torch.equal(got, want)
     assert not torch.equal(K().attention_cache_q4(q, *cache, kv, 0.125, True), want)  # the other form
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 128)])
+def test_a_cache_with_lengths_ends_at_its_capacity(D, group):
+    """250 rows asked for (256 are held): rows behind them are reported, and queries see
+    the rows within the capacity only."""
+    from qwen3_5_vl_cuda_custom_b200.kv_cache import Q4LayerKVCache
+    B, Hq, Hkv, cap = 3, 4, 2, 250
+    cache = Q4LayerKVCache(B, Hkv, cap, D, DEV, group_size=group)
+    k, v = rows((B, Hkv, cap, D), 161).to(DEV), rows((B, Hkv, cap, D), 162).to(DEV)
+    K().kv_append_q4(k, v, *cache.buffers, 0)
+    cache.set_lengths(torch.tensor([249, 248, 3]))
+    K().device_error_check()
+    for step, over in enumerate((None, 0, 1)):
+        q, x = rows((B, Hq, 1, D), 163 + step).to(DEV), rows((B, Hkv, 1, D), 173 + step).to(DEV)
+        out = cache.append_attend(q, x, x, D ** -0.5, False)
+        if over is None:
+            K().device_error_check()
+        else:
+            with pytest.raises(RuntimeError, match="code 2"):
+                K().device_error_check()
+        lens = torch.tensor([min(n + step + 1, cap) for n in (249, 248, 3)], dtype=torch.int32, device=DEV)
+        assert torch.equal(out, K().attention_cache_q4(q, *cache.buffers, lens, D ** -0.5, False, cap))
+    K().device_error_check()
+    assert cache.length == 252
+    cache.reset()
+    cache.set_lengths(torch.tensor([cap, cap - 1, 0]))
+    assert cache.length == cap
