@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+import kv_q4_cases as C
 import kv_q4_ref as R
 from test_gpu_kv_q4 import DEV, SHAPES, K, filled_cache, rows
 
@@ -176,3 +177,93 @@ def test_a_chunk_at_scores_whose_steps_exceed_the_slack(monkeypatch):
     A = (w * vv[0, 0, 140].abs() + vv[0, 0, 3].abs()) / (w + 1)
     tol = A * (2 ** -10 + math.expm1(2 ** -12)) + 2 ** -8 * ref.abs()
     assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+# ------------------------------------------------------------------ precision
+@pytest.mark.parametrize("chunk", [True, False])
+@pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("n", [2, 90, 1000, 9000])
+def test_weights_and_values_keep_11_bits(monkeypatch, chunk, D, group, n):
+    force(monkeypatch, chunk)
+    for weights, xs in ((True, (0, 1, 2, 5, 17, 40, 63, 100, 127)), (False, (-50, -20, 0, 20, 36))):
+        for x in xs:
+            case = C.weights_case(D, group, n, x) if weights else C.values_case(D, group, n, x)
+            q, cache, scale = case
+            out = K().attention_cache_q4(q.to(DEV), *[t.to(DEV) for t in cache], n, scale, False)
+            ref, tol = C.bounds(case, n, weights)
+            err = (out.double().cpu() - ref).abs()
+            assert (err <= tol).all(), (weights, x, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("D,group,B,Hq,Hkv,Sq,kv,causal", [
+    (128, 32, 2, 32, 4, 100, 333, True), (128, 128, 2, 32, 4, 64, 64, True), (64, 64, 2, 8, 2, 130, 400, True),
+    (32, 32, 2, 6, 2, 128, 100, True),             # the first 28 queries see nothing
+    (128, 64, 2, 32, 4, 40, 129, False), (128, 32, 1, 5, 1, 33, 700, True), (64, 32, 1, 9, 3, 200, 2500, True),
+])
+def test_a_chunk_within_its_roundings(monkeypatch, D, group, B, Hq, Hkv, Sq, kv, causal):
+    """The form for chunks against 64 bits, with bounds per query: keys, weights and values
+    rounded to 2^-11 each, queries exact; scores off by d = (2^-11 + 2^-17) scale
+    max_k sum_d |q_d k_d| (2^-17: fp32 sums of 128 products and the scale) and the
+    exponential's 2^-13; the output's 2^-8.  Rows behind the length hold NaN and
+    infinities."""
+    force(monkeypatch, True)
+    cap = -(-kv // 16) * 16 + 144
+    cache, kk, vv = filled_cache(B, Hkv, cap, D, group, 145, 0.5)
+    for t, bad in ((cache[0], 255), (cache[1], math.nan), (cache[2], 255), (cache[3], math.inf)):
+        t[:, :, kv:] = bad
+    q = rows((B, Hq, Sq, D), 146, 0.5)
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, causal).double().cpu()
+    ref, A = R.attention(q, kk, vv, [kv] * B, D ** -0.5, causal)
+    G = Hq // Hkv
+    size = torch.matmul(q.double().abs().view(B, Hkv, G * Sq, D), kk[:, :, :kv].abs().transpose(-1, -2))
+    size = size.amax(-1).view(B, Hq, Sq).transpose(1, 2)[..., None]  # per query
+    d = (2.0 ** -11 + 2.0 ** -17) * D ** -0.5 * size + 2.0 ** -13
+    tol = A.view(B, Sq, Hq, D) * (2 ** -10 + torch.expm1(2 * d)) + 2 ** -8 * ref.abs().view(B, Sq, Hq, D)
+    err = (out - ref).abs().view(B, Sq, Hq, D)
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("kv", [400, 9000])
+def test_rows_of_zeros_beside_large_values(monkeypatch, kv):
+    """On the codes, values of 0 weigh what others do as long as those stay below 2^40:
+    every second row is 0, the rest 2^39 .. 2^40, weights 1 and 2^-20."""
+    force(monkeypatch, False)
+    B, Hq, Hkv, D, group = 1, 2, 1, 128, 32
+    cache, _, _ = filled_cache(B, Hkv, -(-kv // 16) * 16, D, group, 147, 0.5)
+    cache[0].zero_()                                   # keys: s = 0, m = 0 or -1
+    cache[1][..., 0], cache[1][..., 1] = 0, 0
+    cache[1][:, :, 3::4, :, 1] = -1
+    cache[3][..., 0], cache[3][..., 1] = 2.0 ** 35, 2.0 ** 39
+    cache[3][:, :, ::2] = 0
+    q = torch.full((B, Hq, 1, D), 20 * math.log(2) / D).bfloat16()
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, 1.0, False).double().cpu()
+    ref, A = R.attention(q, R.values(cache[0], cache[1]), R.values(cache[2], cache[3]), [kv], 1.0, False)
+    tol = A * (2 ** -10 + 2 ** -17) + 2 ** -8 * ref.abs()
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+def test_chunks_in_flight_together_and_again(monkeypatch):
+    """Two calls on two streams, replays of a captured one, a NaN key and a NaN value
+    among the rows: the same bits every time."""
+    force(monkeypatch, True)
+    B, Hq, Hkv, Sq, kv, D, group = 2, 8, 2, 60, 3000, 128, 32
+    cache, _, _ = filled_cache(B, Hkv, 3008, D, group, 148)
+    cache[1][0, 1, 2970, 2] = cache[3][1, 0, 2960, 1] = math.nan
+    q = rows((B, Hq, Sq, D), 149).to(DEV)
+    want = K().attention_cache_q4(q, *cache, kv, 0.09, True)
+    bits = want.view(torch.int16)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(K().attention_cache_q4(q, *cache, kv, 0.09, True))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs.append(K().attention_cache_q4(q, *cache, kv, 0.09, True))
+    for _ in range(3):
+        outs[-1].zero_()
+        graph.replay()
+        assert all(torch.equal(o.view(torch.int16), bits) for o in outs)
+    assert want[0].isnan().any() and not want[:, :20].isnan().any()

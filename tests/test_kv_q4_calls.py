@@ -83,3 +83,14 @@ def test_the_reference_mask_over_caches_with_lengths(monkeypatch):
     assert cache.lengths.tolist() == [0, 0] and mask(cache) is True
     cache.reset()
     assert mask(cache) is True
+
+
+@pytest.mark.parametrize("weights", [True, False])
+@pytest.mark.parametrize("x", [0, 5, 40, 100])
+def test_the_precision_cases_tell_8_bits_from_11(weights, x):
+    """What the attention kernels are held to (test_gpu_kv_q4_values.py) excludes weights
+    or values of bf16's 8 bits."""
+    import kv_q4_cases as C
+    case = C.weights_case(64, 32, 90, x) if weights else C.values_case(64, 32, 90, x - 50)
+    ref, tol = C.bounds(case, 90, weights)
+    assert ((C.with_bf16(case, 90, weights) - ref).abs() > 1.2 * tol).all()
