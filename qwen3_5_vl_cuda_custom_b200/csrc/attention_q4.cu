@@ -1044,6 +1044,7 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
   if (kv_len > cap)
     return fail(Q35_ERR_SHAPE, "attn_q4: %lld rows exceed the capacity %lld", (long long)kv_len,
                 (long long)cap);
+  if (const int bad = q4::check_scale("attn_q4", scale)) return bad;
   if (B * Sq == 0) return Q35_OK;
   if (!q || !out) return fail(Q35_ERR_INVALID, "attn_q4: null");
   if (!aligned16(q) || !aligned16(out))

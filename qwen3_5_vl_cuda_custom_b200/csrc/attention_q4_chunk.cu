@@ -328,6 +328,7 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   if (kv_len > cap)
     return fail(Q35_ERR_SHAPE, "attn_q4_chunk: %lld rows exceed the capacity %lld",
                 (long long)kv_len, (long long)cap);
+  if (const int bad = q4::check_scale("attn_q4_chunk", scale)) return bad;
   if (B * Sq == 0) return Q35_OK;
   if (!q || !out || !workspace) return fail(Q35_ERR_INVALID, "attn_q4_chunk: null");
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace))

@@ -45,6 +45,13 @@ inline int check_cache(const char *what, const void *kc, const void *ks, const v
   return Q35_OK;
 }
 
+// The factor of the scores, for both forms of attention: beyond 2^100 (or NaN) one would
+// give NaN and the other finite numbers.
+inline int check_scale(const char *what, float scale) {
+  if (scale >= -0x1p100f && scale <= 0x1p100f) return Q35_OK;
+  return fail(Q35_ERR_INVALID, "%s: scale %g", what, static_cast<double>(scale));
+}
+
 // value = minimum + code * scale, rounded once to fp32 (code * scale is exact:
 // 4 x 8 significant bits).
 __device__ __forceinline__ float value(float code, uint32_t pair) {

@@ -94,3 +94,16 @@ def test_the_precision_cases_tell_8_bits_from_11(weights, x):
     case = C.weights_case(64, 32, 90, x) if weights else C.values_case(64, 32, 90, x - 50)
     ref, tol = C.bounds(case, 90, weights)
     assert ((C.with_bf16(case, 90, weights) - ref).abs() > 1.2 * tol).all()
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 2.0 ** 101, -(2.0 ** 120)])
+def test_scales_out_of_range_are_refused(scale):
+    import ctypes
+    from qwen3_5_vl_cuda_custom_b200 import _lib, build
+    build.build()
+    lib, p = _lib.load(), ctypes.c_void_p(256)  # never dereferenced: validation fails first
+    args = [p] * 6
+    assert lib.q35_attn_q4_fwd(*args, 1, 8, 2, 1, 16, None, 16, 64, 32, scale, 0, p, None) == 1
+    assert "scale" in lib.q35_last_error_message().decode()
+    assert lib.q35_attn_q4_chunk_fwd(*args, 1, 8, 2, 64, 16, 16, 64, 32, scale, 1, p, None) == 1
+    assert "scale" in lib.q35_last_error_message().decode()
