@@ -1019,6 +1019,7 @@ using namespace q35;
 extern "C" int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                          int D) {
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || Sq <= 0 || D <= 0) return 0;
+  if (Sq >= int64_t(1) << 31) return 0;
   if (kv_len < 0 || kv_len >= (int64_t(1) << 31) - 256) return 0;
   int64_t most = 0;  // of the calls with and without kv_lens
   for (int lens = 0; lens < 2; ++lens) {
@@ -1038,14 +1039,14 @@ extern "C" int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k
   const int st = q4::check_cache("attn_q4", k_codes, k_scales, v_codes, v_scales, B, Hkv, D, group,
                                  cap);
   if (st) return st;
-  if (Sq < 0 || kv_len < 0 || Hq <= 0 || Hq % Hkv != 0)
+  if (Sq < 0 || Sq >= int64_t(1) << 31 || kv_len < 0 || Hq <= 0 || Hq % Hkv != 0)
     return fail(Q35_ERR_SHAPE, "attn_q4: Sq %lld, kv_len %lld, Hq %d, Hkv %d", (long long)Sq,
                 (long long)kv_len, Hq, Hkv);
   if (kv_len > cap)
     return fail(Q35_ERR_SHAPE, "attn_q4: %lld rows exceed the capacity %lld", (long long)kv_len,
                 (long long)cap);
   if (const int bad = q4::check_scale("attn_q4", scale)) return bad;
-  if (B * Sq == 0) return Q35_OK;
+  if (B == 0 || Sq == 0) return Q35_OK;
   if (!q || !out) return fail(Q35_ERR_INVALID, "attn_q4: null");
   if (!aligned16(q) || !aligned16(out))
     return fail(Q35_ERR_ALIGN, "attn_q4: q, out not 16-byte aligned");

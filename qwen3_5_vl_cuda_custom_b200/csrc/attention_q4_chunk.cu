@@ -322,14 +322,14 @@ extern "C" int q35_attn_q4_chunk_fwd(const void *q, const void *k_codes, const v
   int st = q4::check_cache("attn_q4_chunk", k_codes, k_scales, v_codes, v_scales, B, Hkv, D, group,
                            cap);
   if (st) return st;
-  if (Sq < 0 || kv_len < 1 || Hq <= 0 || Hq % Hkv != 0)
+  if (Sq < 0 || Sq >= int64_t(1) << 31 || kv_len < 1 || Hq <= 0 || Hq % Hkv != 0)
     return fail(Q35_ERR_SHAPE, "attn_q4_chunk: Sq %lld, kv_len %lld, Hq %d, Hkv %d", (long long)Sq,
                 (long long)kv_len, Hq, Hkv);
   if (kv_len > cap)
     return fail(Q35_ERR_SHAPE, "attn_q4_chunk: %lld rows exceed the capacity %lld",
                 (long long)kv_len, (long long)cap);
   if (const int bad = q4::check_scale("attn_q4_chunk", scale)) return bad;
-  if (B * Sq == 0) return Q35_OK;
+  if (B == 0 || Sq == 0) return Q35_OK;
   if (!q || !out || !workspace) return fail(Q35_ERR_INVALID, "attn_q4_chunk: null");
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace))
     return fail(Q35_ERR_ALIGN, "attn_q4_chunk: q, out or workspace not 16-byte aligned");

@@ -338,10 +338,10 @@ extern "C" int q35_kv_append_q4(const void *k_new, const void *v_new, const int6
                                  group, cap);
   if (st) return st;
   if (S < 0) return fail(Q35_ERR_SHAPE, "kv_append_q4: %lld rows", (long long)S);
-  if (offsets ? S > cap : (offset < 0 || offset + S > cap))
+  if (S > cap || (!offsets && (offset < 0 || offset > cap - S)))
     return fail(Q35_ERR_SHAPE, "kv_append_q4: offset %lld + %lld rows exceed capacity %lld",
                 (long long)(offsets ? 0 : offset), (long long)S, (long long)cap);
-  if (B * S == 0) return Q35_OK;
+  if (B == 0 || S == 0) return Q35_OK;
   if (!k_new || !v_new || !k_strides || !v_strides)
     return fail(Q35_ERR_INVALID, "kv_append_q4: null");
   if (!aligned16(k_new) || !aligned16(v_new))
@@ -352,7 +352,7 @@ extern "C" int q35_kv_append_q4(const void *k_new, const void *v_new, const int6
   int *err = device_error_word();
   if (!err) return fail(Q35_ERR_CUDA, "kv_append_q4: no device error word");
   const int64_t rows = B * Hkv * S, step = kAppendThreads / (D / 16);
-  if (B >= (int64_t(1) << 31) / Hkv || rows >= (int64_t(1) << 30))
+  if (rows >= (int64_t(1) << 30))
     return fail(Q35_ERR_SHAPE, "kv_append_q4: too many rows");
   int64_t ctas = (rows + step - 1) / step;  // per K and V; at most the resident ones
   const int64_t most = (int64_t(num_sms()) * kAppendCtas + 1) / 2;
@@ -389,21 +389,19 @@ extern "C" int q35_kv_read_q4(const void *k_codes, const void *k_scales, const v
   const int st = q4::check_cache("kv_read_q4", k_codes, k_scales, v_codes, v_scales, B, Hkv, D,
                                  group, cap);
   if (st) return st;
-  if (n < 0 || out_cap < n)
+  if (n < 0 || out_cap < n || out_cap >= (int64_t(1) << 31))
     return fail(Q35_ERR_SHAPE, "kv_read_q4: %lld rows into %lld", (long long)n, (long long)out_cap);
-  if (starts ? n > cap : (start < 0 || start + n > cap))
+  if (n > cap || (!starts && (start < 0 || start > cap - n)))
     return fail(Q35_ERR_SHAPE, "kv_read_q4: rows %lld + %lld exceed capacity %lld",
                 (long long)(starts ? 0 : start), (long long)n, (long long)cap);
-  if (B * out_cap == 0) return Q35_OK;
+  if (B == 0 || out_cap == 0) return Q35_OK;
   if (!k_out || !v_out) return fail(Q35_ERR_INVALID, "kv_read_q4: null");
   if (!aligned16(k_out) || !aligned16(v_out))
     return fail(Q35_ERR_ALIGN, "kv_read_q4: outputs not 16-byte aligned");
   int *err = device_error_word();
   if (!err) return fail(Q35_ERR_CUDA, "kv_read_q4: no device error word");
-  if (out_cap >= (int64_t(1) << 31))
-    return fail(Q35_ERR_SHAPE, "kv_read_q4: %lld rows", (long long)out_cap);
   const int64_t rows = B * Hkv * out_cap, step = kThreads / (D / 8);
-  if (B >= (int64_t(1) << 31) / Hkv || rows >= (int64_t(1) << 31) - 4 * step)
+  if (rows >= (int64_t(1) << 31) - 4 * step)
     return fail(Q35_ERR_SHAPE, "kv_read_q4: too many rows");
   const Cache c{static_cast<uint32_t *>(const_cast<void *>(k_codes)),
                 static_cast<uint32_t *>(const_cast<void *>(k_scales)),

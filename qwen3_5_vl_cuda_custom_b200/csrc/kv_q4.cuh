@@ -38,7 +38,9 @@ inline int check_cache(const char *what, const void *kc, const void *ks, const v
                 (long long)B, Hkv, (long long)cap);
   if (cap >= (int64_t(1) << 31) - 256)
     return fail(Q35_ERR_SHAPE, "%s: capacity %lld does not fit 31 bits", what, (long long)cap);
-  if (B * Hkv * cap == 0) return Q35_OK;
+  if (B >= (int64_t(1) << 31) / Hkv)
+    return fail(Q35_ERR_SHAPE, "%s: %lld sequences x %d heads", what, (long long)B, Hkv);
+  if (B == 0 || cap == 0) return Q35_OK;
   if (!kc || !ks || !vc || !vs) return fail(Q35_ERR_INVALID, "%s: null cache pointer", what);
   if (!aligned16(kc) || !aligned16(ks) || !aligned16(vc) || !aligned16(vs))
     return fail(Q35_ERR_ALIGN, "%s: cache pointers not 16-byte aligned", what);

@@ -107,3 +107,27 @@ def test_scales_out_of_range_are_refused(scale):
     assert "scale" in lib.q35_last_error_message().decode()
     assert lib.q35_attn_q4_chunk_fwd(*args, 1, 8, 2, 64, 16, 16, 64, 32, scale, 1, p, None) == 1
     assert "scale" in lib.q35_last_error_message().decode()
+
+
+HUGE = 1 << 62
+
+
+def test_sizes_whose_products_overflow_are_refused():
+    """Nothing wraps to an accepted size, and no plan divides by a wrapped 0."""
+    import ctypes
+    from qwen3_5_vl_cuda_custom_b200 import _lib, build
+    build.build()
+    lib, p = _lib.load(), ctypes.c_void_p(256)  # never dereferenced: validation fails first
+    st = (ctypes.c_int64 * 3)(1024, 512, 64)
+    for B, Sq in ((1, HUGE), (4, HUGE), (2, 1 << 32), (HUGE, 4), (1 << 31, 1)):
+        for Hq, Hkv in ((8, 1), (8, 2), (8, 8)):
+            assert lib.q35_attn_q4_workspace(B, Hq, Hkv, Sq, 16, 64) == 0
+            assert lib.q35_attn_q4_chunk_workspace(B, Hq, Hkv, Sq, 16, 64) == 0
+            assert lib.q35_attn_q4_prefers_chunk(B, Hq, Hkv, Sq, 16, 64) == 0
+            assert lib.q35_attn_q4_fwd(*[p] * 6, B, Hq, Hkv, Sq, 16, None, 16, 64, 32, 0.1, 0, p, None) == 2
+            assert lib.q35_attn_q4_chunk_fwd(*[p] * 6, B, Hq, Hkv, Sq, 16, 16, 64, 32, 0.1, 0, p, None) == 2
+    for B, S, offset in ((1, 4, (1 << 63) - 2), (HUGE, 4, 0), (1 << 60, 16, 0), (1, HUGE, 0), (1 << 31, 1, 0)):
+        assert lib.q35_kv_append_q4(p, p, st, st, p, p, p, p, B, 2, S, 64, 32, 16, offset, None, None) == 2
+        assert lib.q35_kv_read_q4(p, p, p, p, p, p, B, 2, S, S, 64, 32, 16, offset, None, None) == 2
+    for out_cap in (HUGE, 1 << 31):
+        assert lib.q35_kv_read_q4(p, p, p, p, p, p, 4, 2, 4, out_cap, 64, 32, 16, 0, None, None) == 2
