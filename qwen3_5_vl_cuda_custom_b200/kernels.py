@@ -589,6 +589,13 @@ def _per_sequence(t: torch.Tensor, name: str, B: int, device) -> torch.Tensor:
     return t
 
 
+def _first_row(name: str, row, cap: int) -> int:
+    row = int(row)
+    if row < 0 or row > cap:  # (and what does not fit 64 bits)
+        raise RuntimeError(f"{name}: row {row} of a cache of {cap}")
+    return row
+
+
 def _same_device(t: torch.Tensor, name: str, device) -> torch.Tensor:
     if t.device != device:
         raise RuntimeError(f"{name}: on {t.device}, the cache is on {device}")
@@ -640,7 +647,7 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scal
     if isinstance(offset, torch.Tensor):
         rows = _per_sequence(offset, "kv_append_q4.offset", B, dev)
     else:
-        first = int(offset)
+        first = _first_row("kv_append_q4", offset, cap)
     k_strides = _lib.strides_arg(ks)
     _lib.call("q35_kv_append_q4", k.data_ptr(), v.data_ptr(), k_strides,
               k_strides if ks == vs else _lib.strides_arg(vs), k_codes.data_ptr(), k_scales.data_ptr(),
@@ -663,7 +670,7 @@ def kv_read_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Ten
     if isinstance(start, torch.Tensor):
         starts = _per_sequence(start, "kv_read_q4.start", B, dev)
     else:
-        first = int(start)
+        first = _first_row("kv_read_q4", start, cap)
     k = torch.empty(B, Hkv, n, D, device=dev, dtype=_BF16)
     v = torch.empty_like(k)
     _lib.call("q35_kv_read_q4", k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),

@@ -131,3 +131,19 @@ def test_sizes_whose_products_overflow_are_refused():
         assert lib.q35_kv_read_q4(p, p, p, p, p, p, B, 2, S, S, 64, 32, 16, offset, None, None) == 2
     for out_cap in (HUGE, 1 << 31):
         assert lib.q35_kv_read_q4(p, p, p, p, p, p, 4, 2, 4, out_cap, 64, 32, 16, 0, None, None) == 2
+
+
+@pytest.mark.parametrize("row", [-1, 17, 1 << 32, 1 << 64, (1 << 64) + 3, -(1 << 64)])
+def test_rows_that_fit_no_cache_are_refused(monkeypatch, row):
+    """A Python int beyond 64 bits must not reach the library as another number."""
+    monkeypatch.setattr(K, "_cache_q4", lambda *a: (2, 1, 16, 32, 32))
+    monkeypatch.setattr(K, "_strided_rows", lambda t, *a: (t, t.stride()))
+    monkeypatch.setattr(K, "_stream", lambda t: None)
+    monkeypatch.setattr(K.torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(K._lib, "call", lambda *a: None)
+    cache = [torch.zeros(2, 1, 16, 16, dtype=torch.uint8)] * 4
+    x = torch.zeros(2, 1, 1, 32, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        K.kv_append_q4(x, x, *cache, row)
+    with pytest.raises(RuntimeError):
+        K.kv_read_q4(*cache, row, 1)
