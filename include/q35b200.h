@@ -500,12 +500,14 @@ Q35_API int q35_kv_read_q4(const void *k_codes, const void *k_scales, const void
  * kv head (a decode step, drafted tokens).  causal != 0: query s sees keys
  * <= s + len - Sq.  A query that sees no key gives zeros.  A kv_lens entry
  * outside [0, kv_len] is clamped and recorded as a device error (code 2, site
- * 311).  |scale| <= 2^100.  Scores need |q| and |scale q| < 2^100, and lose bits of
- * queries 2^-100 of the largest among their kv head's.  Weights and values are rounded to
- * 11 bits, values at most to 2^-15 of the largest scale of their row; rows a query sees
- * need |v| between 2^-60 and 2^100 (beyond: rounded to 0, or infinite).  A NaN reaches the
- * queries that see its row only.  workspace: fp32 scratch of q35_attn_q4_workspace(...)
- * floats, asked for with the launch's device current (q35_set_sm_limit does not matter). */
+ * 311; the expert exchange's site 311 comes with code 1).  |scale| <= 2^100.  Scores need
+ * |q| and |scale q| < 2^100, and lose bits of queries 2^-100 of the largest among their kv
+ * head's.  Weights and values are rounded to 11 bits, values at most to 2^-15 of the
+ * largest scale of their row; rows a query sees need |v| between 2^-60 and 2^100 (beyond:
+ * rounded to 0, or infinite), and rows 2^105 smaller than another, zeros counting as 2^-60,
+ * lose their weight.  A NaN reaches the queries that see its row only.  workspace: fp32
+ * scratch of q35_attn_q4_workspace(...) floats, asked for with the launch's device current
+ * (q35_set_sm_limit does not matter).                                       */
 Q35_API int64_t q35_attn_q4_workspace(int64_t B, int Hq, int Hkv, int64_t Sq, int64_t kv_len,
                                       int D);
 Q35_API int q35_attn_q4_fwd(const void *q, const void *k_codes, const void *k_scales,

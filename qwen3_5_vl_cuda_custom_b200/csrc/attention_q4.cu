@@ -42,7 +42,9 @@
 // for all groups of the key, so V is off by at most 2^-11 of itself or 2^-15 of the
 // largest s of its key (a code step is s).  Weights reach 2^15 (kLift), so they have
 // all 11 bits down to 2^-29 of the largest.
-// Visible values: |V| between 2^-60 and 2^100.
+// Visible values: |V| between 2^-60 and 2^100, rows of 0 counting as 2^-60.  Where two
+// visible rows are 2^105 apart the smaller one's weight no longer enters the sum (fp32's
+// smallest number is 2^-126, the larger one's weight 2^15): beside zeros, 2^40 is safe.
 //
 // V's operand wants pairs of neighbouring keys.  A transposing ldmatrix over the
 // codes as 16-bit units (four codes) gives exactly that: a lane receives, for two
@@ -65,11 +67,13 @@
 // are XOR-swizzled by the row, so that both the 16-byte reads of K and the 8-row
 // reads of V touch every bank once.
 //
-// Measured (32/4 heads x 128, groups of 32): 64 sequences x 8193 keys 67.8 us, 5.0 TB/s
-// (the copies alone 61; a plain copy moves 6.5 TB/s); one sequence x 131072 keys 21.7 us;
-// x 500 keys 6.6 us.  595 warp instructions per 32-key tile, issue slots 60 % busy: what
-// bounds it is copies and arithmetic together, the 16x8 matrix instructions (one per 2
-// clocks and SM) holding up the logic operations beside them.
+// Measured in a captured graph (32/4 heads x 128, groups of 32): 64 sequences x 8193 keys
+// 69.2 us, 4.9 TB/s (the copies alone 61; a plain copy moves 6.5 TB/s); one sequence x
+// 131072 keys 23.9 us; x 500 keys 7.4 us.  595 warp instructions per 32-key tile, issue
+// slots 59 % busy: what bounds it is copies and arithmetic together, the 16x8 matrix
+// instructions (one per 2 clocks and SM) holding up the logic operations beside them.
+// More than 16 query rows unpack every key again: 64 sequences x 8192 keys, 2 kv heads, 8,
+// 16, 32, 64 and 128 rows 41.8, 68.3, 96.9, 250 and 354 us.
 // Tried: P and V in bf16 (64.0 us when this form took 68.7, the errors above), P as two
 // bf16 parts (70.8, 0.0021 to 0.0023); e4m3 operands for K (emulated: 48M instructions
 // for 37M), shifts as multiplications (12 % slower), a tile's scores together with the

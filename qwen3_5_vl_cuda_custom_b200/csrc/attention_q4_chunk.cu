@@ -22,8 +22,9 @@
 //      splits as fill it, which leave fp32 partials ...
 //   4. attn_q4_splits_kernel: ... joined here.
 //
-// Measured, that chunk: 101 us (attention 80, the rest mostly operands), 0.42 of the
-// measured matrix peak; relative error 0.0018.
+// Measured, that chunk: 104 us in a captured graph, 0.41 of the measured matrix peak (one
+// by one under ncu: largest values 5.9, operands 15.1, attention 89.9, join 10.4 us);
+// relative error 0.0017.
 #include <cuda_fp16.h>
 #include <float.h>
 #include <limits.h>

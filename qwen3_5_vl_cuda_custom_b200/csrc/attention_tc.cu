@@ -489,7 +489,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // warpgroups (warps 4-7 head a, 8-11 head b) rise to 208, enough to hold a
 // whole 128-score row without spilling.  The split uses exactly the launch
 // allocation: 128 * 88 + 256 * 208 = 384 * 168 (the kernel must be built with
-// 168 registers per thread, which 384 threads and one CTA per SM give).
+// 168 registers per thread, which 384 threads and one CTA per SM give; it spills
+// 4 bytes, 16 in the fp16 form).
 constexpr int kThreads2 = 384;
 constexpr int kRegsLaunch2 = 168, kRegsCtl2 = 88, kRegsSoftmax2 = 208;
 static_assert(128 * kRegsCtl2 + 256 * kRegsSoftmax2 <= kThreads2 * kRegsLaunch2,

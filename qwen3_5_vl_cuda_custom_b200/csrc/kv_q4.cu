@@ -18,10 +18,10 @@
 //
 // Both are launched ahead of the kernel in front (4096 rows appended: 3.7, not 4.1 us).
 //
-// Measured (4 kv heads x 128): 8 x 8192 rows appended in 38.4 us, 4.4 TB/s (223
-// instructions per warp and 512 channels, 40 of them paired fp32 at half rate; issue
-// slots 68 % busy), 4096 rows 3.7 us, 64 sequences x 1 row 1.8 us; 16 x 8192 rows read in
-// 58.3 us, 6.0 TB/s.
+// Measured (4 kv heads x 128): 8 x 8192 rows appended in 39.9 us with groups of 32 or 64,
+// 39.2 with 128, 4.4 TB/s (223 instructions per warp and 512 channels, 40 of them paired
+// fp32 at half rate; issue slots 68 % busy), 4096 rows 3.7 us, 64 sequences x 1 row 1.8 us;
+// 16 x 8192 rows read in 59.0 us, 5.9 TB/s.
 #include <type_traits>
 
 #include "kv_q4.cuh"
@@ -34,7 +34,8 @@ using q4::Cache;
 constexpr int kThreads = 256;
 // A CTA prefetches its next rows while it quantises: 7 CTAs of 128 threads per SM hold
 // in registers (6, 7 and 8 CTAs: 8 x 8192 rows 39.8, 39.1 and 38.6 us, 4096 rows 4.0,
-// 4.1 and 4.4).
+// 4.1 and 4.4), but for 8 bytes of spills at head_dim 128 with groups of 32 and 64, and 64
+// with 32.
 constexpr int kAppendThreads = 128, kAppendCtas = 7;
 
 struct Rows {
@@ -113,7 +114,9 @@ __device__ __forceinline__ float code_exact(float x, float lo, float s) {
 // group's (scale, minimum).  The threads of a group are neighbours.
 //
 // The codes are the 64-bit rule's, halves included (x - m and s have few bits: one
-// channel in 500 lies exactly on a half).  With d = x - m, r within 2^-24 of 1/s and
+// channel in 500 lies exactly on a half).  The quotient is a reciprocal's, one Newton step
+// and a correction by its exact remainder (Markstein, Computation of elementary functions
+// on the IBM RISC System/6000 processor, 1990): with d = x - m, r within 2^-24 of 1/s and
 // y0 = d r, the rest d - y0 s is exact in one fma (it has at most 10 bits), so
 // y = y0 + rest r is d / s rounded to fp32, but for 2^-23 of a step.  If d is exact, it
 // is either (n + 1/2) s, then y = n + 1/2, or off by a step of d at least, which is more

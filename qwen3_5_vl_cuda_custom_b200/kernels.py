@@ -700,7 +700,13 @@ def attention_cache_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.T
     an int ``kv_len`` a chunk of a prompt goes through a temporary fp16 copy of the
     rows (512 bytes of K and V per row and kv head, against 160 stored at head_dim 128)
     and the tensor-memory attention kernels, unless there is no memory for the copy;
-    with a length per sequence chunks run on the codes too."""
+    with a length per sequence chunks run on the codes too.
+
+    Both forms keep 11 bits of the weights and of V; the chunk's copy also of K, down to
+    2^-27 of the largest row of the head, seen or not, and nothing of what is 2^-39 of
+    it.  On the codes V is exact to 2^-15 of the largest scale of its row and needs |v|
+    below 2^100 (below 2^40 beside rows of zeros).  A NaN or an infinity in a row reaches
+    the queries that see it only."""
     B, Hkv, cap, D, group = _cache_q4("attention_cache_q4", k_codes, k_scales, v_codes, v_scales)
     dev = k_codes.device
     if torch.cuda.current_device() != dev.index:  # plans and workspaces are per device
