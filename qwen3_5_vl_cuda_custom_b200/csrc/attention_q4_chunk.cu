@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) attn_q4_splits_kernel(F16Extra x, ui
     v.z = fmaf(o.z, f, v.z);
     v.w = fmaf(o.w, f, v.w);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : (1.f / kPartScale) / l;
   const int64_t bh = row / Sq, sq = row - bh * Sq, b = bh / Hq, h = bh - b * Hq;
   *reinterpret_cast<uint2 *>(out + ((b * Sq + sq) * Hq + h) * x.D + ch) =
       make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));

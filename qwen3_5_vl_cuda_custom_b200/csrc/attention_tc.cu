@@ -146,7 +146,7 @@ __device__ __forceinline__ int split_tiles(const AttnParams &p, int split, int n
   return max(0, min(n_all - j0, p.x.tiles_per_split));
 }
 // kF16 epilogue of one query row: D columns of O (read 32 at a time from TMEM by the
-// whole warp) as bf16, or as an fp32 partial with its (max in log2 units, sum).
+// whole warp) times f as bf16, or as an fp32 partial with its (max in log2 units, sum).
 // (Keys and values stored as NaN are zeros among the operands: the blocks of 32 channels
 // of a row that sees one get their NaN here.)
 __device__ __forceinline__ void store_row_f16(const AttnParams &p, uint32_t o_tm, bool some,
@@ -157,7 +157,7 @@ __device__ __forceinline__ void store_row_f16(const AttnParams &p, uint32_t o_tm
   const int *nan = p.x.nan + (static_cast<int64_t>(b) * p.Hkv + h / (p.Hq / p.Hkv)) * 4;
   const int64_t row = (static_cast<int64_t>(b) * p.Hq + h) * p.Sq + qi;
   const int64_t slot = row * p.x.splits + split;
-  const float all = p.x.part ? f : (l > 0.f ? f / l : 0.f);
+  const float all = p.x.part ? kPartScale : l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
   for (int c = 0; c < p.x.D / 32; ++c) {
     const float inv = nan[c] <= last ? NAN : all;
@@ -174,8 +174,9 @@ __device__ __forceinline__ void store_row_f16(const AttnParams &p, uint32_t o_tm
       float4 *dst = reinterpret_cast<float4 *>(p.x.part + slot * p.x.D + c * 32);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        dst[i] = make_float4(__uint_as_float(r[4 * i]) * inv, __uint_as_float(r[4 * i + 1]) * inv,
-                             __uint_as_float(r[4 * i + 2]) * inv, __uint_as_float(r[4 * i + 3]) * inv);
+        dst[i] = make_float4(
+            __uint_as_float(r[4 * i]) * inv * f, __uint_as_float(r[4 * i + 1]) * inv * f,
+            __uint_as_float(r[4 * i + 2]) * inv * f, __uint_as_float(r[4 * i + 3]) * inv * f);
     } else {
       uint4 *dst = reinterpret_cast<uint4 *>(
           p.out + ((static_cast<int64_t>(b) * p.Sq + qi) * p.Hq + h) * p.x.D + c * 32);
@@ -184,8 +185,8 @@ __device__ __forceinline__ void store_row_f16(const AttnParams &p, uint32_t o_tm
         uint32_t u[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          u[k] = pack_bf2(__uint_as_float(r[8 * i + 2 * k]) * inv,
-                          __uint_as_float(r[8 * i + 2 * k + 1]) * inv);
+          u[k] = pack_bf2(__uint_as_float(r[8 * i + 2 * k]) * inv * f,
+                          __uint_as_float(r[8 * i + 2 * k + 1]) * inv * f);
         dst[i] = make_uint4(u[0], u[1], u[2], u[3]);
       }
     }

@@ -6,6 +6,10 @@
 
 namespace q35 {
 
+// Partial sums are stored times this: they are up to 2^53 (weights to 2^15, values to 2^14,
+// 2^24 keys) times an output factor of up to 2^114, which fp32 does not hold.
+constexpr float kPartScale = 0x1p-40f;
+
 struct F16Extra {
   const float2 *scales; // [B * Hkv]: the scale in log2 units, what the output is multiplied by
   const int *nan;       // [B * Hkv][4]: first key that makes 32 output channels NaN each

@@ -267,3 +267,21 @@ def test_chunks_in_flight_together_and_again(monkeypatch):
         graph.replay()
         assert all(torch.equal(o.view(torch.int16), bits) for o in outs)
     assert want[0].isnan().any() and not want[:, :20].isnan().any()
+
+
+@pytest.mark.parametrize("chunk,top", [(True, 126), (True, 100), (True, -90), (False, 98), (False, -50)])
+@pytest.mark.parametrize("kv", [150, 9000])
+def test_large_and_small_values_in_one_run_and_in_several(monkeypatch, chunk, top, kv):
+    """Values up to 2^top: runs and splits of the keys leave partial sums in fp32, which
+    have to hold them.  Equal weights (queries of 0), so the bounds are 2^-11 for values,
+    2^-11 for weights, 2^-12 for the exponential and 2^-17 for sums, and the output's."""
+    force(monkeypatch, chunk)
+    B, Hq, Hkv, Sq, D, group = 1, 4, 2, 20, 64, 32
+    cache, _, _ = filled_cache(B, Hkv, -(-kv // 16) * 16, D, group, 151, 0.5)
+    cache[3][..., 0], cache[3][..., 1] = 2.0 ** (top - 4), 2.0 ** (top - 6)
+    vv = R.values(cache[2], cache[3])
+    q = torch.zeros(B, Hq, Sq, D, dtype=torch.bfloat16)
+    out = K().attention_cache_q4(q.to(DEV), *cache, kv, D ** -0.5, False).double().cpu()
+    ref = vv[:, :, :kv].mean(2).repeat_interleave(Hq // Hkv, 1).reshape(B, 1, Hq * D)
+    tol = ref.abs() * (2 ** -10 + 2 ** -12 + 2 ** -17 + 2 ** -8)
+    assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
