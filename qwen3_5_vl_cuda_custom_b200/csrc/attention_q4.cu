@@ -456,9 +456,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
     uint32_t qf[NT][J][4];
     uint32_t qm[NT][2];  // 2^(X-81) sum(Q_t) of group t in three bf16 parts
     int lim[NT][2];      // keys the column's query sees
-    uint32_t top = 0u;
+    uint32_t largest = 0u;  // exponent
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      uint32_t top = 0u;
       const int r = (rg * NT + nt) * 8 + g;
       const uint16_t *src = nullptr;
       if (r < p.R) {
@@ -473,10 +474,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) attn_q4_kernel(P
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = max_abs2(top, qf[nt][j][i]);
       }
+      // (an infinite query spoils its own row; the others' power of two goes by the rest)
+      const uint32_t e0 = top >> 7 & 0xffu, e1 = top >> 23 & 0xffu;
+      largest = max(largest, max(e0 == 255u ? 0u : e0, e1 == 255u ? 0u : e1));
     }
-    // (an infinite query spoils its own row; the others' power of two goes by the rest)
-    const uint32_t e0 = top >> 7 & 0xffu, e1 = top >> 23 & 0xffu;
-    const int e = __reduce_max_sync(0xffffffffu, max(e0 == 255u ? 0u : e0, e1 == 255u ? 0u : e1));
+    const int e = __reduce_max_sync(0xffffffffu, largest);
     const int up_by = max(-60, min(187 - e, 75));  // X
     const float up = __uint_as_float(static_cast<uint32_t>(127 + 52 + up_by) << 23);
     const float scale_up = p.scale_log2 * 0x1p20f *

@@ -285,3 +285,21 @@ def test_large_and_small_values_in_one_run_and_in_several(monkeypatch, chunk, to
     ref = vv[:, :, :kv].mean(2).repeat_interleave(Hq // Hkv, 1).reshape(B, 1, Hq * D)
     tol = ref.abs() * (2 ** -10 + 2 ** -12 + 2 ** -17 + 2 ** -8)
     assert ((out - ref).abs() <= tol).all(), float(((out - ref).abs() / tol).max())
+
+
+def test_an_infinite_query_among_sixteen_rows(monkeypatch):
+    """Rows of one group, eight apart: the second's largest number lies where the first
+    holds the infinity."""
+    force(monkeypatch, False)
+    B, Hq, Hkv, kv, D, group = 64, 64, 4, 4096, 64, 32
+    cache, _, _ = filled_cache(1, Hkv, kv, D, group, 153, 0.5)
+    cache = [t.repeat(B, *[1] * (t.dim() - 1)) for t in cache]
+    q = rows((B, Hq, 1, D), 154, 0.5).to(DEV)
+    q[:, 8::16] *= 2.0 ** -30
+    q[:, 8::16, :, 0] = 2.0 ** 30
+    want = K().attention_cache_q4(q, *cache, kv, 2.0 ** -27, False).view(B, Hq, D)
+    q[:, ::16, :, 0] = math.inf
+    got = K().attention_cache_q4(q, *cache, kv, 2.0 ** -27, False).view(B, Hq, D)
+    assert got[:, ::16].isnan().all() and torch.isfinite(want).all()
+    got[:, ::16] = want[:, ::16]
+    assert torch.equal(got, want)
